@@ -1,0 +1,818 @@
+// Attention over KV caches: causal prompts and trees of drafted tokens, with
+// grouped heads, over cached tokens in pages followed by new packed tokens.
+#include <cfloat>
+
+#include "attn.cuh"
+#include "kernels.cuh"
+
+namespace cb {
+namespace attn {
+namespace {
+
+constexpr int kThreads = 512;    // 2 softmax warpgroups, loaders, MMA warp
+constexpr int kMaxSlots = 12;
+
+struct FwdArgs {
+  KvSource kv;
+  const char *q;
+  int64_t q_tok, q_head;           // bytes
+  char *out;
+  int64_t o_tok, o_head;           // bytes
+  float *lse;
+  int64_t l_tok, l_head;           // elements
+  const uint8_t *mask;
+  int64_t mask_row;
+  const int32_t *plan;
+  float *part_o, *part_lse;        // [slot][row tile rows][D], [slot][rows]
+  int ctas, group, tree;
+  float scale, c;                  // c = scale * log2(e)
+};
+
+// Shared memory: the Q tile(s), a ring of K and V tiles, then this.
+struct Control {
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t done;
+  alignas(16) uint32_t valid[8][4];  // which keys of a tile there are
+  float2 ml[2][kTile];             // two-tile form: each half's (max, sum)
+  uint32_t tmem;
+  int give_up;
+  int bad_v;                       // a masked tile held inf or NaN
+};
+
+template <int D, bool kDual>
+struct Shape {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kQTiles = kDual ? 1 : 2;
+  static constexpr int kSlots = D == 128 ? (kDual ? 6 : 5) : 12;
+  static constexpr int kPending = kSlots - 2 < 6 ? kSlots - 2 : 6;
+  static constexpr int kSmem =
+      (kQTiles + kSlots) * kTileBytes + (int)sizeof(Control);
+  static_assert(kSlots <= kMaxSlots, "ring");
+  static_assert(kSmem <= 232448, "shared memory of one SM");
+};
+
+// First key tile of an item in which some row does not see every key.
+__device__ __forceinline__ int first_masked_tile(const Segment &s, int group,
+                                                 int tree) {
+  return (s.cached + (tree ? 0 : s.row0 / group + 1)) / kTile;
+}
+
+// The loader's queue of copies in flight: one cp.async group per tile.
+template <int N>
+struct Pending {
+  uint32_t bar[N];
+  uint32_t check[N];               // V tile to rid of inf and NaN, or 0
+  int n = 0;
+};
+
+// ------------------------------------------------------------------ kernel
+// Mathematics.  Row r of an item is (token i, head g of the group): s_rj =
+// scale q_r . k_j over the visible keys j, o_r = sum_j softmax_j(s_rj) v_j,
+// in one pass over the key tiles with a running maximum m and sum l per row.
+// The heads of a group are rows of one item, so K and V are read once per
+// group.  S = Q K^T and O += P V run on tcgen05 with 128-row tiles: S, P and
+// O stay in TMEM, P (rounded to the inputs' 16 bits, as an MMA operand must
+// be; its sum l is taken in FP32 before the rounding) overwrites its own S,
+// and a thread owns one row, so no reduction crosses threads.  O is rescaled
+// only when a row's maximum grew by more than 2^8 (P and l then exceed 1 by
+// at most that, far inside both types' ranges).
+//
+// Two forms.  More than 128 rows: two row tiles share each K and V tile and
+// take turns (one's MMAs run under the other's exponentials).  Up to 128
+// rows (decode): one row tile, and the two warpgroups take alternate key
+// tiles, each with its own m, l and O, joined in the epilogue.
+template <int D, bool kBf16, bool kDual>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_fwd_kernel(const __grid_constant__ FwdArgs a) {
+  using Sh = Shape<D, kDual>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sm_q = smem_u32(smem);
+  const uint32_t sm_ring = sm_q + Sh::kQTiles * Sh::kTileBytes;
+  Control &ct = *reinterpret_cast<Control *>(
+      smem + (Sh::kQTiles + Sh::kSlots) * Sh::kTileBytes);
+  volatile int *give_up = &ct.give_up;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (sm_q & 1023) {               // the swizzle needs 1024-byte alignment
+    if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1u);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Sh::kSlots; ++i) {
+      mbar_init(smem_u32(&ct.full[i]), 4);
+      mbar_init(smem_u32(&ct.empty[i]), 1);
+    }
+    mbar_init(smem_u32(&ct.q_full), 4);
+    mbar_init(smem_u32(&ct.q_empty), 1);
+    mbar_init(smem_u32(&ct.done), 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(smem_u32(&ct.s_full[w]), 1);
+      mbar_init(smem_u32(&ct.p_full[w]), 4);
+      mbar_init(smem_u32(&ct.o_full[w]), 1);
+    }
+    ct.give_up = 0;
+    ct.bad_v = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) tc_alloc(smem_u32(&ct.tmem), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ct.tmem;
+
+  const Segment *segs =
+      reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
+  const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
+
+  if (warp < 8) {
+    // ------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int w = warp >> 2;                       // warpgroup
+    const int rt = (warp & 3) * 32 + lane;         // row of the tile
+    const int r = (kDual ? 0 : w * kTile) + rt;    // row of the item
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tm_s = lane_base + w * 128;
+    const uint32_t tm_o = lane_base + 256 + w * 128;
+    const float grow = 8.f / a.c;                  // allowed growth of m
+    uint32_t s_phase = 0, o_phase = 0, o_phase2 = 0;
+    int tiles_done = 0;
+    for (int si = seg_begin; si < seg_end; ++si) {
+      const Segment sg = segs[si];
+      const int n_end = kDual ? sg.t1 : (w ? sg.n1 : sg.n0);
+      const int t_all = kDual ? sg.t1 : max(sg.n0, sg.n1);
+      const int t_first = kDual ? sg.t0 + w : sg.t0;
+      const bool warp_on = r - lane < sg.rows;
+      const bool row_on = r < sg.rows;
+      const int tok = (sg.row0 + r) / a.group;
+      const int head = sg.hk * a.group + (sg.row0 + r) - tok * a.group;
+      // causal: keys below lim are visible; tree: cached ones and the mask's
+      const int lim =
+          !row_on ? 0 : a.tree ? sg.cached : sg.cached + tok + 1;
+      const int masked_from = first_masked_tile(sg, a.group, a.tree);
+      const uint8_t *mrow =
+          a.tree && row_on ? a.mask + (int64_t)(sg.tok0 + tok) * a.mask_row
+                           : nullptr;
+      float m = -INFINITY, l = 0.f;
+      bool seen = false, first = true;
+      for (int t = t_first; t < n_end; t += kDual ? 2 : 1) {
+        mbar_wait(smem_u32(&ct.s_full[w]), s_phase, give_up);
+        s_phase ^= 1;
+        if (warp_on) {
+          tc_fence_after();
+          uint32_t x[4][32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tc_ld32(x[i], tm_s + i * 32);
+          const uint4 vw = *reinterpret_cast<const uint4 *>(
+              ct.valid[(tiles_done + t - sg.t0) & 7]);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tc_hold(x[i]);
+          const bool partial =
+              (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu || t >= masked_from;
+          if (partial) {
+            const uint32_t words[4] = {vw.x, vw.y, vw.z, vw.w};
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j0 = t * kTile + i * 32;
+              const int nvis = min(max(lim - j0, 0), 32);
+              uint32_t vis = nvis == 32 ? 0xffffffffu : (1u << nvis) - 1;
+              if (mrow != nullptr && j0 + 32 > sg.cached) {
+                const int e = min(j0 + 32, sg.cached + sg.n_new);
+                for (int j = max(j0, sg.cached); j < e; ++j)
+                  if (mrow[j - sg.cached]) vis |= 1u << (j - j0);
+              }
+              vis &= words[i];
+              any |= vis;
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((vis >> e) & 1)) x[i][e] = 0xff800000u;  // -inf
+            }
+            seen |= any != 0;
+          } else {
+            seen = true;
+          }
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v0 = __uint_as_float(x[i][0]);
+            float v1 = __uint_as_float(x[i][1]);
+#pragma unroll
+            for (int e = 2; e < 32; e += 2) {
+              v0 = fmaxf(v0, __uint_as_float(x[i][e]));
+              v1 = fmaxf(v1, __uint_as_float(x[i][e + 1]));
+            }
+            mx[i] = fmaxf(v0, v1);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // m == -inf: any finite top is growth
+          if (__any_sync(0xffffffffu, top > m + grow)) {
+            const float m_new = fmaxf(m, top);
+            if (!first) {
+              const float f =
+                  m == -INFINITY ? (l == 0.f ? 1.f : 0.f)
+                                 : ex2((m - m_new) * a.c);
+              l *= f;
+#pragma unroll 1
+              for (int i = 0; i < D / 16; ++i) {
+                uint32_t o[16];
+                tc_ld16(o, tm_o + i * 16);
+                tc_wait_ld();
+                tc_hold(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc_st16(tm_o + i * 16, o);
+              }
+            }
+            m = m_new;
+          }
+          first = false;
+          const float mc = m == -INFINITY ? 0.f : m * a.c;
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float y0 =
+                  ex2(fmaf(__uint_as_float(x[i][2 * e]), a.c, -mc));
+              const float y1 =
+                  ex2(fmaf(__uint_as_float(x[i][2 * e + 1]), a.c, -mc));
+              s0 += y0;
+              s1 += y1;
+              p[e] = pack16<kBf16>(y0, y1);
+            }
+            tc_st16(tm_s + i * 16, p);
+          }
+          l += s0 + s1;
+          tc_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ct.p_full[w]));
+      }
+      tiles_done += t_all - sg.t0;
+
+      // ---------------------------------------------------- epilogue
+      const bool steps = n_end > t_first;
+      bool steps2 = false;                 // the other half's, two-tile form
+      float m2 = -INFINITY, l2 = 0.f;
+      if (kDual) {
+        steps2 = w ? true : sg.t1 > sg.t0 + 1;
+        ct.ml[w][rt] = make_float2(m, seen && l == 0.f ? -1.f : l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float2 other = ct.ml[w ^ 1][rt];
+        m2 = other.x;
+        l2 = other.y;
+        if (l2 == -1.f) {
+          seen = true;
+          l2 = 0.f;
+        }
+      }
+      if (steps) {
+        mbar_wait(smem_u32(&ct.o_full[w]), o_phase, give_up);
+        o_phase ^= 1;
+      }
+      if (kDual && steps2) {
+        mbar_wait(smem_u32(&ct.o_full[w ^ 1]), o_phase2, give_up);
+        o_phase2 ^= 1;
+      }
+      tc_fence_after();
+      if (warp_on) {
+        float mm = kDual ? fmaxf(m, m2) : m;
+        const float mc = mm == -INFINITY ? 0.f : mm * a.c;
+        // a half whose maximum is -inf holds no weight (or NaN, which stays)
+        float f1 = 1.f, f2 = 0.f, lsum = l;
+        if (kDual) {
+          f1 = m == -INFINITY ? (l == 0.f ? 0.f : l) : ex2(m * a.c - mc);
+          f2 = m2 == -INFINITY ? (l2 == 0.f ? 0.f : l2) : ex2(m2 * a.c - mc);
+          lsum = l * f1 + l2 * f2;
+        }
+        const bool empty = lsum == 0.f;
+        float inv = empty ? 0.f : 1.f / lsum;
+        const float fill = empty && seen ? NAN : 0.f;
+        const float lse =
+            empty ? -INFINITY : mm * a.scale + logf(lsum);
+        f1 *= inv;
+        f2 *= inv;
+        if (!steps || empty) f1 = 0.f;
+        if (!kDual || !steps2 || empty) f2 = 0.f;
+        const bool fix = ct.bad_v != 0;
+        // two-tile form: each warpgroup writes half of the columns
+        constexpr int kCols = kDual ? D / 2 : D;
+        const int c_base = kDual ? w * kCols : 0;
+        const int64_t prow =
+            (int64_t)sg.part * (Sh::kQTiles * kTile) + r;
+        char *orow = a.out + (int64_t)(sg.tok0 + tok) * a.o_tok +
+                     (int64_t)head * a.o_head;
+#pragma unroll 1
+        for (int cb0 = 0; cb0 < kCols; cb0 += 32) {
+          const int col = c_base + cb0;
+          float o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = fill;
+          uint32_t u[32];
+          if (steps) {
+            tc_ld32(u, tm_o + col);
+            tc_wait_ld();
+            tc_hold(u);
+            if (f1 != 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
+            }
+          }
+          if (kDual && steps2) {
+            tc_ld32(u, lane_base + 256 + (w ^ 1) * 128 + col);
+            tc_wait_ld();
+            tc_hold(u);
+            if (f2 != 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
+            }
+          }
+          if (row_on) {
+            if (fix) {
+              // Masked tiles went in with inf and NaN as zeros; rows that
+              // see such a value get it back here.
+              const int jend = min(n_end * kTile, sg.cached + sg.n_new);
+              const int last = kDual ? min(sg.t1 * kTile,
+                                           sg.cached + sg.n_new)
+                                     : jend;
+              for (int j = max(sg.t0, masked_from) * kTile; j < last; ++j) {
+                const char *vp;
+                if (j < sg.cached) {
+                  const int id = page_of(a.kv, sg.b, j);
+                  if (id < 0) continue;
+                  vp = a.kv.vp + id * a.kv.vp_page + sg.hk * a.kv.vp_head +
+                       (j % a.kv.page) * a.kv.vp_tok;
+                } else {
+                  if (mrow != nullptr ? !mrow[j - sg.cached] : j >= lim)
+                    continue;
+                  vp = a.kv.v + (int64_t)(sg.tok0 + j - sg.cached) *
+                                    a.kv.v_tok +
+                       sg.hk * a.kv.v_head;
+                }
+                for (int e = 0; e < 32; ++e) {
+                  const uint16_t bits =
+                      reinterpret_cast<const uint16_t *>(vp)[col + e];
+                  const uint16_t ex = kBf16 ? 0x7f80 : 0x7c00;
+                  if ((bits & ex) != ex) continue;
+                  const uint16_t mant = kBf16 ? 0x007f : 0x03ff;
+                  o[e] += (bits & mant) ? NAN
+                          : (bits & 0x8000) ? -INFINITY
+                                            : INFINITY;
+                }
+              }
+            }
+            if (sg.part >= 0) {
+              float4 *dst = reinterpret_cast<float4 *>(
+                  a.part_o + prow * D + col);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2],
+                                     o[4 * e + 3]);
+            } else {
+              uint4 *dst = reinterpret_cast<uint4 *>(orow + col * 2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                dst[e] = make_uint4(
+                    pack16<kBf16>(o[8 * e], o[8 * e + 1]),
+                    pack16<kBf16>(o[8 * e + 2], o[8 * e + 3]),
+                    pack16<kBf16>(o[8 * e + 4], o[8 * e + 5]),
+                    pack16<kBf16>(o[8 * e + 6], o[8 * e + 7]));
+            }
+          }
+        }
+        if (row_on && (!kDual || w == 0)) {
+          if (sg.part >= 0)
+            a.part_lse[prow] = lse;
+          else
+            a.lse[(int64_t)(sg.tok0 + tok) * a.l_tok +
+                  (int64_t)head * a.l_head] = lse;
+        }
+      }
+      tc_fence_before();
+      if (kDual) asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------- loaders
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    constexpr int kChunks = D / 8;                 // 16-byte chunks of a row
+    constexpr int kRowsPer = 32 / kChunks;         // rows per warp step
+    const int lw = warp - 8;
+    const int chunk = lane % kChunks, sub_row = lane / kChunks;
+    Pending<Sh::kPending> pend;
+    uint32_t item = 0, q_phase = 1;
+
+    // Chunk `chunk` of row `row` of a tile, in the 128-byte swizzle.
+    auto place = [&](int row) {
+      return (uint32_t)((chunk >> 3) * (kTile * 128) + row * 128 +
+                        (((chunk & 7) ^ (row & 7)) << 4));
+    };
+    auto signal = [&](uint32_t bar, uint32_t check) {
+      if (check) {
+        // A masked tile: a key some rows do not see must not reach them
+        // through 0 * inf, so inf and NaN go in as zeros (and are added
+        // back for the rows that see them in the epilogue).
+        const uint32_t ex = kBf16 ? 0x7f807f80u : 0x7c007c00u;
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          const uint32_t at = check + place(lw * 32 + i * kRowsPer + sub_row);
+          uint32_t v[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(at)
+                       : "memory");
+          uint32_t bad = 0;
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = v[e] & ex;
+            uint32_t keep = 0;
+            if ((x & 0xffffu) != (ex & 0xffffu)) keep |= 0xffffu;
+            if ((x >> 16) != (ex >> 16)) keep |= 0xffff0000u;
+            bad |= ~keep;
+            v[e] &= keep;
+          }
+          if (bad) {
+            ct.bad_v = 1;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                         : "memory");
+          }
+        }
+      }
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto flush = [&]() {
+      cp_async_wait<0>();
+#pragma unroll
+      for (int i = 0; i < Sh::kPending; ++i)
+        if (i < pend.n) signal(pend.bar[i], pend.check[i]);
+      pend.n = 0;
+    };
+    // Waits for a free place; what is in flight is handed over first when
+    // that takes long, since the consumers may be waiting for it.
+    auto wait_free = [&](uint32_t bar, uint32_t parity) {
+      if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
+      flush();
+      mbar_wait(bar, parity, give_up);
+      __syncwarp();
+    };
+    auto push = [&](uint32_t bar, uint32_t check) {
+      cp_async_commit();
+      if (pend.n == Sh::kPending) {
+        cp_async_wait<Sh::kPending>();
+        signal(pend.bar[0], pend.check[0]);
+#pragma unroll
+        for (int i = 0; i + 1 < Sh::kPending; ++i) {
+          pend.bar[i] = pend.bar[i + 1];
+          pend.check[i] = pend.check[i + 1];
+        }
+        pend.n = Sh::kPending - 1;
+      }
+#pragma unroll
+      for (int i = 0; i < Sh::kPending; ++i)
+        if (i == pend.n) {
+          pend.bar[i] = bar;
+          pend.check[i] = check;
+        }
+      ++pend.n;
+    };
+    // One tile: lane `i` of the warp holds the address of its row i (0: the
+    // row is not there and reads as zeros).
+    auto copy_rows = [&](uint32_t dst, const char *row_ptr) {
+#pragma unroll
+      for (int i = 0; i < 32 / kRowsPer; ++i) {
+        const int rl = i * kRowsPer + sub_row;
+        const uint64_t p =
+            __shfl_sync(0xffffffffu, (uint64_t)row_ptr, rl);
+        const char *src = p ? (const char *)p + chunk * 16 : a.q;
+        cp_async16(dst + place(lw * 32 + rl), src, p ? 16 : 0);
+      }
+    };
+
+    uint32_t tile_no = 0;
+    for (int si = seg_begin; si < seg_end; ++si) {
+      const Segment sg = segs[si];
+      const int t_all = kDual ? sg.t1 : max(sg.n0, sg.n1);
+      const int masked_from = first_masked_tile(sg, a.group, a.tree);
+      // Q
+      wait_free(smem_u32(&ct.q_empty), q_phase);
+      q_phase ^= 1;
+      for (int qt = 0; qt < Sh::kQTiles; ++qt) {
+        const int r = qt * kTile + lw * 32 + lane;
+        const char *src = nullptr;
+        if (r < sg.rows) {
+          const int tok = (sg.row0 + r) / a.group;
+          const int head =
+              sg.hk * a.group + (sg.row0 + r) - tok * a.group;
+          src = a.q + (int64_t)(sg.tok0 + tok) * a.q_tok +
+                (int64_t)head * a.q_head;
+        }
+        copy_rows(sm_q + qt * Sh::kTileBytes, src);
+      }
+      push(smem_u32(&ct.q_full), 0);
+      // K and V tiles
+      const int total = sg.cached + sg.n_new;
+      auto page_at = [&](int t) {        // the page of this lane's key
+        const int key = t * kTile + lw * 32 + lane;
+        return key < sg.cached ? page_of(a.kv, sg.b, key) : -1;
+      };
+      int page = page_at(sg.t0);
+      for (int t = sg.t0; t < t_all; ++t) {
+        const int key = t * kTile + lw * 32 + lane;
+        const char *kp = nullptr, *vp = nullptr;
+        if (key < sg.cached) {
+          if (page >= 0) {
+            const int off = key % a.kv.page;
+            kp = a.kv.kp + page * a.kv.kp_page + sg.hk * a.kv.kp_head +
+                 off * a.kv.kp_tok;
+            vp = a.kv.vp + page * a.kv.vp_page + sg.hk * a.kv.vp_head +
+                 off * a.kv.vp_tok;
+          }
+        } else if (key < total) {
+          const int64_t n = sg.tok0 + key - sg.cached;
+          kp = a.kv.k + n * a.kv.k_tok + sg.hk * a.kv.k_head;
+          vp = a.kv.v + n * a.kv.v_tok + sg.hk * a.kv.v_head;
+        }
+        if (t + 1 < t_all) page = page_at(t + 1);
+        const uint32_t there = __ballot_sync(0xffffffffu, kp != nullptr);
+        {
+          const uint32_t slot = item % Sh::kSlots;
+          const uint32_t ph = (item / Sh::kSlots) & 1;
+          wait_free(smem_u32(&ct.empty[slot]), ph ^ 1);
+          if (lane == 0) ct.valid[tile_no & 7][lw] = there;
+          copy_rows(sm_ring + slot * Sh::kTileBytes, kp);
+          push(smem_u32(&ct.full[slot]), 0);
+          ++item;
+        }
+        {
+          const uint32_t slot = item % Sh::kSlots;
+          const uint32_t ph = (item / Sh::kSlots) & 1;
+          const uint32_t dst = sm_ring + slot * Sh::kTileBytes;
+          wait_free(smem_u32(&ct.empty[slot]), ph ^ 1);
+          copy_rows(dst, vp);
+          push(smem_u32(&ct.full[slot]), t >= masked_from ? dst : 0);
+          ++item;
+        }
+        ++tile_no;
+      }
+    }
+    flush();
+  } else {
+    // ------------------------------------------------------------ MMA
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 12 && lane == 0) {
+      constexpr uint32_t id_qk = mma_idesc(kBf16, kTile, false);
+      constexpr uint32_t id_pv = mma_idesc(kBf16, D, true);
+      uint32_t base = 0, q_phase = 0;
+      uint32_t p_phase[2] = {0, 0};
+      auto wait_item = [&](uint32_t item) {
+        const uint32_t slot = item % Sh::kSlots;
+        mbar_wait(smem_u32(&ct.full[slot]), (item / Sh::kSlots) & 1, give_up);
+        return slot;
+      };
+      for (int si = seg_begin; si < seg_end; ++si) {
+        const Segment *sp = segs + si;
+        const int t0 = sp->t0;
+        const int n0 = kDual ? sp->t1 : sp->n0, n1 = kDual ? sp->t1 : sp->n1;
+        const int t_all = max(n0, n1);
+        // steps in order: (tile t, buffer w); w = row tile, or, in the
+        // two-tile form, the parity of the key tile
+        int left = kDual ? t_all - t0 : max(n0 - t0, 0) + max(n1 - t0, 0);
+        auto qk = [&](int t, int w) {
+          const uint32_t it = base + 2 * (t - t0);
+          const uint32_t slot = wait_item(it);
+          tc_fence_after();
+          const uint32_t q = sm_q + (kDual ? 0 : w * Sh::kTileBytes);
+          const uint32_t k = sm_ring + slot * Sh::kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
+            mma_ss(tmem + w * 128, tile_desc(q + off, 0),
+                   tile_desc(k + off, 0), id_qk, kk != 0);
+          }
+          const bool last = kDual || w == (t < n1 ? 1 : 0);
+          if (last) tc_commit(smem_u32(&ct.empty[slot]));
+          tc_commit(smem_u32(&ct.s_full[w]));
+          if (--left == 0) tc_commit(smem_u32(&ct.q_empty));
+        };
+        mbar_wait(smem_u32(&ct.q_full), q_phase, give_up);
+        q_phase ^= 1;
+        if (kDual) {
+          qk(t0, 0);
+          if (t0 + 1 < t_all) qk(t0 + 1, 1);
+        } else {
+          if (t0 < n0) qk(t0, 0);
+          if (t0 < n1) qk(t0, 1);
+        }
+        for (int t = t0; t < t_all; ++t) {
+          const uint32_t it_v = base + 2 * (t - t0) + 1;
+#pragma unroll
+          for (int h = 0; h < (kDual ? 1 : 2); ++h) {
+            const int w = kDual ? (t - t0) & 1 : h;
+            const int n_end = w ? n1 : n0;
+            if (!kDual && t >= n_end) continue;
+            const uint32_t slot = wait_item(it_v);
+            mbar_wait(smem_u32(&ct.p_full[w]), w ? p_phase[1] : p_phase[0],
+                      give_up);
+            if (w)
+              p_phase[1] ^= 1;
+            else
+              p_phase[0] ^= 1;
+            tc_fence_after();
+            const uint32_t v = sm_ring + slot * Sh::kTileBytes;
+            const bool fresh = kDual ? t < t0 + 2 : t == t0;
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
+                     tile_desc(v + kk * 2048, kTile * 128), id_pv,
+                     !(fresh && kk == 0));
+            const bool last_use = kDual || w == (t < n1 ? 1 : 0);
+            if (last_use) tc_commit(smem_u32(&ct.empty[slot]));
+            const int t_next = t + (kDual ? 2 : 1);
+            if (t_next < n_end)
+              qk(t_next, w);
+            else
+              tc_commit(smem_u32(&ct.o_full[w]));
+          }
+        }
+        base += 2 * (t_all - t0);
+      }
+      // TMEM is freed only when no MMA is in flight.
+      tc_commit(smem_u32(&ct.done));
+      int gave_up = 0;
+      mbar_wait(smem_u32(&ct.done), 0, &gave_up);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partial results of items that several CTAs worked on: one warp
+// per row, weights exp(lse_p - max lse), in the order of the parts.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256)
+    attn_merge_kernel(const __grid_constant__ FwdArgs a, const Merge *merges,
+                      int slot_rows) {
+  const Merge mg = merges[blockIdx.y];
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= mg.rows) return;
+  const int64_t row0 = (int64_t)mg.part0 * slot_rows + r;
+  float top = -INFINITY;
+  for (int p = lane; p < mg.parts; p += 32)
+    top = fmaxf(top, a.part_lse[row0 + (int64_t)p * slot_rows]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr int kPer = D / 32;
+  float acc[kPer] = {}, total = 0.f;
+  for (int p = 0; p < mg.parts; ++p) {
+    const int64_t row = row0 + (int64_t)p * slot_rows;
+    const float lse = a.part_lse[row];
+    // a part without weight counts only when no part has any (its value is
+    // then 0, or NaN where keys were seen but none had weight)
+    const float wgt = top == -INFINITY ? (lse == -INFINITY ? 1.f : lse)
+                                       : __expf(lse - top);
+    if (lse == -INFINITY && top != -INFINITY) continue;
+    if (top != -INFINITY || lse != lse) total += wgt;
+    const float *src = a.part_o + row * D + lane * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] = fmaf(src[e], wgt, acc[e]);
+  }
+  const float inv = top == -INFINITY ? 1.f : 1.f / total;
+  const int tok = (mg.row0 + r) / a.group;
+  const int head = mg.hk * a.group + (mg.row0 + r) - tok * a.group;
+  char *dst = a.out + (int64_t)(mg.tok0 + tok) * a.o_tok +
+              (int64_t)head * a.o_head + lane * kPer * 2;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2)
+    *reinterpret_cast<uint32_t *>(dst + e * 2) =
+        pack16<kBf16>(acc[e] * inv, acc[e + 1] * inv);
+  if (lane == 0)
+    a.lse[(int64_t)(mg.tok0 + tok) * a.l_tok + (int64_t)head * a.l_head] =
+        top == -INFINITY ? (total != total ? NAN : -INFINITY)
+                         : top + logf(total);
+}
+
+template <int D, bool kBf16, bool kDual>
+int run_fwd(const FwdArgs &a, const cascade_attn_plan_info_t &p,
+            cudaStream_t s) {
+  using Sh = Shape<D, kDual>;
+  auto *kernel = attn_fwd_kernel<D, kBf16, kDual>;
+  // setmaxnreg hands the launch's registers from the loaders and the MMA
+  // warps to the softmax warps: 256 x 200 + 128 x 72 + 128 x 40 = 512 x 128.
+  // A launch with fewer would wait for ever, so it is refused.
+  cudaFuncAttributes fa;
+  CB_CUDA(cudaFuncGetAttributes(&fa, kernel));
+  CB_CHECK(fa.numRegs == 128, CASCADE_ERR_UNSUPPORTED,
+           "attention kernel built with an unexpected register count");
+  CB_CUDA(cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+  kernel<<<p.ctas, kThreads, Sh::kSmem, s>>>(a);
+  count_launches(1);
+  CB_CUDA(cudaGetLastError());
+  if (p.merges > 0) {
+    const Merge *merges = reinterpret_cast<const Merge *>(
+        a.plan + seg_offset(p.ctas) + (int64_t)p.segments * 16);
+    const dim3 grid((unsigned)div_up(p.merge_rows, 8), (unsigned)p.merges);
+    attn_merge_kernel<D, kBf16>
+        <<<grid, 256, 0, s>>>(a, merges, Sh::kQTiles * kTile);
+    count_launches(1);
+    CB_CUDA(cudaGetLastError());
+  }
+  return CASCADE_OK;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace cb
+
+extern "C" int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
+                                    const cascade_attn_args_t *args,
+                                    void *stream) {
+  using namespace cb::attn;
+  cb::clear_error();
+  CB_CHECK(plan && args, CASCADE_ERR_INVALID, "null pointer argument");
+  const cascade_attn_plan_info_t &p = *plan;
+  CB_CHECK(p.kind == CASCADE_ATTN_FORWARD, CASCADE_ERR_INVALID,
+           "the plan is not one for attention");
+  CB_CHECK(args->dtype == CASCADE_KV_FP16 || args->dtype == CASCADE_KV_BF16,
+           CASCADE_ERR_INVALID, "dtype must be FP16 or BF16");
+  int rc = check_args(p, *args, true);
+  if (rc != CASCADE_OK || p.segments == 0) return rc;
+  CB_CHECK(args->out && args->lse, CASCADE_ERR_INVALID,
+           "null pointer argument");
+  CB_CHECK((((uintptr_t)args->out | (uint64_t)(args->out_tok * 2) |
+             (uint64_t)(args->out_head * 2)) &
+            15) == 0,
+           CASCADE_ERR_INVALID, "out must have 16-byte aligned rows");
+  CB_CHECK(!p.tree || args->mask, CASCADE_ERR_INVALID,
+           "a plan for trees needs a mask");
+  CB_CHECK(args->workspace_bytes >= p.workspace_bytes &&
+               (p.workspace_bytes == 0 || args->workspace),
+           CASCADE_ERR_INVALID, "workspace too small");
+  FwdArgs a{};
+  fill_source(*args, p, &a.kv);
+  a.q = static_cast<const char *>(args->q);
+  a.q_tok = args->q_tok * 2;
+  a.q_head = args->q_head * 2;
+  a.out = static_cast<char *>(args->out);
+  a.o_tok = args->out_tok * 2;
+  a.o_head = args->out_head * 2;
+  a.lse = args->lse;
+  a.l_tok = args->lse_tok;
+  a.l_head = args->lse_head;
+  a.mask = args->mask;
+  a.mask_row = args->mask_row;
+  a.plan = args->plan;
+  const int64_t rows = (int64_t)p.parts * p.row_tile;
+  a.part_o = static_cast<float *>(args->workspace);
+  a.part_lse = a.part_o + rows * p.head_dim;
+  a.ctas = p.ctas;
+  a.group = p.q_heads / p.kv_heads;
+  a.tree = p.tree;
+  a.scale = args->scale;
+  a.c = args->scale * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf = args->dtype == CASCADE_KV_BF16;
+  const bool dual = p.row_tile == kTile;
+  if (p.head_dim == 128) {
+    if (dual)
+      return bf ? run_fwd<128, true, true>(a, p, s)
+                : run_fwd<128, false, true>(a, p, s);
+    return bf ? run_fwd<128, true, false>(a, p, s)
+              : run_fwd<128, false, false>(a, p, s);
+  }
+  if (dual)
+    return bf ? run_fwd<64, true, true>(a, p, s)
+              : run_fwd<64, false, true>(a, p, s);
+  return bf ? run_fwd<64, true, false>(a, p, s)
+            : run_fwd<64, false, false>(a, p, s);
+}
+
+extern "C" int cascade_diag_attn_timeouts(uint64_t *count) {
+  using namespace cb::attn;
+  cb::clear_error();
+  CB_CHECK(count, CASCADE_ERR_INVALID, "null pointer argument");
+  void *mine = nullptr;
+  CB_CUDA(cudaGetSymbolAddress(&mine, g_timeouts));
+  const unsigned int *other = weights_timeouts_symbol();
+  CB_CHECK(other, CASCADE_ERR_CUDA, "no device symbol");
+  unsigned int v[2] = {0, 0};
+  CB_CUDA(cudaMemcpy(&v[0], mine, 4, cudaMemcpyDeviceToHost));
+  CB_CUDA(cudaMemcpy(&v[1], other, 4, cudaMemcpyDeviceToHost));
+  *count = (uint64_t)v[0] + v[1];
+  return CASCADE_OK;
+}

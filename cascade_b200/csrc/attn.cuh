@@ -1,0 +1,291 @@
+// Device pieces shared by the attention kernels (sm_100a): mbarriers with
+// bounded waits, tcgen05 / TMEM access, cp.async, and the records that the
+// host-side plan hands to the kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace cb {
+namespace attn {
+
+// ------------------------------------------------------------------ plan
+// The plan buffer is int32: [0, ctas] the first segment of each CTA (and the
+// end), padded to 16 ints, then the segments, then the merges.
+struct Segment {      // one CTA's consecutive work on one item
+  int tok0;           // the sequence's first packed token
+  int n_new;          // its new tokens
+  int cached;         // its cached tokens
+  int b;              // its row of the page table
+  int hk;             // key/value head
+  int row0;           // first row of the item (row = token * group + head)
+  int t0, t1;         // attention: key tiles; weights: row chunks
+  int part;           // partial slot, or -1 when the item is whole
+  int n0, n1;         // attention: end of the key tiles of either row tile
+  int rows;           // attention: rows of the item
+  int key0;           // weights: first key of the item
+  int fill;           // weights: the item ends its sequence's keys
+  int pad[2];
+};
+static_assert(sizeof(Segment) == 64, "segments are 16 ints");
+
+struct Merge {        // one item that several CTAs worked on
+  int tok0, hk, row0;
+  int rows;           // attention: rows of the item; weights: keys there are
+  int part0, parts;
+  int b, key0;
+};
+static_assert(sizeof(Merge) == 32, "merges are 8 ints");
+
+constexpr int kTile = 128;       // keys of a key tile, rows of a row tile
+
+inline __host__ __device__ int seg_offset(int ctas) {
+  return (ctas + 1 + 15) / 16 * 16;
+}
+
+// --------------------------------------------------------- PTX wrappers
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar),
+               "r"(count)
+               : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Waits of this source file's kernels that gave up, on this device.
+static __device__ unsigned int g_timeouts;
+
+// A wait on another role of the same CTA.  Every role's loops are finite and
+// no address depends on data that a wait guards, so a wait that runs out
+// (two seconds) sets the CTA's flag, lets every later wait of the CTA
+// through, and the kernel ends by itself.
+__device__ __forceinline__ void mbar_wait_slow(uint32_t bar,
+                                                   uint32_t parity,
+                                                   volatile int *give_up) {
+  uint64_t t0 = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try(bar, parity)) return;
+    if ((n & 63) == 0) {
+      if (*give_up) return;
+      uint64_t t;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t0 == 0) t0 = t;
+      if (t - t0 > 2000000000ull) {
+        *give_up = 1;
+        atomicAdd(&g_timeouts, 1u);
+        return;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity,
+                                          volatile int *give_up) {
+  if (mbar_try(bar, parity)) return;
+  mbar_wait_slow(bar, parity, give_up);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src,
+                                           uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(
+                   dst),
+               "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Generic-proxy writes to shared memory become visible to tcgen05.mma.
+__device__ __forceinline__ void fence_async_proxy() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_alloc(uint32_t smem_dst, uint32_t cols) {
+  asm volatile(
+      "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+          smem_dst),
+      "r"(cols)
+      : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ void tc_dealloc(uint32_t tmem, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(
+                   tmem),
+               "r"(cols)
+               : "memory");
+}
+// Arrives on `bar` once every tcgen05.mma this thread issued has finished.
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 "
+      "[%0];" ::"r"(bar)
+      : "memory");
+}
+
+// D[128 x N] (+)= A[128 x 16] B[16 x N], A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b,
+                                       uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// The same with A in TMEM (two 16-bit values a column, one row a lane).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b,
+                                       uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(
+          d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+// Shared-memory matrix descriptor of a tile in the 128-byte swizzle: rows of
+// 64 16-bit values (128 bytes), 8-row groups 1024 bytes apart, further
+// 64-value column blocks `lbo` bytes apart (used when the rows run along K).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lbo >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// kind::f16 instruction descriptor: 128 x n, FP32 accumulator; `mn_b` when
+// B's rows run along K (its columns are contiguous).
+__host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int n,
+                                                 bool mn_b) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) |
+         ((mn_b ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTile >> 4) << 24);
+}
+
+#define CB_R8(x, i)                                                          \
+  "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]),                \
+      "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
+#define CB_I8(x, i)                                                          \
+  "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]),     \
+      "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
+#define CB_K8(x, i)                                                          \
+  "+r"(x[i]), "+r"(x[i + 1]), "+r"(x[i + 2]), "+r"(x[i + 3]),                \
+      "+r"(x[i + 4]), "+r"(x[i + 5]), "+r"(x[i + 6]), "+r"(x[i + 7])
+
+// 32 consecutive columns of this warp's 32 lanes; complete after tc_wait_ld.
+__device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : CB_R8(x, 0), CB_R8(x, 8), CB_R8(x, 16), CB_R8(x, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_ld16(uint32_t (&x)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : CB_R8(x, 0), CB_R8(x, 8)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr,
+                                        const uint32_t (&x)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::CB_I8(x, 0),
+      CB_I8(x, 8), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// Keeps uses of the loaded values behind the wait that completes them.
+__device__ __forceinline__ void tc_hold(uint32_t (&x)[32]) {
+  asm volatile("" : CB_K8(x, 0), CB_K8(x, 8), CB_K8(x, 16), CB_K8(x, 24));
+}
+__device__ __forceinline__ void tc_hold(uint32_t (&x)[16]) {
+  asm volatile("" : CB_K8(x, 0), CB_K8(x, 8));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two floats to two 16-bit values in one word, to nearest even.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (kBf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// ---------------------------------------------------- where a key's row is
+struct KvSource {
+  const char *k, *v;               // new tokens, packed
+  int64_t k_tok, k_head, v_tok, v_head;               // strides in bytes
+  const char *kp, *vp;             // pages
+  int64_t kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok;
+  const int32_t *table;
+  int64_t table_row;               // entries between rows of the table
+  int32_t page, pages;             // tokens of a page, pages there are
+};
+
+// Checks of a call's pointers, alignment and strides (host).
+int check_args(const cascade_attn_plan_info_t &p,
+               const cascade_attn_args_t &a, bool forward);
+void fill_source(const cascade_attn_args_t &a,
+                 const cascade_attn_plan_info_t &p, KvSource *s);
+
+unsigned int *weights_timeouts_symbol();
+
+// Page of cached token `key` of sequence b, or -1 when the table names none.
+__device__ __forceinline__ int page_of(const KvSource &s, int b, int key) {
+  const int id = __ldg(s.table + (int64_t)b * s.table_row + key / s.page);
+  return id >= 0 && id < s.pages ? id : -1;
+}
+
+}  // namespace attn
+}  // namespace cb

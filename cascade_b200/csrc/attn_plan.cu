@@ -1,0 +1,383 @@
+// The host side of the attention operators: plans (which CTA does which part
+// of a batch) and the checks of a call's arguments.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <queue>
+#include <vector>
+
+#include "attn.cuh"
+
+namespace cb {
+namespace attn {
+
+int check_args(const cascade_attn_plan_info_t &p,
+               const cascade_attn_args_t &a, bool forward) {
+  CB_CHECK(p.segments == 0 || a.plan, CASCADE_ERR_INVALID,
+           "null pointer argument");
+  CB_CHECK(((uintptr_t)a.plan & 15) == 0 &&
+               ((uintptr_t)a.workspace & 15) == 0,
+           CASCADE_ERR_INVALID,
+           "the plan and the workspace must be 16-byte aligned");
+  CB_CHECK(std::isfinite(a.scale) && a.scale > 0.f, CASCADE_ERR_INVALID,
+           "scale must be finite and above 0");
+  uint64_t bits = (uintptr_t)a.q | (uintptr_t)a.k;
+  int64_t strides = a.q_tok | a.q_head | a.k_tok | a.k_head;
+  if (forward) {
+    bits |= (uintptr_t)a.v;
+    strides |= a.v_tok | a.v_head;
+  }
+  CB_CHECK(p.tokens == 0 || (a.q && a.k && (a.v || !forward)),
+           CASCADE_ERR_INVALID, "null pointer argument");
+  if (p.max_cached > 0) {
+    CB_CHECK(a.k_pages && a.table && (a.v_pages || !forward) && a.pages >= 0,
+             CASCADE_ERR_INVALID, "cached tokens need pages and a table");
+    bits |= (uintptr_t)a.k_pages;
+    strides |= a.kp_page | a.kp_head | a.kp_tok;
+    if (forward) {
+      bits |= (uintptr_t)a.v_pages;
+      strides |= a.vp_page | a.vp_head | a.vp_tok;
+    }
+  }
+  CB_CHECK((bits & 15) == 0 && (strides & 7) == 0, CASCADE_ERR_INVALID,
+           "rows of q, k, v and the pages must start on 16-byte boundaries");
+  return CASCADE_OK;
+}
+
+void fill_source(const cascade_attn_args_t &a,
+                 const cascade_attn_plan_info_t &p, KvSource *s) {
+  s->k = static_cast<const char *>(a.k);
+  s->v = static_cast<const char *>(a.v);
+  s->k_tok = a.k_tok * 2;
+  s->k_head = a.k_head * 2;
+  s->v_tok = a.v_tok * 2;
+  s->v_head = a.v_head * 2;
+  s->kp = static_cast<const char *>(a.k_pages);
+  s->vp = static_cast<const char *>(a.v_pages);
+  s->kp_page = a.kp_page * 2;
+  s->kp_head = a.kp_head * 2;
+  s->kp_tok = a.kp_tok * 2;
+  s->vp_page = a.vp_page * 2;
+  s->vp_head = a.vp_head * 2;
+  s->vp_tok = a.vp_tok * 2;
+  s->table = a.table;
+  s->table_row = a.table_row;
+  s->page = p.page_size > 0 ? p.page_size : 1;
+  s->pages = a.pages;
+}
+
+namespace {
+
+struct Item {
+  Segment seg;       // t0, t1: its whole range of units
+  int units() const { return seg.t1 - seg.t0; }
+};
+
+// Time per unit (a key tile, or a chunk of rows) and per segment, and what a
+// merge costs, in nanoseconds.  They decide between splits only; results do
+// not depend on them beyond the order in which partial sums are joined.
+struct Costs {
+  double unit, unit_bytes, segment, merge, part_bytes;
+};
+
+constexpr double kBytesPerNs = 6200;       // HBM, all SMs together
+
+std::vector<std::vector<Segment>> whole_items(const std::vector<Item> &items,
+                                              int ctas, const Costs &c,
+                                              double *makespan) {
+  std::vector<int> order(items.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
+    return items[x].units() > items[y].units();
+  });
+  ctas = (int)std::min<size_t>(ctas, items.size());
+  std::vector<std::vector<Segment>> out(ctas);
+  using Load = std::pair<double, int>;
+  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> heap;
+  for (int i = 0; i < ctas; ++i) heap.push({0.0, i});
+  const double unit =
+      std::max(c.unit, c.unit_bytes * ctas / kBytesPerNs);
+  *makespan = 0;
+  for (int i : order) {
+    Load l = heap.top();
+    heap.pop();
+    l.first += items[i].units() * unit + c.segment;
+    *makespan = std::max(*makespan, l.first);
+    out[l.second].push_back(items[i].seg);
+    heap.push(l);
+  }
+  return out;
+}
+
+// Cuts the items, laid end to end, into `ctas` equal runs.
+std::vector<std::vector<Segment>> equal_runs(const std::vector<Item> &items,
+                                             int ctas, const Costs &c,
+                                             bool fwd,
+                                             std::vector<Merge> *merges,
+                                             int *parts) {
+  const double ov = c.segment / c.unit;
+  double total = 0;
+  for (const Item &it : items) total += it.units() + ov;
+  const double quota = total / ctas;
+  std::vector<std::vector<Segment>> out(ctas);
+  double pos = 0;
+  int cta = 0;
+  std::vector<std::pair<int, size_t>> pieces;       // (CTA, its segment)
+  for (const Item &it : items) {
+    const int units = it.units();
+    int done = 0;
+    pieces.clear();
+    do {
+      // units of this item in front of the end of this CTA's run
+      const double room = (cta + 1) * quota - pos - ov / 2;
+      int end = units;
+      if (cta < ctas - 1)
+        end = (int)std::lround(
+            std::min(std::max(room, (double)done), (double)units));
+      if (end > done || units == 0) {
+        Segment s = it.seg;
+        s.t0 = it.seg.t0 + done;
+        s.t1 = it.seg.t0 + end;
+        pieces.push_back({cta, out[cta].size()});
+        out[cta].push_back(s);
+        done = end;
+      }
+      if (done < units) ++cta;
+    } while (done < units);
+    if (pieces.size() > 1) {
+      Merge m{};
+      m.tok0 = it.seg.tok0;
+      m.hk = it.seg.hk;
+      m.row0 = it.seg.row0;
+      m.rows = fwd ? it.seg.rows : it.seg.n_new + it.seg.cached;
+      m.part0 = *parts;
+      m.parts = (int)pieces.size();
+      m.b = it.seg.b;
+      m.key0 = it.seg.key0;
+      merges->push_back(m);
+      for (const auto &at : pieces) out[at.first][at.second].part = (*parts)++;
+    }
+    pos += units + ov;
+    while (cta < ctas - 1 && pos >= (cta + 1) * quota) ++cta;
+  }
+  return out;
+}
+
+int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
+              const int32_t *n_cached, int32_t *buf, size_t capacity) {
+  cascade_attn_plan_info_t &p = *info;
+  const bool fwd = p.kind == CASCADE_ATTN_FORWARD;
+  const int group = p.q_heads / p.kv_heads;
+  const int sms = p.sms > 0 ? p.sms : sm_count();
+  int64_t tokens = 0;
+  int max_new = 0, max_cached = 0, max_keys = 0;
+  for (int b = 0; b < p.batch; ++b) {
+    const int c = n_cached ? n_cached[b] : 0;
+    CB_CHECK(n_new[b] >= 0 && c >= 0, CASCADE_ERR_INVALID,
+             "lengths must not be negative");
+    CB_CHECK((int64_t)n_new[b] + c <= (1 << 30), CASCADE_ERR_INVALID,
+             "a sequence has at most 2^30 tokens");
+    CB_CHECK((int64_t)n_new[b] * group <= (1 << 30), CASCADE_ERR_INVALID,
+             "a sequence has at most 2^30 query rows");
+    tokens += n_new[b];
+    max_new = std::max(max_new, n_new[b]);
+    max_cached = std::max(max_cached, c);
+    max_keys = std::max(max_keys, n_new[b] + c);
+  }
+  CB_CHECK(tokens <= (1 << 30), CASCADE_ERR_INVALID,
+           "at most 2^30 packed tokens");
+  CB_CHECK(max_cached == 0 || p.page_size > 0, CASCADE_ERR_INVALID,
+           "cached tokens need a page size");
+  p.tokens = tokens;
+  p.max_new = max_new;
+  p.max_cached = max_cached;
+  p.max_keys = max_keys;
+  p.table_cols =
+      p.page_size > 0 ? (int)div_up(max_cached, p.page_size) : 0;
+  // Up to 128 rows fit one row tile: the form for decode.
+  const int row_tile =
+      !fwd || (int64_t)max_new * group > kTile ? 2 * kTile : kTile;
+  p.row_tile = row_tile;
+
+  std::vector<Item> items;
+  int64_t count = 0, tok0 = 0;
+  for (int b = 0; b < p.batch; ++b) {
+    const int64_t keys = (int64_t)n_new[b] + (n_cached ? n_cached[b] : 0);
+    count += (int64_t)p.kv_heads *
+             (fwd ? (int64_t)div_up((uint64_t)n_new[b] * group, row_tile)
+                  : std::max<int64_t>(1, (int64_t)div_up(keys, row_tile)));
+  }
+  CB_CHECK(count <= (1 << 24), CASCADE_ERR_INVALID,
+           "the batch is too large for one call");
+  items.reserve(count);
+  for (int b = 0; b < p.batch; ++b) {
+    const int n = n_new[b], c = n_cached ? n_cached[b] : 0;
+    for (int hk = 0; hk < p.kv_heads; ++hk) {
+      Item it{};
+      it.seg.tok0 = (int)tok0;
+      it.seg.n_new = n;
+      it.seg.cached = c;
+      it.seg.b = b;
+      it.seg.hk = hk;
+      it.seg.part = -1;
+      if (fwd) {
+        const int rows = n * group;
+        // key tiles that the rows up to `last` (not included) see
+        auto tiles = [&](int last) {
+          const int keys = c + (p.tree ? n : (last - 1) / group + 1);
+          return (int)div_up(keys, kTile);
+        };
+        for (int r = 0; r < rows; r += row_tile) {
+          it.seg.row0 = r;
+          it.seg.rows = std::min(row_tile, rows - r);
+          it.seg.t0 = 0;
+          it.seg.n0 = tiles(std::min(rows, r + kTile));
+          it.seg.n1 =
+              it.seg.rows > kTile ? tiles(std::min(rows, r + row_tile)) : 0;
+          it.seg.t1 = std::max(it.seg.n0, it.seg.n1);
+          items.push_back(it);
+        }
+      } else {
+        const int w = std::min(n, p.window);
+        it.seg.row0 = n - w;              // first token that counts
+        it.seg.rows = w * group;
+        const int chunks = (int)div_up((uint64_t)it.seg.rows, kTile);
+        const int keys = c + n;
+        int key = 0;
+        do {
+          // rows of tokens before key - cached see none of these keys
+          const int64_t first =
+              std::max<int64_t>(0, (int64_t)key - c - it.seg.row0);
+          it.seg.key0 = key;
+          it.seg.t0 = std::min<int64_t>(chunks, first * group / kTile);
+          it.seg.t1 = chunks;
+          it.seg.fill = key + row_tile >= keys;
+          items.push_back(it);
+          key += row_tile;
+        } while (key < keys);
+      }
+    }
+    tok0 += n;
+  }
+
+  // Time of a unit measured on a B200 (D = 128): a key tile against 256 rows
+  // is bound by the exponentials and the MMAs; against one row tile by the
+  // latency of one step, or by HBM once all SMs read.
+  Costs cost{};
+  const double tile_bytes = 2.0 * kTile * p.head_dim;
+  if (fwd) {
+    cost.unit = row_tile == kTile ? 600 : 1400;
+    cost.unit_bytes = row_tile == kTile ? 2 * tile_bytes : 0;
+    cost.segment = 1500;
+    cost.part_bytes = 8.0 * (p.head_dim + 1) *
+                      std::min<int64_t>(row_tile, (int64_t)max_new * group);
+  } else {
+    const int64_t rows = (int64_t)std::min(max_new, p.window) * group;
+    cost.unit = 200 + 1000.0 * std::min<int64_t>(rows, kTile) / kTile;
+    cost.unit_bytes = 0;
+    cost.segment = 1500;
+    cost.part_bytes = 8.0 * row_tile;
+  }
+  cost.merge = 3500;
+
+  std::vector<std::vector<Segment>> best;
+  std::vector<Merge> merges;
+  int parts = 0;
+  if (!items.empty()) {
+    double t_best;
+    best = whole_items(items, sms, cost, &t_best);
+    double units = 0;
+    int most = 0;
+    for (const Item &it : items) {
+      units += it.units();
+      most = std::max(most, it.units());
+    }
+    // Runs of equal length over n CTAs; worth it where whole items leave
+    // SMs idle, and splitting needs something to split.
+    int n_best = 0;
+    if (most > 1) {
+      for (int n = sms; n >= 2; n = n * 3 / 4) {
+        if (units < n) continue;
+        const double unit =
+            std::max(cost.unit, cost.unit_bytes * n / kBytesPerNs);
+        const double t = (units * unit + items.size() * cost.segment) / n +
+                         cost.segment + cost.merge +
+                         2.0 * n * cost.part_bytes / 4000.0;
+        if (t < t_best * 0.97) {
+          t_best = t;
+          n_best = n;
+        }
+      }
+    }
+    if (n_best) best = equal_runs(items, n_best, cost, fwd, &merges, &parts);
+  }
+  size_t segments = 0;
+  for (const auto &v : best) segments += v.size();
+  const size_t ints = (size_t)seg_offset((int)best.size()) + segments * 16 +
+                      merges.size() * 8;
+  CB_CHECK(ints <= (size_t)INT32_MAX, CASCADE_ERR_INVALID,
+           "the batch is too large for one call");
+  p.ints = (int)ints;
+  p.ctas = (int)best.size();
+  p.segments = (int)segments;
+  p.parts = parts;
+  p.merges = (int)merges.size();
+  p.merge_rows = 0;
+  for (const Merge &m : merges)
+    p.merge_rows = std::max(p.merge_rows, fwd ? m.rows : row_tile);
+  p.workspace_bytes =
+      (uint64_t)parts * row_tile * (fwd ? p.head_dim + 1 : 1) * 4;
+  if (ints > capacity || !buf) return CASCADE_OK;
+  std::memset(buf, 0, ints * 4);
+  Segment *out = reinterpret_cast<Segment *>(buf + seg_offset(p.ctas));
+  int at = 0;
+  for (int c = 0; c < p.ctas; ++c) {
+    buf[c] = at;
+    for (Segment s : best[c]) {
+      if (fwd) {
+        s.n0 = std::max(s.t0, std::min(s.n0, s.t1));
+        s.n1 = std::max(s.t0, std::min(s.n1, s.t1));
+      }
+      out[at++] = s;
+    }
+  }
+  buf[p.ctas] = at;
+  if (!merges.empty())
+    std::memcpy(out + at, merges.data(), merges.size() * sizeof(Merge));
+  return CASCADE_OK;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace cb
+
+extern "C" int cascade_attn_plan(cascade_attn_plan_info_t *info,
+                                 const int32_t *new_lengths,
+                                 const int32_t *cached_lengths, int32_t *out,
+                                 size_t capacity) {
+  cb::clear_error();
+  CB_CHECK(info, CASCADE_ERR_INVALID, "null pointer argument");
+  const cascade_attn_plan_info_t &p = *info;
+  CB_CHECK(p.kind == CASCADE_ATTN_FORWARD || p.kind == CASCADE_ATTN_WEIGHTS,
+           CASCADE_ERR_INVALID, "unknown kind of plan");
+  CB_CHECK(p.batch >= 0 && (p.batch == 0 || new_lengths),
+           CASCADE_ERR_INVALID, "bad batch");
+  CB_CHECK(p.head_dim == 64 || p.head_dim == 128, CASCADE_ERR_INVALID,
+           "head_dim must be 64 or 128");
+  CB_CHECK(p.kv_heads > 0 && p.q_heads > 0 && p.q_heads % p.kv_heads == 0 &&
+               p.q_heads <= 65536,
+           CASCADE_ERR_INVALID,
+           "q_heads must be a multiple of kv_heads");
+  CB_CHECK(p.page_size >= 0 && p.sms >= 0, CASCADE_ERR_INVALID,
+           "bad page size or SM count");
+  CB_CHECK(p.kind == CASCADE_ATTN_FORWARD || p.window > 0,
+           CASCADE_ERR_INVALID, "window must be above 0");
+  try {
+    return cb::attn::make_plan(info, new_lengths, cached_lengths, out,
+                               capacity);
+  } catch (const std::bad_alloc &) {
+    cb::set_error("out of host memory for the plan");
+    return CASCADE_ERR_NOMEM;
+  }
+}

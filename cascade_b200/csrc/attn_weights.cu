@@ -1,0 +1,420 @@
+// Attention weight of every key: the sum over query rows of exp(s - lse).
+#include "attn.cuh"
+#include "kernels.cuh"
+
+namespace cb {
+namespace attn {
+namespace {
+
+constexpr int kWThreads = 416;     // 2 x 4 summing warps, 4 loaders, MMA
+constexpr int kKeys = 2 * kTile;   // keys of an item
+constexpr int kKSlots = 2, kQSlots = 3;
+
+struct WeightArgs {
+  KvSource kv;
+  const char *q;
+  int64_t q_tok, q_head;           // bytes
+  const float *lse;
+  int64_t l_tok, l_head;
+  const float *before;
+  int64_t b_seq, b_head;
+  float *out;
+  int64_t o_seq, o_head;
+  const int32_t *plan;
+  float *part;                     // [slot][256]
+  int ctas, group, width, fill;
+  float c;                         // scale * log2(e)
+};
+
+struct WControl {
+  alignas(16) float lse2[kQSlots][kTile];      // lse of a chunk's rows, in powers of two
+  uint64_t k_full[kKSlots], k_empty[kKSlots];
+  uint64_t q_full[kQSlots], q_empty[kQSlots];
+  uint64_t s_full[2][2], s_empty[2][2];
+  uint64_t done;
+  uint32_t tmem;
+  int give_up;
+};
+
+template <int D>
+constexpr int weights_smem() {
+  return (2 * kKSlots + kQSlots) * kTile * D * 2 + (int)sizeof(WControl);
+}
+static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
+
+// Mathematics.  w_j = sum over the rows r that see key j of
+// exp(scale k_j . q_r - lse_r).  The product is formed transposed, S^T =
+// K Q^T, with 128 keys as the rows of a tcgen05 tile: a thread owns one key
+// and adds along its own row, so the sum over the rows of all heads of a
+// group needs no reduction across threads and no atomics, and its order is
+// fixed.  256 keys stay resident while chunks of up to 128 query rows
+// stream by; a decode step's few rows are one chunk of N = 16, 32, ...
+// columns, and the keys stream.  Key j is seen by the rows of tokens from j
+// on, so a thread's mask is one row number.  A chunk's sum is taken by
+// itself before it joins the total.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kWThreads, 1)
+    attn_weights_kernel(const __grid_constant__ WeightArgs a) {
+  constexpr int kTileBytes = kTile * D * 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sm_k = smem_u32(smem);
+  const uint32_t sm_q = sm_k + 2 * kKSlots * kTileBytes;
+  WControl &ct = *reinterpret_cast<WControl *>(
+      smem + (2 * kKSlots + kQSlots) * kTileBytes);
+  volatile int *give_up = &ct.give_up;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (sm_k & 1023) {
+    if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1u);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kKSlots; ++i) {
+      mbar_init(smem_u32(&ct.k_full[i]), 4);
+      mbar_init(smem_u32(&ct.k_empty[i]), 1);
+    }
+    for (int i = 0; i < kQSlots; ++i) {
+      mbar_init(smem_u32(&ct.q_full[i]), 4);
+      mbar_init(smem_u32(&ct.q_empty[i]), 9);   // the MMAs and 8 warps
+    }
+    for (int w = 0; w < 2; ++w)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&ct.s_full[w][i]), 1);
+        mbar_init(smem_u32(&ct.s_empty[w][i]), 4);
+      }
+    mbar_init(smem_u32(&ct.done), 1);
+    ct.give_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) tc_alloc(smem_u32(&ct.tmem), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ct.tmem;
+
+  const Segment *segs =
+      reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
+  const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
+
+  if (warp < 8) {
+    // ---------------------------------------------------------- sums
+    const int w = warp >> 2;
+    const int kt = w * kTile + (warp & 3) * 32 + lane;   // key of the item
+    const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
+    uint32_t chunk_no = 0;
+    for (int si = seg_begin; si < seg_end; ++si) {
+      const Segment sg = segs[si];
+      const int total = sg.cached + sg.n_new;
+      const int key = sg.key0 + kt;
+      bool there = key < total;
+      if (there && key < sg.cached) there = page_of(a.kv, sg.b, key) >= 0;
+      const int64_t wi = (int64_t)sg.hk;
+      float prev = 0.f;
+      if (key < total && a.before != nullptr)
+        prev = a.before[sg.b * a.b_seq + wi * a.b_head + key];
+      // rows from `from` on see this key
+      const int64_t from =
+          (int64_t)(key - sg.cached - sg.row0) * a.group;
+      float sum = 0.f;
+      for (int ch = sg.t0; ch < sg.t1; ++ch, ++chunk_no) {
+        const uint32_t buf = chunk_no & 1, slot = chunk_no % kQSlots;
+        const int n = min(kTile, sg.rows - ch * kTile);
+        mbar_wait(smem_u32(&ct.s_full[w][buf]), (chunk_no >> 1) & 1, give_up);
+        tc_fence_after();
+        const float4 *l4 = reinterpret_cast<const float4 *>(ct.lse2[slot]);
+        const int64_t hidden = from - (int64_t)ch * kTile;
+        const bool whole = __all_sync(0xffffffffu, hidden <= 0);
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < n; i += 32) {
+          uint32_t x[32];
+          tc_ld32(x, tm + buf * 128 + i);
+          tc_wait_ld();
+          tc_hold(x);
+          if (!whole || i + 32 > n) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;  // -inf
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 l = l4[i / 4 + e];
+            s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
+            s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
+            s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
+            s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&ct.s_empty[w][buf]));
+          mbar_arrive(smem_u32(&ct.q_empty[slot]));
+        }
+        sum += (s0 + s1) + (s2 + s3);
+      }
+      if (!there) sum = 0.f;
+      if (sg.part >= 0)
+        a.part[(int64_t)sg.part * kKeys + kt] = sum;
+      else if (key < total)
+        a.out[sg.b * a.o_seq + wi * a.o_head + key] = prev + sum;
+      if (sg.fill && a.fill)
+        for (int k = total + kt; k < a.width; k += kKeys)
+          a.out[sg.b * a.o_seq + wi * a.o_head + k] =
+              a.before != nullptr
+                  ? a.before[sg.b * a.b_seq + wi * a.b_head + k]
+                  : 0.f;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------- loaders
+    constexpr int kChunks = D / 8;
+    constexpr int kRowsPer = 32 / kChunks;
+    constexpr int kPending = 3;
+    const int lw = warp - 8;
+    const int chunk = lane % kChunks, sub_row = lane / kChunks;
+    uint32_t pend[kPending];
+    int n_pend = 0;
+    uint32_t k_no = 0, q_no = 0;
+    auto place = [&](int row) {
+      return (uint32_t)((chunk >> 3) * (kTile * 128) + row * 128 +
+                        (((chunk & 7) ^ (row & 7)) << 4));
+    };
+    auto signal = [&](uint32_t bar) {
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto flush = [&]() {
+      cp_async_wait<0>();
+#pragma unroll
+      for (int i = 0; i < kPending; ++i)
+        if (i < n_pend) signal(pend[i]);
+      n_pend = 0;
+    };
+    auto wait_free = [&](uint32_t bar, uint32_t parity) {
+      if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
+      flush();
+      mbar_wait(bar, parity, give_up);
+      __syncwarp();
+    };
+    auto push = [&](uint32_t bar) {
+      cp_async_commit();
+      if (n_pend == kPending) {
+        cp_async_wait<kPending>();
+        signal(pend[0]);
+#pragma unroll
+        for (int i = 0; i + 1 < kPending; ++i) pend[i] = pend[i + 1];
+        n_pend = kPending - 1;
+      }
+#pragma unroll
+      for (int i = 0; i < kPending; ++i)
+        if (i == n_pend) pend[i] = bar;
+      ++n_pend;
+    };
+    auto copy_rows = [&](uint32_t dst, const char *row_ptr) {
+#pragma unroll
+      for (int i = 0; i < 32 / kRowsPer; ++i) {
+        const int rl = i * kRowsPer + sub_row;
+        const uint64_t p =
+            __shfl_sync(0xffffffffu, (uint64_t)row_ptr, rl);
+        const char *src = p ? (const char *)p + chunk * 16 : a.q;
+        cp_async16(dst + place(lw * 32 + rl), src, p ? 16 : 0);
+      }
+    };
+    for (int si = seg_begin; si < seg_end; ++si) {
+      const Segment sg = segs[si];
+      if (sg.t0 >= sg.t1) continue;
+      const int total = sg.cached + sg.n_new;
+      const char *kp[2] = {nullptr, nullptr};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = sg.key0 + h * kTile + lw * 32 + lane;
+        if (key < sg.cached) {
+          const int page = page_of(a.kv, sg.b, key);
+          if (page >= 0)
+            kp[h] = a.kv.kp + page * a.kv.kp_page + sg.hk * a.kv.kp_head +
+                    (key % a.kv.page) * a.kv.kp_tok;
+        } else if (key < total) {
+          kp[h] = a.kv.k + (int64_t)(sg.tok0 + key - sg.cached) * a.kv.k_tok +
+                  sg.hk * a.kv.k_head;
+        }
+      }
+      {
+        const uint32_t slot = k_no % kKSlots;
+        wait_free(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1);
+        copy_rows(sm_k + 2 * slot * kTileBytes, kp[0]);
+        copy_rows(sm_k + (2 * slot + 1) * kTileBytes, kp[1]);
+        push(smem_u32(&ct.k_full[slot]));
+        ++k_no;
+      }
+      for (int ch = sg.t0; ch < sg.t1; ++ch, ++q_no) {
+        const uint32_t slot = q_no % kQSlots;
+        const int n = min(kTile, sg.rows - ch * kTile);
+        const int r = lw * 32 + lane;
+        const char *src = nullptr;
+        float l2 = INFINITY;                  // a row that counts for nothing
+        if (r < n) {
+          const int row = ch * kTile + r;
+          const int tok = row / a.group;
+          const int64_t head = sg.hk * a.group + row - tok * a.group;
+          const int64_t at = (int64_t)sg.tok0 + sg.row0 + tok;
+          src = a.q + at * a.q_tok + head * a.q_head;
+          const float l = a.lse[at * a.l_tok + head * a.l_head];
+          l2 = l == -INFINITY ? INFINITY : l * kLog2e;
+        }
+        wait_free(smem_u32(&ct.q_empty[slot]), ((q_no / kQSlots) & 1) ^ 1);
+        ct.lse2[slot][r] = l2;
+        // the MMA reads the rows up to the next multiple of 32
+        if (lw * 32 < n) copy_rows(sm_q + slot * kTileBytes, src);
+        push(smem_u32(&ct.q_full[slot]));
+      }
+    }
+    flush();
+  } else {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0) {
+      uint32_t k_no = 0, chunk_no = 0;
+      for (int si = seg_begin; si < seg_end; ++si) {
+        const int t0 = segs[si].t0, t1 = segs[si].t1, rows = segs[si].rows;
+        if (t0 >= t1) continue;
+        const uint32_t ks = k_no % kKSlots;
+        mbar_wait(smem_u32(&ct.k_full[ks]), (k_no / kKSlots) & 1, give_up);
+        ++k_no;
+        for (int ch = t0; ch < t1; ++ch, ++chunk_no) {
+          const uint32_t buf = chunk_no & 1, slot = chunk_no % kQSlots;
+          const int n = min(kTile, (rows - ch * kTile + 31) / 32 * 32);
+          const uint32_t idesc = mma_idesc(kBf16, n, false);
+          mbar_wait(smem_u32(&ct.q_full[slot]), (chunk_no / kQSlots) & 1,
+                    give_up);
+          const uint32_t q = sm_q + slot * kTileBytes;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            mbar_wait(smem_u32(&ct.s_empty[w][buf]),
+                      ((chunk_no >> 1) & 1) ^ 1, give_up);
+            tc_fence_after();
+            const uint32_t k = sm_k + (2 * ks + w) * kTileBytes;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
+              mma_ss(tmem + w * 256 + buf * 128, tile_desc(k + off, 0),
+                     tile_desc(q + off, 0), idesc, kk != 0);
+            }
+            tc_commit(smem_u32(&ct.s_full[w][buf]));
+          }
+          tc_commit(smem_u32(&ct.q_empty[slot]));
+        }
+        tc_commit(smem_u32(&ct.k_empty[ks]));
+      }
+      tc_commit(smem_u32(&ct.done));
+      int gave_up = 0;
+      mbar_wait(smem_u32(&ct.done), 0, &gave_up);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
+  }
+}
+
+// Adds the partial sums of items that several CTAs worked on, in order.
+__global__ void __launch_bounds__(kKeys)
+    weights_merge_kernel(const __grid_constant__ WeightArgs a,
+                         const Merge *merges) {
+  const Merge mg = merges[blockIdx.x];
+  const int key = mg.key0 + threadIdx.x;
+  if (key >= mg.rows) return;
+  float sum = 0.f;
+  for (int p = 0; p < mg.parts; ++p)
+    sum += a.part[(int64_t)(mg.part0 + p) * kKeys + threadIdx.x];
+  float prev = 0.f;
+  if (a.before != nullptr)
+    prev = a.before[mg.b * a.b_seq + (int64_t)mg.hk * a.b_head + key];
+  a.out[mg.b * a.o_seq + (int64_t)mg.hk * a.o_head + key] = prev + sum;
+}
+
+template <int D, bool kBf16>
+int run_weights(const WeightArgs &a, const cascade_attn_plan_info_t &p,
+                cudaStream_t s) {
+  auto *kernel = attn_weights_kernel<D, kBf16>;
+  constexpr int smem = weights_smem<D>();
+  CB_CUDA(cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<p.ctas, kWThreads, smem, s>>>(a);
+  count_launches(1);
+  CB_CUDA(cudaGetLastError());
+  if (p.merges > 0) {
+    const Segment *segs =
+        reinterpret_cast<const Segment *>(a.plan + seg_offset(p.ctas));
+    const Merge *merges = reinterpret_cast<const Merge *>(segs + p.segments);
+    weights_merge_kernel<<<p.merges, kKeys, 0, s>>>(a, merges);
+    count_launches(1);
+    CB_CUDA(cudaGetLastError());
+  }
+  return CASCADE_OK;
+}
+
+}  // namespace
+
+unsigned int *weights_timeouts_symbol() {
+  void *p = nullptr;
+  return cudaGetSymbolAddress(&p, g_timeouts) == cudaSuccess
+             ? static_cast<unsigned int *>(p)
+             : nullptr;
+}
+
+}  // namespace attn
+}  // namespace cb
+
+extern "C" int cascade_attn_weights(const cascade_attn_plan_info_t *plan,
+                                    const cascade_attn_args_t *args,
+                                    void *stream) {
+  using namespace cb::attn;
+  cb::clear_error();
+  CB_CHECK(plan && args, CASCADE_ERR_INVALID, "null pointer argument");
+  const cascade_attn_plan_info_t &p = *plan;
+  CB_CHECK(p.kind == CASCADE_ATTN_WEIGHTS, CASCADE_ERR_INVALID,
+           "the plan is not one for attention weights");
+  CB_CHECK(args->dtype == CASCADE_KV_FP16 || args->dtype == CASCADE_KV_BF16,
+           CASCADE_ERR_INVALID, "dtype must be FP16 or BF16");
+  int rc = check_args(p, *args, false);
+  if (rc != CASCADE_OK || p.segments == 0) return rc;
+  CB_CHECK(args->weights && (p.tokens == 0 || args->lse),
+           CASCADE_ERR_INVALID, "null pointer argument");
+  CB_CHECK(args->width >= p.max_keys, CASCADE_ERR_INVALID,
+           "rows of weights are shorter than the longest sequence");
+  CB_CHECK(!args->add || args->before, CASCADE_ERR_INVALID,
+           "null pointer argument");
+  CB_CHECK(args->workspace_bytes >= p.workspace_bytes &&
+               (p.workspace_bytes == 0 || args->workspace),
+           CASCADE_ERR_INVALID, "workspace too small");
+  WeightArgs a{};
+  fill_source(*args, p, &a.kv);
+  a.q = static_cast<const char *>(args->q);
+  a.q_tok = args->q_tok * 2;
+  a.q_head = args->q_head * 2;
+  a.lse = args->lse;
+  a.l_tok = args->lse_tok;
+  a.l_head = args->lse_head;
+  a.before = args->add ? args->before : nullptr;
+  a.b_seq = args->before_seq;
+  a.b_head = args->before_head;
+  a.out = args->weights;
+  a.o_seq = args->weights_seq;
+  a.o_head = args->weights_head;
+  a.plan = args->plan;
+  a.part = static_cast<float *>(args->workspace);
+  a.ctas = p.ctas;
+  a.group = p.q_heads / p.kv_heads;
+  a.width = args->width;
+  a.fill = args->fill;
+  a.c = args->scale * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf = args->dtype == CASCADE_KV_BF16;
+  if (p.head_dim == 128)
+    return bf ? run_weights<128, true>(a, p, s)
+              : run_weights<128, false>(a, p, s);
+  return bf ? run_weights<64, true>(a, p, s) : run_weights<64, false>(a, p, s);
+}

@@ -1,0 +1,407 @@
+// Eviction from KV caches: which tokens to keep by their accumulated
+// attention weight, and the gather that makes the shorter caches.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace cb {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kDigit = 8, kBins = 1 << kDigit;
+constexpr int kHeld = 40960;       // weights of a slice held in shared memory
+
+struct SelectArgs {
+  const float *w;
+  int64_t stride[3];               // elements, of the three row dimensions
+  int dim1, dim2;                  // rows are (i0 * dim1 + i1) * dim2 + i2
+  const int32_t *lengths;          // per i0, or null: all `width`
+  int width, budget, recent, sink;
+  int32_t *keep;                   // [rows][budget]
+};
+
+struct SelectShared {
+  uint32_t hist[kBins * 32];       // one counter per bin and lane
+  uint32_t bins[2][kBins];         // this CTA's totals, read by the cluster
+  uint32_t above[kSelWarps], equal[kSelWarps];
+  uint32_t cta[2];                 // (above, equal) of this CTA's slice
+  uint32_t digit, left;
+};
+
+// Unsigned integers in the order of the weights: -0 equals 0, and NaN ranks
+// with -inf, below every number.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  uint32_t u = __float_as_uint(w);
+  if (w != w) u = 0xff800000u;
+  if (u == 0x80000000u) u = 0;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One cluster per row of weights; each CTA takes one slice of the row.  The
+// need-th largest weight is found digit by digit (4 x 8 bits): every lane of
+// a warp counts into its own column of the histogram, so equal weights (a
+// row of zeros, the common case after a long prompt) cost no more than
+// different ones; the counts of the cluster's CTAs are added over
+// distributed shared memory.  Then one ordered pass writes the positions
+// above that weight, and the lowest positions of those equal to it.
+__global__ void __launch_bounds__(kSelThreads)
+    evict_select_kernel(const __grid_constant__ SelectArgs a) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks();
+  const int rank = (int)cluster.block_rank();
+  extern __shared__ __align__(16) uint8_t raw[];
+  SelectShared &sh = *reinterpret_cast<SelectShared *>(raw);
+  float *held = reinterpret_cast<float *>(raw + sizeof(SelectShared));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t row = blockIdx.x / ranks;
+  const int i2 = (int)(row % a.dim2);
+  const int i1 = (int)(row / a.dim2 % a.dim1);
+  const int i0 = (int)(row / a.dim2 / a.dim1);
+  const float *w = a.w + i0 * a.stride[0] + i1 * a.stride[1] +
+                   i2 * a.stride[2];
+  int32_t *keep = a.keep + row * a.budget;
+  int len = a.width;
+  if (a.lengths != nullptr) len = min(max(a.lengths[i0], 0), a.width);
+  const int kept = min(len, a.budget);
+  for (int i = kept + rank * kSelThreads + tid; i < a.budget;
+       i += ranks * kSelThreads)
+    keep[i] = -1;
+  if (len <= a.budget) {           // the same for the whole cluster
+    for (int i = rank * kSelThreads + tid; i < len; i += ranks * kSelThreads)
+      keep[i] = i;
+    return;
+  }
+  // candidates are [sink, len - recent); the rest is kept anyway
+  const int lo = a.sink, hi = len - a.recent;
+  const int n = hi - lo;
+  int need = a.budget - a.sink - a.recent;
+  for (int i = rank * kSelThreads + tid; i < lo; i += ranks * kSelThreads)
+    keep[i] = i;
+  for (int i = rank * kSelThreads + tid; i < a.recent;
+       i += ranks * kSelThreads)
+    keep[a.budget - a.recent + i] = hi + i;
+  if (need == 0) return;
+
+  // this CTA's slice, in whole warps' worths of candidates
+  const int per = (int)div_up(div_up(n, 32), ranks) * 32;
+  const int s0 = min(n, rank * per), s1 = min(n, s0 + per);
+  const float *src = w + lo + s0;
+  const int m = s1 - s0;
+  const bool in_smem = per <= kHeld;
+  if (in_smem) {
+    for (int i = tid; i < m; i += kSelThreads) held[i] = src[i];
+    src = held;
+  }
+
+  uint32_t prefix = 0;
+  for (int shift = 24; shift >= 0; shift -= kDigit) {
+    for (int i = tid; i < kBins * 32; i += kSelThreads) sh.hist[i] = 0;
+    __syncthreads();
+    const uint32_t high = shift == 24 ? 0 : 0xffffffffu << (shift + 8);
+    for (int i = tid; i < m; i += kSelThreads) {
+      const uint32_t u = order_of(src[i]);
+      if ((u & high) == prefix)
+        atomicAdd(&sh.hist[((u >> shift) & 255) * 32 + lane], 1u);
+    }
+    __syncthreads();
+    uint32_t *bins = sh.bins[(shift >> 3) & 1];
+    if (tid < kBins) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) c += sh.hist[tid * 32 + ((i + tid) & 31)];
+      bins[tid] = c;
+    }
+    cluster.sync();
+    if (warp == 0) {
+      // bins from the top, eight a lane: lane 0 holds 255..248
+      uint32_t c[8], own = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        c[e] = 0;
+        for (int r = 0; r < ranks; ++r)
+          c[e] += cluster.map_shared_rank(bins, r)[255 - (lane * 8 + e)];
+        own += c[e];
+      }
+      uint32_t incl = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      uint32_t before = incl - own;
+      if (before < (uint32_t)need && incl >= (uint32_t)need) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (before < (uint32_t)need && before + c[e] >= (uint32_t)need) {
+            sh.digit = 255 - (lane * 8 + e);
+            sh.left = need - before;
+            break;
+          }
+          before += c[e];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= sh.digit << shift;
+    need = (int)sh.left;           // still to take among this digit's
+  }
+  // now: everything above `prefix`, and the first `need` equal to it
+  const int warp_per = (int)div_up(div_up(m, 32), kSelWarps) * 32;
+  const int b0 = min(m, warp * warp_per), b1 = min(m, b0 + warp_per);
+  uint32_t above = 0, equal = 0;
+  for (int i = b0; i < b1; i += 32) {
+    const uint32_t u = i + lane < b1 ? order_of(src[i + lane]) : 0;
+    const bool there = i + lane < b1;
+    above += __popc(__ballot_sync(0xffffffffu, there && u > prefix));
+    equal += __popc(__ballot_sync(0xffffffffu, there && u == prefix));
+  }
+  if (lane == 0) {
+    sh.above[warp] = above;
+    sh.equal[warp] = equal;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t x = 0, y = 0;
+    for (int i = 0; i < kSelWarps; ++i) {
+      const uint32_t cx = sh.above[i], cy = sh.equal[i];
+      sh.above[i] = x;
+      sh.equal[i] = y;
+      x += cx;
+      y += cy;
+    }
+    sh.cta[0] = x;
+    sh.cta[1] = y;
+  }
+  cluster.sync();
+  uint32_t x = sh.above[warp], y = sh.equal[warp];
+  for (int r = 0; r < rank; ++r) {
+    const uint32_t *o = cluster.map_shared_rank(sh.cta, r);
+    x += o[0];
+    y += o[1];
+  }
+  for (int i = b0; i < b1; i += 32) {
+    const bool there = i + lane < b1;
+    const uint32_t u = there ? order_of(src[i + lane]) : 0;
+    const uint32_t below = (1u << lane) - 1;
+    const uint32_t gt = __ballot_sync(0xffffffffu, there && u > prefix);
+    const uint32_t eq = __ballot_sync(0xffffffffu, there && u == prefix);
+    const uint32_t my_eq = y + __popc(eq & below);
+    // kept before this one: all above, and the equal ones up to `need`
+    const uint32_t at = x + __popc(gt & below) + min(my_eq, (uint32_t)need);
+    if (there && (u > prefix || (u == prefix && my_eq < (uint32_t)need)))
+      keep[a.sink + at] = lo + s0 + i + lane;
+    x += __popc(gt);
+    y += __popc(eq);
+  }
+  cluster.sync();                  // the slices' totals are read remotely
+}
+
+// ------------------------------------------------------------------ gather
+constexpr int kGatherTensors = 1024;   // descriptors of one launch
+constexpr int kGThreads = 256;
+
+struct GatherArgs {
+  const int32_t *keep;             // [items][heads][kept]
+  char *out;                       // [items][2][heads][kept][row bytes]
+  const int32_t *table;            // paged sources: [items][table_row]
+  int64_t table_row, stride_page;  // the latter in elements
+  int64_t table_cols;
+  int32_t page, pages, seq;        // seq: tokens of an unpaged source
+  int32_t heads, kept, row_bytes, elem, vec;
+  int32_t item0, shared_keep, layers;
+  cascade_kv_tensor_t t[kGatherTensors];
+};
+
+// One thread copies one vector of one kept row; a block takes the rows of
+// one head of one tensor.  Each row of head_dim values is contiguous, so a
+// row's bytes move as full sectors whatever the row's neighbours do.
+template <typename V>
+__global__ void __launch_bounds__(kGThreads)
+    evict_gather_kernel(const __grid_constant__ GatherArgs a) {
+  const int head = blockIdx.y % a.heads, ti = blockIdx.y / a.heads;
+  const int item = a.item0 + (ti >> 1);
+  const cascade_kv_tensor_t t = a.t[ti];
+  const int per_row = a.row_bytes / (int)sizeof(V);
+  const int32_t *keep =
+      a.keep + ((int64_t)(a.shared_keep ? item / a.layers : item) * a.heads +
+                head) * a.kept;
+  const char *base = reinterpret_cast<const char *>(t.ptr) +
+                     (int64_t)head * t.stride_head * a.elem;
+  V *out = reinterpret_cast<V *>(
+      a.out + (((int64_t)(2 * a.item0 + ti)) * a.heads + head) * a.kept *
+                  (int64_t)a.row_bytes);
+  const int64_t units = (int64_t)a.kept * per_row;
+  constexpr int kPer = 4;
+  const int64_t first =
+      (int64_t)blockIdx.x * kGThreads * kPer + threadIdx.x;
+  V v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t u = first + i * kGThreads;
+    v[i] = V{};
+    if (u >= units) continue;
+    const int r = (int)(u / per_row), c = (int)(u - (int64_t)r * per_row);
+    const int pos = keep[r];
+    const char *src = nullptr;
+    if (a.table != nullptr) {
+      if (pos >= 0 && pos / a.page < a.table_cols) {
+        const int id =
+            a.table[(int64_t)item * a.table_row + pos / a.page];
+        if (id >= 0 && id < a.pages)
+          src = base + (id * a.stride_page +
+                        (int64_t)(pos % a.page) * t.stride_seq) * a.elem;
+      }
+    } else if (pos >= 0 && pos < a.seq) {
+      src = base + (int64_t)pos * t.stride_seq * a.elem;
+    }
+    if (src != nullptr) v[i] = reinterpret_cast<const V *>(src)[c];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t u = first + i * kGThreads;
+    if (u < units) out[u] = v[i];
+  }
+}
+
+}  // namespace
+}  // namespace cb
+
+extern "C" int cascade_kv_evict_select(
+    const float *d_weights, const int64_t dims[3], const int64_t strides[3],
+    int32_t width, const int32_t *d_lengths, int32_t budget, int32_t recent,
+    int32_t sink, int32_t *d_keep, void *stream) {
+  using namespace cb;
+  clear_error();
+  CB_CHECK(dims && strides, CASCADE_ERR_INVALID, "null pointer argument");
+  CB_CHECK(dims[0] >= 0 && dims[1] >= 0 && dims[2] >= 0 && width >= 0,
+           CASCADE_ERR_INVALID, "negative size");
+  CB_CHECK(budget > 0 && recent >= 0 && sink >= 0 &&
+               (int64_t)recent + sink <= budget,
+           CASCADE_ERR_INVALID,
+           "budget must be above 0 and at least recent + sink");
+  const int64_t big = (int64_t)1 << 28;
+  CB_CHECK(dims[0] <= big && dims[1] <= big && dims[2] <= big &&
+               dims[0] * dims[1] <= big && dims[0] * dims[1] * dims[2] <= big,
+           CASCADE_ERR_INVALID, "too many rows of weights");
+  const int64_t rows = dims[0] * dims[1] * dims[2];
+  if (rows == 0) return CASCADE_OK;
+  CB_CHECK((d_weights || width == 0) && d_keep, CASCADE_ERR_INVALID,
+           "null pointer argument");
+  SelectArgs a{};
+  a.w = d_weights;
+  for (int i = 0; i < 3; ++i) a.stride[i] = strides[i];
+  a.dim1 = (int)dims[1];
+  a.dim2 = (int)dims[2];
+  a.lengths = d_lengths;
+  a.width = width;
+  a.budget = budget;
+  a.recent = recent;
+  a.sink = sink;
+  a.keep = d_keep;
+  // One CTA reads about 4096 weights a microsecond, so a row is spread over
+  // more CTAs while SMs are idle and each still has that much to do; a
+  // slice that does not fit shared memory is read from L2 in every pass.
+  int ranks = 1;
+  while (ranks < 8 && rows * ranks * 2 <= 2 * sm_count() &&
+         width / (ranks * 2) >= 2048)
+    ranks *= 2;
+  const int64_t per = (int64_t)div_up(div_up(width, 32), ranks) * 32;
+  size_t smem = sizeof(SelectShared);
+  if (per <= kHeld) smem += (size_t)per * 4;
+  CB_CUDA(cudaFuncSetAttribute(evict_select_kernel,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)(sizeof(SelectShared) + kHeld * 4)));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * ranks));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CB_CUDA(cudaLaunchKernelEx(&cfg, evict_select_kernel, a));
+  count_launches(1);
+  return CASCADE_OK;
+}
+
+extern "C" int cascade_kv_evict_gather(
+    const cascade_kv_tensor_t *src, uint32_t items, uint32_t layers,
+    uint32_t heads, uint32_t seq, uint32_t head_dim, uint32_t elem_bytes,
+    const int32_t *d_keep, uint32_t kept, const int32_t *d_table,
+    int64_t table_row, int64_t table_cols, int64_t stride_page, uint32_t page, uint32_t pages,
+    void *d_out, void *stream) {
+  using namespace cb;
+  clear_error();
+  CB_CHECK(elem_bytes == 2 || elem_bytes == 4, CASCADE_ERR_INVALID,
+           "elements have 2 or 4 bytes");
+  CB_CHECK(heads <= 65535 && (uint64_t)head_dim * elem_bytes < (1u << 30) &&
+               seq <= INT32_MAX && kept <= INT32_MAX && page <= INT32_MAX &&
+               pages <= INT32_MAX && items <= INT32_MAX / 2,
+           CASCADE_ERR_INVALID, "a size is out of range");
+  CB_CHECK(layers >= 1, CASCADE_ERR_INVALID, "layers must be above 0");
+  if (items == 0 || heads == 0 || head_dim == 0 || kept == 0)
+    return CASCADE_OK;
+  CB_CHECK(src && d_keep && d_out, CASCADE_ERR_INVALID,
+           "null pointer argument");
+  CB_CHECK(!d_table || (page > 0 && table_cols >= 0), CASCADE_ERR_INVALID,
+           "a page table needs a page size");
+  static thread_local GatherArgs a;
+  a.keep = d_keep;
+  a.out = static_cast<char *>(d_out);
+  a.table = d_table;
+  a.table_row = table_row;
+  a.table_cols = table_cols;
+  a.stride_page = stride_page;
+  a.page = (int)(page ? page : 1);
+  a.pages = (int)pages;
+  a.seq = (int)seq;
+  a.heads = (int)heads;
+  a.kept = (int)kept;
+  a.row_bytes = (int)(head_dim * elem_bytes);
+  a.elem = (int)elem_bytes;
+  a.shared_keep = layers > 1;
+  a.layers = (int)layers;
+  // 16-byte vectors when every row starts on a 16-byte boundary, else
+  // elements one by one.
+  uint64_t bits = (uintptr_t)d_out | (uint64_t)a.row_bytes |
+                  (uint64_t)(d_table ? stride_page * elem_bytes : 0);
+  for (uint32_t i = 0; i < items * 2; ++i) {
+    CB_CHECK(src[i].ptr || (d_table ? pages == 0 : seq == 0),
+             CASCADE_ERR_INVALID, "null pointer argument");
+    bits |= src[i].ptr | (uint64_t)(src[i].stride_head * elem_bytes) |
+            (uint64_t)(src[i].stride_seq * elem_bytes);
+  }
+  const int vec = bits & 15 ? (int)elem_bytes : 16;
+  const uint64_t units = (uint64_t)kept * (a.row_bytes / vec);
+  const uint64_t blocks = div_up(units, kGThreads * 4);
+  CB_CHECK(blocks <= INT32_MAX, CASCADE_ERR_INVALID, "kept is too large");
+  const uint32_t step_max = 65535 / heads < (uint32_t)kGatherTensors
+                                ? (65535 / heads) & ~1u
+                                : (uint32_t)kGatherTensors;
+  CB_CHECK(step_max >= 2, CASCADE_ERR_INVALID, "too many heads");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (uint32_t t0 = 0; t0 < items * 2; t0 += step_max) {
+    const uint32_t n =
+        items * 2 - t0 < step_max ? items * 2 - t0 : step_max;
+    a.item0 = (int)(t0 / 2);
+    for (uint32_t i = 0; i < n; ++i) a.t[i] = src[t0 + i];
+    const dim3 grid((unsigned)blocks, n * heads);
+    if (vec == 16)
+      evict_gather_kernel<uint4><<<grid, kGThreads, 0, s>>>(a);
+    else if (elem_bytes == 4)
+      evict_gather_kernel<uint32_t><<<grid, kGThreads, 0, s>>>(a);
+    else
+      evict_gather_kernel<uint16_t><<<grid, kGThreads, 0, s>>>(a);
+    count_launches(1);
+    CB_CUDA(cudaGetLastError());
+  }
+  return CASCADE_OK;
+}

@@ -1,0 +1,592 @@
+"""Operators over KV caches on the device: attention that reads a cache, the
+attention weight each cached token received, and eviction by it.
+
+They work on what cascade_b200.kvwire loads from the store and hand back what
+it stores.  A server's step over stored prefixes:
+
+    pages, found = kvwire.load_kv_pages(store, block_ids, ...)   # 16-token
+    plan = kvattn.AttentionPlan(new, cached, q_heads=32, kv_heads=8,
+                                head_dim=128, page_size=16)
+    for layer in ...:                    # one plan serves every layer
+        kv = pages[:, layer, 0], pages[:, layer, 1]
+        out, lse = kvattn.prompt_attention(plan, q, k, v, kv, table)
+
+New tokens are packed: `q` is [tokens, q heads, dim], `k` and `v` [tokens, kv
+heads, dim], sequence after sequence; the lengths live in the plan.  Cached
+tokens are in pages [pages, kv heads, page, dim] that an int32 `page_table`
+[sequences, columns] names in order; the new tokens follow the cached ones.
+An entry outside [0, pages) names no page: its tokens are never read and
+count as unseen.  Query head h uses key/value head h // (q_heads //
+kv_heads).  Tensors are float16 or bfloat16, head_dim 64 or 128 and
+contiguous; other strides may be anything whose rows start on 16-byte
+boundaries (a slice of a fused projection, a [1, heads, seq, dim] cache
+permuted to [seq, heads, dim]).  Rows of `out` that belong to no sequence are
+left as they were.  There are no backward passes: tensors that require a
+gradient are refused while gradients are enabled.
+
+Work is enqueued on the current stream of the tensors' device.  A plan may be
+used on any stream, and in captured graphs for as long as it is kept alive;
+workspaces are allocated per call, so calls on several streams and graphs
+that overlap share nothing.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import _lib, kvwire
+from ._lib import check
+
+FORWARD, WEIGHTS = 0, 1            # CASCADE_ATTN_*
+
+_i32, _i64, _u64, _f32 = (ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64,
+                          ctypes.c_float)
+_vp, _u32, _int, _sz = (ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int,
+                        ctypes.c_size_t)
+
+
+class _PlanInfo(ctypes.Structure):
+    """cascade_attn_plan_info_t."""
+    _fields_ = [(n, _i32) for n in (
+        "kind", "batch", "q_heads", "kv_heads", "head_dim", "page_size",
+        "tree", "window", "sms", "ints", "ctas", "segments", "parts",
+        "merges", "merge_rows", "row_tile", "max_new", "max_cached",
+        "max_keys", "table_cols")] + [("tokens", _i64),
+                                      ("workspace_bytes", _u64)]
+
+
+class _Args(ctypes.Structure):
+    """cascade_attn_args_t."""
+    _fields_ = [("dtype", _i32), ("pages", _i32), ("scale", _f32),
+                ("add", _i32), ("plan", _vp), ("q", _vp), ("k", _vp),
+                ("v", _vp)] + [(n, _i64) for n in (
+                    "q_tok", "q_head", "k_tok", "k_head", "v_tok",
+                    "v_head")] + [("k_pages", _vp), ("v_pages", _vp)] + [
+                        (n, _i64) for n in (
+                            "kp_page", "kp_head", "kp_tok", "vp_page",
+                            "vp_head", "vp_tok")] + [
+        ("table", _vp), ("table_row", _i64), ("mask", _vp),
+        ("mask_row", _i64), ("out", _vp), ("out_tok", _i64),
+        ("out_head", _i64), ("lse", _vp), ("lse_tok", _i64),
+        ("lse_head", _i64), ("before", _vp), ("before_seq", _i64),
+        ("before_head", _i64), ("weights", _vp), ("weights_seq", _i64),
+        ("weights_head", _i64), ("width", _i32), ("fill", _i32),
+        ("workspace", _vp), ("workspace_bytes", _u64)]
+
+
+_lib.register("cascade_attn_plan", _int, [_vp, _vp, _vp, _vp, _sz])
+_lib.register("cascade_attn_forward", _int, [_vp, _vp, _vp])
+_lib.register("cascade_attn_weights", _int, [_vp, _vp, _vp])
+_lib.register("cascade_kv_evict_select", _int,
+              [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp])
+_lib.register("cascade_kv_evict_gather", _int,
+              [_vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _u32, _vp, _i64,
+               _i64, _i64, _u32, _u32, _vp, _vp])
+_lib.register("cascade_diag_attn_timeouts", _int, [ctypes.POINTER(_u64)])
+
+
+# ------------------------------------------------------------------- plans
+def _host_lengths(x, name):
+    import numpy as np
+    if hasattr(x, "detach"):
+        x = x.detach().cpu().numpy()
+    a = np.asarray(x)
+    if a.size == 0:
+        a = a.astype(np.int64)
+    if a.ndim != 1 or a.dtype.kind not in "iu":
+        raise TypeError(f"{name} must be a 1-D sequence of integers")
+    if a.size and (int(a.min()) < 0 or int(a.max()) > 1 << 30):
+        raise ValueError(f"{name} must be in [0, 2**30]")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _cuda_device(device):
+    import torch
+    d = torch.device(device)
+    if d.type != "cuda":
+        raise ValueError("the attention operators run on CUDA devices only")
+    return d if d.index is not None else torch.device(
+        "cuda", torch.cuda.current_device())
+
+
+class _Plan:
+    """The division of one batch among the SMs, made once on the host from
+    its lengths and used by every layer's call."""
+
+    def __init__(self, kind, new_lengths, cached_lengths, q_heads, kv_heads,
+                 head_dim, page_size, device, tree=False, window=1):
+        import numpy as np
+        import torch
+        new = _host_lengths(new_lengths, "new_lengths")
+        cached = (np.zeros_like(new) if cached_lengths is None
+                  else _host_lengths(cached_lengths, "cached_lengths"))
+        if cached.size != new.size:
+            raise ValueError("one cached length per sequence: "
+                             f"{cached.size} for {new.size}")
+        self.device = _cuda_device(device)
+        info = _PlanInfo(
+            kind=kind, batch=new.size, q_heads=q_heads, kv_heads=kv_heads,
+            head_dim=head_dim, page_size=page_size or 0, tree=int(tree),
+            window=window)
+        with torch.cuda.device(self.device):
+            buf = np.empty(4096, np.int32)
+            for _ in range(2):
+                check(_lib.load().cascade_attn_plan(
+                    ctypes.byref(info), new.ctypes.data, cached.ctypes.data,
+                    buf.ctypes.data, buf.size))
+                if info.ints <= buf.size:
+                    break
+                buf = np.empty(info.ints, np.int32)
+            # a blocking copy: the plan is ready for every stream
+            self._buf = torch.from_numpy(buf[:info.ints].copy()).to(
+                self.device)
+        self._stream = torch.cuda.current_stream(self.device)
+        self._info = info
+        self._ref = ctypes.byref(info)
+        self.batch, self.tokens = info.batch, info.tokens
+        self.q_heads, self.kv_heads = info.q_heads, info.kv_heads
+        self.head_dim, self.page_size = info.head_dim, info.page_size
+        self.max_new, self.max_cached = info.max_new, info.max_cached
+        self.max_keys, self.tree = info.max_keys, bool(info.tree)
+
+
+class AttentionPlan(_Plan):
+    """Plan of prompt_attention (or, with tree=True, tree_attention) for a
+    batch of sequences with `new_lengths` new tokens each behind
+    `cached_lengths` cached ones (host integers; None: none cached)."""
+
+    def __init__(self, new_lengths, cached_lengths=None, *, q_heads,
+                 kv_heads, head_dim, page_size=None, tree=False,
+                 device="cuda"):
+        super().__init__(FORWARD, new_lengths, cached_lengths, q_heads,
+                         kv_heads, head_dim, page_size, device, tree=tree)
+
+
+class WeightsPlan(_Plan):
+    """Plan of attention_weights.  `window`: how many of each sequence's
+    last new tokens count (None: all)."""
+
+    def __init__(self, new_lengths, cached_lengths=None, *, q_heads,
+                 kv_heads, head_dim, page_size=None, window=None,
+                 device="cuda"):
+        if window is None:
+            window = (1 << 31) - 1
+        if not 0 < window < 1 << 31:
+            raise ValueError("window must be above 0")
+        super().__init__(WEIGHTS, new_lengths, cached_lengths, q_heads,
+                         kv_heads, head_dim, page_size, device,
+                         window=window)
+
+
+# ------------------------------------------------------------------ checks
+def _dtype(q):
+    import torch
+    codes = {torch.float16: 0, torch.bfloat16: 1}
+    if q.dtype not in codes:
+        raise TypeError(f"q must be float16 or bfloat16, not {q.dtype}")
+    return codes[q.dtype]
+
+
+def _strides(t):
+    """Element strides with 0 for dimensions of one element, whose stride
+    torch leaves arbitrary."""
+    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+
+
+def _rows(name, t, shape, dtype, device):
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}; got "
+                         f"{tuple(t.shape)}")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} on {device}; got {t.dtype} "
+                         f"on {t.device}")
+    st = _strides(t)
+    if st[-1] not in (0, 1):
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    align = 16 // t.element_size()
+    if t.data_ptr() % 16 or any(s % align for s in st[:-1]):
+        raise ValueError(f"{name}: rows must start on 16-byte boundaries")
+    return t.data_ptr(), st
+
+
+def _no_grad(*tensors):
+    import torch
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the attention operators have no backward pass: "
+                           "call them under torch.no_grad()")
+
+
+def _writable(name, t):
+    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} must not be an expanded tensor")
+
+
+def _common(plan, kind, q, k, v, k_pages, v_pages, page_table, scale):
+    """The arguments that both kinds of call share."""
+    if plan._info.kind != kind:
+        raise ValueError("the plan is of the other kind: AttentionPlan for "
+                         "attention, WeightsPlan for attention_weights")
+    dev, n = plan.device, plan.tokens
+    H, G, D = plan.q_heads, plan.kv_heads, plan.head_dim
+    if q.dim() != 3 or q.shape[0] < n:
+        raise ValueError(f"q must be [>= {n} tokens, {H}, {D}]; got "
+                         f"{tuple(q.shape)}")
+    rows = q.shape[0]
+    a = _Args(dtype=_dtype(q))
+    if scale is None:
+        a.scale = 1.0 / math.sqrt(D)
+    else:
+        a.scale = scale
+        if not (math.isfinite(scale) and a.scale > 0.0
+                and math.isfinite(a.scale)):
+            raise ValueError("scale must be finite and above 0")
+    a.q, st = _rows("q", q, (rows, H, D), q.dtype, dev)
+    a.q_tok, a.q_head = st[:2]
+    a.k, st = _rows("k", k, (rows, G, D), q.dtype, dev)
+    a.k_tok, a.k_head = st[:2]
+    if v is not None:
+        a.v, st = _rows("v", v, (rows, G, D), q.dtype, dev)
+        a.v_tok, a.v_head = st[:2]
+    if plan.max_cached:
+        if k_pages is None or page_table is None:
+            raise ValueError("the plan has cached tokens: pages and "
+                             "page_table are needed")
+        shape = (k_pages.shape[0], G, plan.page_size, D)
+        a.pages = shape[0]
+        a.k_pages, st = _rows("k_pages", k_pages, shape, q.dtype, dev)
+        a.kp_page, a.kp_head, a.kp_tok = st[:3]
+        if v_pages is not None:
+            a.v_pages, st = _rows("v_pages", v_pages, shape, q.dtype, dev)
+            a.vp_page, a.vp_head, a.vp_tok = st[:3]
+        a.table, a.table_row = _table(page_table, plan.batch,
+                                      plan._info.table_cols, dev)
+    a.plan = plan._buf.data_ptr()
+    return a
+
+
+def _table(page_table, batch, cols, dev):
+    import torch
+    if (page_table.dim() != 2 or page_table.shape[0] != batch
+            or page_table.shape[1] < cols):
+        raise ValueError(f"page_table must be [{batch}, >= {cols}]; got "
+                         f"{tuple(page_table.shape)}")
+    if page_table.dtype != torch.int32 or page_table.device != dev:
+        raise ValueError(f"page_table must be int32 on {dev}")
+    st = _strides(page_table)
+    if st[1] not in (0, 1):
+        raise ValueError("page_table: rows must be contiguous")
+    return page_table.data_ptr(), st[0]
+
+
+def _launch(plan, a, fn):
+    """Runs fn on the current stream of the plan's device."""
+    import torch
+    dev = plan.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _launch(plan, a, fn)
+    stream = torch.cuda.current_stream(dev)
+    if stream != plan._stream:
+        # the plan's memory must not be handed out while this call reads it
+        plan._buf.record_stream(stream)
+    size = plan._info.workspace_bytes
+    if size:
+        # freed on return: the allocator hands it out again only to work
+        # ordered behind this call on the same stream
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+        a.workspace_bytes = size
+    check(fn(plan._ref, ctypes.byref(a), stream.cuda_stream))
+
+
+# --------------------------------------------------------------- attention
+def _forward(plan, q, k, v, mask, pages, page_table, scale, out, lse):
+    import torch
+    k_pages, v_pages = pages if pages is not None else (None, None)
+    _no_grad(q, k, v, k_pages, v_pages)
+    if pages is not None and v_pages is None:
+        raise ValueError("pages is a pair (k_pages, v_pages)")
+    a = _common(plan, FORWARD, q, k, v, k_pages, v_pages, page_table, scale)
+    dev, shape = plan.device, (q.shape[0], plan.q_heads, plan.head_dim)
+    if mask is not None:
+        if (mask.dim() != 2 or mask.shape[0] != shape[0]
+                or mask.shape[1] < plan.max_new):
+            raise ValueError(f"mask must be [{shape[0]}, >= {plan.max_new}]; "
+                             f"got {tuple(mask.shape)}")
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev:
+            raise ValueError(f"mask must be bool or uint8 on {dev}")
+        st = _strides(mask)
+        if st[1] not in (0, 1) or (st[1] == 0 and mask.shape[1] > 1):
+            raise ValueError("mask: rows must be contiguous")
+        a.mask, a.mask_row = mask.data_ptr(), st[0]
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    else:
+        _writable("out", out)
+    a.out, st = _rows("out", out, shape, q.dtype, dev)
+    a.out_tok, a.out_head = st[:2]
+    if lse is None:
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+    else:
+        _writable("lse", lse)
+        if (tuple(lse.shape) != shape[:2] or lse.dtype != torch.float32
+                or lse.device != dev):
+            raise ValueError(f"lse must be float32 {shape[:2]} on {dev}")
+    a.lse = lse.data_ptr()
+    a.lse_tok, a.lse_head = _strides(lse)
+    if plan.tokens:
+        _launch(plan, a, _lib.load().cascade_attn_forward)
+    return out, lse
+
+
+def prompt_attention(plan, q, k, v, pages=None, page_table=None, *,
+                     scale=None, out=None, lse=None):
+    """Causal attention of packed new tokens: each sees its sequence's cached
+    tokens and the new ones up to itself.  Whole prompts, the rest of a
+    prompt whose prefix came from the store, and single tokens of a decode
+    step are all this call; they differ in the plan's lengths only.
+
+    q [tokens, q heads, dim], k and v [tokens, kv heads, dim]; pages =
+    (k_pages, v_pages) and page_table where the plan has cached tokens;
+    scale defaults to 1 / sqrt(dim).  Returns (out, lse): out as q, lse
+    float32 [tokens, q heads], the natural log of the sum of exp(score)."""
+    if plan.tree:
+        raise ValueError("the plan is for trees: use tree_attention")
+    return _forward(plan, q, k, v, None, pages, page_table, scale, out, lse)
+
+
+def tree_attention(plan, q, k, v, mask, pages=None, page_table=None, *,
+                   scale=None, out=None, lse=None):
+    """Attention of drafted tokens, which are not in the cache yet: each sees
+    its sequence's cached tokens and the drafts its mask row names.  mask
+    [tokens, >= longest tree] bool: mask[t, j] says that packed token t sees
+    draft j of its own sequence (itself only where the mask says so).  A
+    token that sees nothing at all gets zeros and lse -inf.  The plan is made
+    with tree=True; otherwise as prompt_attention."""
+    if not plan.tree:
+        raise ValueError("the plan is causal: make it with tree=True")
+    if mask is None:
+        raise ValueError("tree_attention needs a mask")
+    return _forward(plan, q, k, v, mask, pages, page_table, scale, out, lse)
+
+
+def attention_weights(plan, q, k, lse, k_pages=None, page_table=None, *,
+                      scale=None, add_to=None, out=None):
+    """The attention weight that every token received: out[b, kv head, j] =
+    add_to + the sum of exp(score - lse) over the query heads of the group
+    and the last `window` new tokens of sequence b that see token j
+    (causally).  lse is prompt_attention's, for the same tokens and scale.
+
+    add_to and out are float32 [sequences, kv heads, width >= longest
+    sequence] with contiguous rows; out may be add_to itself.  Returns out;
+    without one, a new tensor whose positions behind a sequence's end hold
+    add_to's values (or 0).  In a given out those are left as they were."""
+    import torch
+    _no_grad(q, k, lse, k_pages, add_to)
+    a = _common(plan, WEIGHTS, q, k, None, k_pages, None, page_table, scale)
+    dev = plan.device
+    if (tuple(lse.shape) != (q.shape[0], plan.q_heads)
+            or lse.dtype != torch.float32 or lse.device != dev):
+        raise ValueError("lse must be float32 "
+                         f"{(q.shape[0], plan.q_heads)} on {dev}")
+    a.lse = lse.data_ptr()
+    a.lse_tok, a.lse_head = _strides(lse)
+
+    def rows(name, t):
+        if (t.dim() != 3 or tuple(t.shape[:2]) != (plan.batch, plan.kv_heads)
+                or t.shape[2] < plan.max_keys):
+            raise ValueError(
+                f"{name} must be [{plan.batch}, {plan.kv_heads}, >= "
+                f"{plan.max_keys}]; got {tuple(t.shape)}")
+        if t.dtype != torch.float32 or t.device != dev:
+            raise ValueError(f"{name} must be float32 on {dev}")
+        st = _strides(t)
+        if st[2] not in (0, 1) or (st[2] == 0 and t.shape[2] > 1):
+            raise ValueError(f"{name}: rows must be contiguous")
+        return t.data_ptr(), st
+
+    if out is None:
+        width = plan.max_keys if add_to is None else add_to.shape[-1]
+        out = torch.empty((plan.batch, plan.kv_heads, width),
+                          dtype=torch.float32, device=dev)
+        a.fill = 1
+    else:
+        _writable("out", out)
+    a.weights, st = rows("out", out)
+    a.weights_seq, a.weights_head = st[:2]
+    a.width = out.shape[2]
+    if add_to is not None:
+        a.before, st = rows("add_to", add_to)
+        a.before_seq, a.before_head = st[:2]
+        a.width = min(a.width, add_to.shape[2])
+        a.add = 1
+    if out.numel():
+        _launch(plan, a, _lib.load().cascade_attn_weights)
+    return out
+
+
+# ---------------------------------------------------------------- eviction
+def select_kept(weights, budget, recent=0, sink=0, lengths=None):
+    """The tokens to keep: weights is float32 [sequences, ..., tokens] (up to
+    three leading dimensions, contiguous rows).  Each row keeps its first
+    `sink` and last `recent` tokens and those of the largest weights, ties to
+    the lowest position, `budget` in all; NaN ranks below every number.
+    lengths (int32 CUDA [sequences], clamped to the row) ends the rows of a
+    sequence early.  Returns int32 [sequences, ..., budget], ascending; a row
+    of fewer tokens than budget keeps all and ends in -1."""
+    import torch
+    if weights.dtype != torch.float32 or not weights.is_cuda:
+        raise ValueError("weights must be a float32 CUDA tensor")
+    if not 2 <= weights.dim() <= 4:
+        raise ValueError("weights has 1 to 3 dimensions before the tokens; "
+                         f"got shape {tuple(weights.shape)}")
+    st = _strides(weights)
+    if weights.shape[-1] > 1 and st[-1] != 1:
+        raise ValueError("weights: rows must be contiguous")
+    if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
+        raise ValueError("budget must be above 0 and at least recent + sink "
+                         f"(got {budget}, {recent}, {sink})")
+    if max(budget, weights.shape[-1]) >= 1 << 31:
+        raise ValueError("rows have fewer than 2**31 tokens")
+    dev, lead = weights.device, list(weights.shape[:-1])
+    if lengths is not None and (
+            lengths.dtype != torch.int32 or lengths.device != dev
+            or tuple(lengths.shape) != (lead[0],)
+            or not lengths.is_contiguous()):
+        raise ValueError(f"lengths must be int32 [{lead[0]}] on {dev}")
+    keep = torch.empty(lead + [budget], dtype=torch.int32, device=dev)
+    pad = 3 - len(lead)
+    dims = (_i64 * 3)(*(lead + [1] * pad))
+    strides = (_i64 * 3)(*(st[:-1] + [0] * pad))
+    with torch.cuda.device(dev):
+        check(_lib.load().cascade_kv_evict_select(
+            weights.data_ptr(), dims, strides, weights.shape[-1],
+            lengths.data_ptr() if lengths is not None else None, budget,
+            recent, sink, keep.data_ptr(), kvwire._stream(dev)))
+    return keep
+
+
+def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
+    """Shortens n KV caches of one shape (as kvwire.serialize_kv_caches
+    takes them) to `budget` tokens per head by select_kept's rule.  weights:
+    float32 [n, layers, kv heads, seq], or [n, kv heads, seq] for one choice
+    that all layers share.
+
+    Returns (kv, keep): kv [n, layers, 2, kv heads, kept, dim] in the caches'
+    dtype (kept = min(budget, seq)) and the positions, int32 [n, (layers,)
+    kv heads, kept].  cache_views(kv) gives the caches back as tuples."""
+    import torch
+    n = len(caches)
+    if n == 0:
+        raise ValueError("no caches to evict from")
+    desc, (L, H, S, D, dev, dt) = _cache_descriptors(caches)
+    lead = (n, L, H) if weights.dim() == 4 else (n, H)
+    if tuple(weights.shape) != lead + (S,) or weights.device != dev:
+        raise ValueError(f"weights must be {lead + (S,)} on {dev}; got "
+                         f"{tuple(weights.shape)} on {weights.device}")
+    if budget >= S and 0 <= recent and 0 <= sink and \
+            recent + sink <= budget:
+        recent, sink = min(recent, S), 0         # everything is kept
+        budget = max(S, 1)
+    keep = select_kept(weights, budget, recent, sink)
+    kept = min(budget, S)
+    keep = keep[..., :kept]
+    kv = torch.empty((n, L, 2, H, kept, D), dtype=dt, device=dev)
+    with torch.cuda.device(dev):
+        check(_lib.load().cascade_kv_evict_gather(
+            desc.ctypes.data, n * L, L if weights.dim() == 3 else 1, H, S, D,
+            dt.itemsize, keep.data_ptr(), kept, None, 0, 0, 0, 0, 0,
+            kv.data_ptr(), kvwire._stream(dev)))
+    return kv, keep
+
+
+def _cache_descriptors(caches):
+    """(host descriptor rows, geometry) of n caches of one shape."""
+    import numpy as np
+    tensors, geo = [], None
+    for c in caches:
+        pairs = kvwire.extract_kv_pairs(c)
+        if geo is None:
+            geo = kvwire._geometry(pairs)
+        elif len(pairs) != geo[0]:
+            raise ValueError("every cache must have one shape, dtype and "
+                             "device")
+        for kv in pairs:
+            tensors += kv
+    L, H, S, D, dev, dt = geo
+    rows = np.empty((len(tensors), 3), dtype=np.int64)
+    shapes = ((1, H, S, D), (H, S, D))
+    for i, t in enumerate(tensors):
+        if t.shape not in shapes or t.dtype != dt or t.device != dev:
+            raise ValueError("every cache must have one shape, dtype and "
+                             "device")
+        st = t.stride()
+        if D > 1 and st[-1] != 1:
+            raise ValueError("head_dim must be contiguous (stride 1)")
+        rows[i] = (t.data_ptr(), st[-3] if H > 1 else 0,
+                   st[-2] if S > 1 else 0)
+    return rows, geo
+
+
+def cache_views(kv):
+    """evict_kv_caches' kv as a list of caches: tuples of (K, V) per layer,
+    [1, kv heads, kept, dim] each."""
+    return [tuple((l[0].unsqueeze(0), l[1].unsqueeze(0)) for l in c)
+            for c in kv]
+
+
+def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
+                recent=0, sink=0):
+    """The same for one layer of a batch in pages: sequence b's tokens are
+    the first lengths[b] (int32 CUDA [sequences]) of the pages that its row
+    of page_table names; weights is float32 [sequences, kv heads, tokens].
+
+    Returns (k, v, keep): [sequences, kv heads, budget, dim] each and the
+    positions, int32 [sequences, kv heads, budget].  A sequence of fewer
+    tokens keeps them all; its rows behind them are zeros and -1."""
+    import numpy as np
+    import torch
+    dev, dt = k_pages.device, k_pages.dtype
+    if not k_pages.is_cuda or dt.itemsize not in (2, 4):
+        raise ValueError("pages must be CUDA tensors of 2- or 4-byte values")
+    if (k_pages.dim() != 4 or v_pages.shape != k_pages.shape
+            or v_pages.dtype != dt or v_pages.device != dev):
+        raise ValueError("k_pages and v_pages must be [pages, heads, page, "
+                         "dim] of one shape, dtype and device")
+    P, H, page, D = k_pages.shape
+    B = page_table.shape[0] if page_table.dim() else 0
+    if (weights.dim() != 3 or tuple(weights.shape[:2]) != (B, H)
+            or weights.device != dev):
+        raise ValueError(f"weights must be [{B}, {H}, tokens] on {dev}")
+    if page < 1:
+        raise ValueError("pages hold at least one token")
+    desc = np.empty((2, 3), np.int64)
+    st = _strides(k_pages)
+    if _strides(v_pages)[0] != st[0]:
+        raise ValueError("k_pages and v_pages must have one page stride")
+    for i, t in enumerate((k_pages, v_pages)):
+        s = _strides(t)
+        if D > 1 and s[3] != 1:
+            raise ValueError("head_dim must be contiguous (stride 1)")
+        desc[i] = (t.data_ptr(), s[1], s[2])
+    table, table_row = _table(page_table, B, 0, dev)
+    keep = select_kept(weights, budget, recent, sink, lengths)
+    kv = torch.empty((B, 2, H, budget, D), dtype=dt, device=dev)
+    if kv.numel():
+        src = np.tile(desc, (B, 1))
+        with torch.cuda.device(dev):
+            check(_lib.load().cascade_kv_evict_gather(
+                src.ctypes.data, B, 1, H, 0, D,
+                dt.itemsize, keep.data_ptr(), budget, table, table_row,
+                page_table.shape[1], st[0], page, P, kv.data_ptr(),
+                kvwire._stream(dev)))
+    return kv[:, 0], kv[:, 1], keep
+
+
+def wait_timeouts() -> int:
+    """Waits inside attention kernels that gave up on the current device
+    (0 unless something is broken).  Synchronises."""
+    n = _u64(0)
+    check(_lib.load().cascade_diag_attn_timeouts(ctypes.byref(n)))
+    return n.value

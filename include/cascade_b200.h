@@ -146,6 +146,134 @@ int cascade_kv_deserialize_batch(const uint64_t *d_src, uint32_t layers,
                                  const cascade_kv_tensor_t *d_dst, size_t n,
                                  void *stream);
 
+/* ------------------------------------------------------------------ */
+/* Operators over KV caches on the device: attention of prompts and of
+ * drafted tokens over cached tokens, the attention weight each token got,
+ * and eviction by it.  They read what the store hands out
+ * (cascade_kv_deserialize_batch, cascade_store_get_kv_batch) and make the
+ * caches it is given back.
+ *
+ * Layout.  New tokens are packed: sequence 0's tokens, then sequence 1's;
+ * element [token][head][d] is at ptr + (token * tok + head * head_stride +
+ * d) * 2 bytes.  Cached tokens are in pages of page_size tokens: row [page]
+ * [head][token of the page][d].  Sequence b's cached token j is token
+ * j % page_size of page table[b * table_row + j / page_size]; entries
+ * outside [0, pages) name no page: their tokens are never read and count as
+ * unseen.  Strides are in elements, every row of head_dim values starts on a
+ * 16-byte boundary.  Query head h reads key/value head
+ * h / (q_heads / kv_heads). */
+
+/* A plan: which CTA does which part of a batch, made on the host from the
+ * batch's lengths and used by every layer's call of a step. */
+#define CASCADE_ATTN_FORWARD 0
+#define CASCADE_ATTN_WEIGHTS 1
+
+typedef struct {
+  int32_t kind;        /* CASCADE_ATTN_* */
+  int32_t batch;
+  int32_t q_heads, kv_heads;
+  int32_t head_dim;    /* 64 or 128 */
+  int32_t page_size;   /* 0: no cached tokens */
+  int32_t tree;        /* forward: new tokens see what a mask names */
+  int32_t window;      /* weights: the last new tokens that count */
+  int32_t sms;         /* CTAs at most (0: the current device's SMs) */
+  /* outputs of cascade_attn_plan */
+  int32_t ints;        /* int32 values of the plan buffer */
+  int32_t ctas, segments, parts, merges, merge_rows, row_tile;
+  int32_t max_new, max_cached, max_keys, table_cols;
+  int64_t tokens;      /* packed tokens */
+  uint64_t workspace_bytes;
+} cascade_attn_plan_info_t;
+
+/* Fills the output fields of `info` and, where capacity (in int32 values)
+ * allows, the plan buffer `out` (host memory; copied to the device by the
+ * caller).  When info->ints > capacity nothing is written to `out`: call
+ * again with room.  Lengths are host arrays of `batch` entries, all >= 0. */
+int cascade_attn_plan(cascade_attn_plan_info_t *info,
+                      const int32_t *new_lengths,
+                      const int32_t *cached_lengths, int32_t *out,
+                      size_t capacity);
+
+typedef struct {
+  int32_t dtype;       /* CASCADE_KV_FP16 or CASCADE_KV_BF16 */
+  int32_t pages;       /* pages there are */
+  float scale;         /* of the scores, > 0 */
+  int32_t add;         /* weights: add to `before` */
+  const int32_t *plan; /* device copy of the plan buffer */
+  const void *q, *k, *v;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  const void *k_pages, *v_pages;
+  int64_t kp_page, kp_head, kp_tok, vp_page, vp_head, vp_tok;
+  const int32_t *table;
+  int64_t table_row;
+  const uint8_t *mask; /* trees: mask[token * mask_row + j] != 0 where a new
+                          token sees new token j of its sequence */
+  int64_t mask_row;
+  void *out;           /* forward: [token][q head][d], type dtype */
+  int64_t out_tok, out_head;
+  float *lse;          /* [token][q head]: natural log of the sum of
+                          exp(score); written by forward, read by weights */
+  int64_t lse_tok, lse_head;
+  const float *before; /* weights: [sequence][kv head][key] */
+  int64_t before_seq, before_head;
+  float *weights;      /* weights: the same, keys contiguous */
+  int64_t weights_seq, weights_head;
+  int32_t width;       /* weights: keys of a row; >= the longest sequence */
+  int32_t fill;        /* weights: 1 = positions behind a sequence's end are
+                          written too (before's value, or 0) */
+  void *workspace;     /* device, info.workspace_bytes, 16-byte aligned */
+  uint64_t workspace_bytes;
+} cascade_attn_args_t;
+
+/* softmax(scale q k^T) v per query head, over every cached token and, of
+ * the new tokens of its own sequence, those up to itself (or, with a plan
+ * for trees, those its mask row names).  A row that sees nothing is 0 with
+ * lse -inf. */
+int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
+                         const cascade_attn_args_t *args, void *stream);
+
+/* weights[b][kv head][key] = before + the sum over the last `window` new
+ * tokens and the query heads of the group of exp(score - lse), for the
+ * tokens that see the key (causally). */
+int cascade_attn_weights(const cascade_attn_plan_info_t *plan,
+                         const cascade_attn_args_t *args, void *stream);
+
+/* Which tokens of a cache to keep: per row of weights (three leading
+ * dimensions, strides in elements, `width` contiguous weights) the first
+ * `sink` tokens, the last `recent`, and those of the largest weights, ties
+ * to the lowest position; NaN ranks with -inf.  d_lengths (per index of the
+ * first dimension, or NULL: all `width`) is clamped to [0, width].  d_keep
+ * receives `budget` positions per row, ascending; a row of fewer tokens
+ * keeps them all and ends in -1. */
+int cascade_kv_evict_select(const float *d_weights, const int64_t dims[3],
+                            const int64_t strides[3], int32_t width,
+                            const int32_t *d_lengths, int32_t budget,
+                            int32_t recent, int32_t sink, int32_t *d_keep,
+                            void *stream);
+
+/* Gathers the kept rows of K and V: src (HOST array) holds 2 x items
+ * descriptors (item 0's K, V, item 1's, ...) of [heads][tokens][head_dim]
+ * tensors with elements of elem_bytes (2 or 4), an item being one layer of
+ * one cache.  d_keep holds [items / layers][heads][kept] positions (`layers`
+ * consecutive items share theirs; 1: each has its own).  d_out receives
+ * [items][2][heads][kept][head_dim].  A position outside [0, seq) gives a
+ * row of zeros.  With d_table the sources are pages: token j of item i is
+ * token j % page of page d_table[i * table_row + j / page], pages
+ * stride_page elements apart; a table entry outside [0, pages), or a
+ * position behind the table's table_cols entries, gives zeros. */
+int cascade_kv_evict_gather(const cascade_kv_tensor_t *src, uint32_t items,
+                            uint32_t layers, uint32_t heads, uint32_t seq,
+                            uint32_t head_dim, uint32_t elem_bytes,
+                            const int32_t *d_keep, uint32_t kept,
+                            const int32_t *d_table, int64_t table_row,
+                            int64_t table_cols, int64_t stride_page,
+                            uint32_t page, uint32_t pages, void *d_out,
+                            void *stream);
+
+/* Waits inside attention kernels that gave up (0 unless the hardware or the
+ * library is broken).  Synchronous. */
+int cascade_diag_attn_timeouts(uint64_t *count);
+
 /* n device-to-device block copies in one launch (the pool copy that
  * GPUBackend::put/get do with cudaMemcpyAsync, gpu_backend.cu:298-308,
  * 362-377). */

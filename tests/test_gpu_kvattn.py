@@ -1,0 +1,559 @@
+"""The attention operators over KV caches (cascade_b200.kvattn) against plain
+formulas in 64 bits.
+
+Tolerances, from the roundings that the kernels make (u = eps / 2 of the
+16-bit type): the output is rounded once (u |o|), the softmax weights are
+rounded to the type before they multiply V (u A, A = sum p |v|), scores and
+sums are in FP32.  A score's error is at most d = dim 2^-23 max_j scale sum
+|q k|, which moves a weight by a factor of up to exp(2 d); sums over n keys
+add n 2^-23 at most, and the exponential 2^-21."""
+import math
+
+import pytest
+import torch
+
+from cascade_b200 import kvattn
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def paged(gen, lengths, page, heads, dim, dt, cols=None, spare=2):
+    """Random pages (K and V interleaved as a loaded block has them), a
+    shuffled table, and each sequence's (k, v) [heads, tokens, dim]."""
+    counts = [-(-n // page) for n in lengths]
+    P = sum(counts) + spare
+    pool = torch.randn(P, 2, heads, page, dim, generator=gen,
+                       device=DEV).to(dt)
+    ids = torch.randperm(P, generator=gen, device=DEV).to(torch.int32)
+    cols = max(counts + [1]) if cols is None else cols
+    table = torch.full((len(lengths), cols), -1, dtype=torch.int32,
+                       device=DEV)
+    at = 0
+    for b, c in enumerate(counts):
+        table[b, :c] = ids[at:at + c]
+        at += c
+    return pool, table
+
+
+def cached_rows(pool, table, b, n, page):
+    tok = torch.arange(n, device=DEV)
+    ids = table[b].long()[tok // page] if n else tok
+    ok = (ids >= 0) & (ids < pool.shape[0])
+    rows = pool[ids.clamp(0, pool.shape[0] - 1), :, :, tok % page]
+    return rows[:, 0], rows[:, 1], ok      # [n, heads, dim]
+
+
+class Case:
+    def __init__(self, new, cached, heads, kv_heads, dim, dtype, page=16,
+                 tree=False, seed=0, scale=None, mask=None, qmul=1.5):
+        g = torch.Generator(device=DEV).manual_seed(seed + 1)
+        self.new, self.cached, self.page = new, cached, page
+        self.H, self.G, self.D, self.dt = heads, kv_heads, dim, DT[dtype]
+        n = sum(new)
+        qkv = torch.randn(n, heads + 2 * kv_heads, dim, generator=g,
+                          device=DEV)
+        qkv[:, :heads] *= qmul
+        qkv = qkv.to(self.dt)
+        self.q = qkv[:, :heads]
+        self.k = qkv[:, heads:heads + kv_heads]
+        self.v = qkv[:, heads + kv_heads:]
+        self.pool, self.table = paged(g, cached, page, kv_heads, dim,
+                                      self.dt)
+        self.tree, self.scale = tree, scale
+        if tree and mask is None:
+            m = torch.rand(n, max(new), generator=g, device=DEV) < 0.5
+            at = 0
+            for c in new:
+                i = torch.arange(c, device=DEV)
+                m[at + i, i] = True
+                at += c
+            mask = m
+        self.mask = mask
+
+    def plan(self, cls=kvattn.AttentionPlan, **kw):
+        if cls is kvattn.AttentionPlan:
+            kw["tree"] = self.tree
+        return cls(self.new, self.cached, q_heads=self.H, kv_heads=self.G,
+                   head_dim=self.D, page_size=self.page, device=DEV, **kw)
+
+    @property
+    def pages(self):
+        return self.pool[:, 0], self.pool[:, 1]
+
+    def run(self, plan=None, **kw):
+        plan = plan or self.plan()
+        if self.tree:
+            return kvattn.tree_attention(plan, self.q, self.k, self.v,
+                                         self.mask, self.pages, self.table,
+                                         scale=self.scale, **kw)
+        return kvattn.prompt_attention(plan, self.q, self.k, self.v,
+                                       self.pages, self.table,
+                                       scale=self.scale, **kw)
+
+    def sequences(self):
+        """(b, first token, keys k, v [heads, keys, dim], visible [new,
+        keys]) in 64 bits."""
+        at = 0
+        for b, (n, c) in enumerate(zip(self.new, self.cached)):
+            ck, cv, ok = cached_rows(self.pool, self.table, b, c, self.page)
+            k = torch.cat([ck, self.k[at:at + n]]).double().transpose(0, 1)
+            v = torch.cat([cv, self.v[at:at + n]]).double().transpose(0, 1)
+            vis = torch.zeros(n, c + n, dtype=torch.bool, device=DEV)
+            vis[:, :c] = ok
+            if self.tree:
+                vis[:, c:] = self.mask[at:at + n, :n].bool()
+            else:
+                i = torch.arange(n, device=DEV)
+                vis[:, c:] = i[None, :] <= i[:, None]
+            yield b, at, k, v, vis
+            at += n
+
+    def scores(self, at, n, k, vis):
+        s = self.scale or 1 / math.sqrt(self.D)
+        q = self.q[at:at + n].double().transpose(0, 1)
+        kk = k.repeat_interleave(self.H // self.G, 0)
+        sc = s * q @ kk.transpose(1, 2)
+        size = s * q.abs() @ torch.nan_to_num(kk, 0, 0, 0).abs().transpose(
+            1, 2)
+        d = self.D * 2.0 ** -23 * size.amax(-1) if size.shape[-1] else \
+            size.sum(-1)
+        return sc.masked_fill(~vis, -math.inf), d
+
+
+def check_forward(case, out, lse):
+    u = torch.finfo(case.dt).eps / 2
+    for b, at, k, v, vis in case.sequences():
+        n = case.new[b]
+        if n == 0:
+            continue
+        s, d = case.scores(at, n, k, vis)
+        want_lse = torch.logsumexp(s, -1)                  # [H, n]
+        empty = ~vis.any(-1)
+        p = torch.softmax(s, -1).masked_fill(empty[:, None], 0.0)
+        vv = v.repeat_interleave(case.H // case.G, 0)
+        o, mag = p @ vv, p @ vv.abs()
+        slack = 2 * d + s.shape[-1] * 2.0 ** -23 + 2.0 ** -20
+        got = out[at:at + n].double().transpose(0, 1)
+        tol = u * o.abs() + (u + slack[..., None]) * mag * (1 + 2 * u) + 1e-30
+        tol = tol + torch.finfo(case.dt).smallest_normal * u * 2 + \
+            (6e-8 if case.dt is torch.float16 else 0)
+        bad = (got - o).abs() > tol
+        assert not bad.any(), (b, bad.nonzero()[:5].tolist(),
+                               float(((got - o).abs() / tol).max()))
+        gl = lse[at:at + n].double().t()
+        assert (gl[:, empty] == -math.inf).all()
+        assert (got[:, empty] == 0).all()
+        tl = d + s.shape[-1] * 2.0 ** -23 + 2.0 ** -20 + \
+            want_lse.abs() * 2.0 ** -21
+        diff = (gl - want_lse)[:, ~empty].abs()
+        assert (diff <= tl[:, ~empty]).all(), (b, float(diff.max()))
+
+
+SHAPES = [
+    # new, cached, heads, kv heads, dim, page
+    ([1], [0], 4, 1, 64, 16),
+    ([1], [1], 8, 8, 128, 1),
+    ([5, 0, 1, 130], [0, 9, 0, 0], 4, 2, 64, 16),
+    ([1, 1, 1], [127, 128, 129], 32, 8, 128, 16),
+    ([33, 7], [300, 64], 7, 1, 128, 37),
+    ([128, 64, 129], [0, 1, 255], 2, 2, 64, 8),
+    ([300], [77], 8, 2, 128, 16),
+    ([1000, 17], [0, 500], 4, 4, 128, 64),
+    ([600, 1], [1500, 3], 16, 2, 64, 24),
+    ([1], [20000], 8, 1, 128, 16),
+    ([2, 1], [9000, 4000], 12, 4, 64, 37),
+]
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_forward(shape, dtype, tree):
+    new, cached, H, G, D, page = SHAPES[shape]
+    c = Case(new, cached, H, G, D, dtype, page, tree, seed=shape)
+    check_forward(c, *c.run())
+    assert kvattn.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("scale", [0.01, 0.5])
+def test_scale(scale):
+    c = Case([40, 3], [200, 90], 4, 2, 128, "fp16", scale=scale, seed=3)
+    check_forward(c, *c.run())
+
+
+def test_large_scores_keep_their_weight():
+    # scores far beyond exp's range: the running maximum has to move
+    c = Case([50, 1], [500, 700], 4, 2, 64, "bf16", seed=4, qmul=1.0)
+    c.q = c.q * 100
+    check_forward(c, *c.run())
+    c = Case([70], [300], 4, 1, 128, "fp16", seed=5)
+    # scores that rise along the keys: the maximum grows in every tile
+    ramp = torch.arange(300, device=DEV).view(-1, 1) / 8
+    c.q = c.q.clone()
+    c.q[:] = 1.0
+    ids = c.table[0].long()[torch.arange(300, device=DEV) // 16]
+    c.pool[ids, 0, 0, torch.arange(300, device=DEV) % 16] = ramp.to(c.dt)
+    check_forward(c, *c.run())
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (64, 1)])
+def test_rows_without_any_key(heads, kv_heads):
+    # no cached token and an all-false mask row: zeros and -inf
+    new = [6, 40, 3]
+    mask = torch.zeros(sum(new), 40, dtype=torch.bool, device=DEV)
+    mask[6:46] = torch.rand(40, 40, device=DEV) < 0.2
+    mask[10] = False
+    c = Case(new, [0, 0, 5], heads, kv_heads, 64, "bf16", tree=True,
+             mask=mask, seed=6)
+    out, lse = c.run()
+    assert (lse[:6] == -math.inf).all() and (out[:6] == 0).all()
+    assert (lse[46:] > -math.inf).all()
+    check_forward(c, out, lse)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("heads", [2, 16])
+def test_pages_that_are_gone_count_as_unseen(tree, heads):
+    c = Case([3, 20, 1], [500, 300, 64], heads, 2, 128, "fp16", tree=tree,
+             seed=7)
+    c.table[0, 3:9] = -1
+    c.table[1, 0] = -5
+    c.table[1, 7] = c.pool.shape[0]            # behind the last page
+    c.table[2] = 2 ** 31 - 1
+    check_forward(c, *c.run())
+
+
+def _poison(c, b, toks, value, which):
+    """Writes value into K or V of new tokens of sequence b."""
+    at = sum(c.new[:b])
+    t = (c.k, c.v)[which]
+    for i in toks:
+        t[at + i, :, ::3] = value
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("heads", [2, 8, 32])
+def test_masked_infinities_do_not_leak(value, which, heads):
+    # token 9 of a prompt holds inf or NaN: earlier rows do not see it, later
+    # ones do
+    c = Case([30, 12], [40, 0], heads, 2, 64, "bf16", seed=8)
+    clean, clean_lse = c.run()
+    _poison(c, 0, [9, 20], value, which)
+    out, lse = c.run()
+    assert torch.equal(out[:9], clean[:9])
+    assert torch.equal(lse[:9], clean_lse[:9])
+    assert torch.equal(out[30:], clean[30:])
+    if which == 1:
+        assert torch.equal(lse, clean_lse)
+        got = out[9:30, :, ::3].float()
+        if math.isnan(value):
+            assert got.isnan().all()
+        else:
+            assert (got == value).all()
+        rest = torch.ones(64, dtype=torch.bool, device=DEV)
+        rest[::3] = False
+        assert torch.equal(out[..., rest], clean[..., rest])
+
+
+def test_masked_infinities_of_a_tree():
+    c = Case([8, 70], [20, 300], 8, 2, 128, "fp16", tree=True, seed=9)
+    c.mask[:, 5] = False
+    c.mask[3, 5] = True
+    clean, clean_lse = c.run()
+    _poison(c, 0, [5], math.inf, 1)
+    _poison(c, 1, [5], math.nan, 1)
+    out, lse = c.run()
+    seen = c.mask[:, 5]
+    assert torch.equal(out[~seen], clean[~seen])
+    assert torch.equal(lse, clean_lse)
+    assert (out[3, :, ::3] == math.inf).all()
+
+
+def test_all_scores_minus_infinity_is_nan():
+    # keys are seen, but no score is above -inf: 0 / 0, not an empty row
+    c = Case([2], [40], 2, 1, 64, "bf16", seed=10)
+    c.q = torch.full_like(c.q, 1.0)
+    c.k = torch.full_like(c.k, -math.inf)
+    c.pool[:, 0] = -math.inf
+    out, lse = c.run()
+    assert out.isnan().all()
+
+
+def test_scores_of_minus_infinity_weigh_nothing():
+    c = Case([1], [600], 2, 1, 64, "bf16", seed=10)
+    c.q = torch.full_like(c.q, 1.0)
+    clean = c.run()
+    ids = c.table[0].long()
+    c.pool[ids[:20], 0] = -math.inf
+    c2 = c.run()
+    c.table[0, :20] = -1
+    want = c.run()
+    assert torch.equal(c2[0], want[0]) and torch.equal(c2[1], want[1])
+    assert not torch.equal(clean[0], want[0])
+
+
+def test_layouts_and_untouched_rows():
+    # q, out and lse as slices of larger tensors, K and V as a permuted
+    # [heads, tokens, dim] cache, more packed rows than the plan has
+    c = Case([40, 9], [100, 33], 8, 2, 64, "fp16", seed=11)
+    want, want_lse = c.run()
+    n, extra = 49, 7
+    big = torch.zeros(n + extra, 3, 8, 64, dtype=c.dt, device=DEV)
+    big[:n, 1] = c.q
+    kk = torch.zeros(2, n + extra, 80, dtype=c.dt, device=DEV)
+    vv = torch.zeros_like(kk)
+    kk[:, :n, 8:72] = c.k.transpose(0, 1)
+    vv[:, :n, 16:80] = c.v.transpose(0, 1)
+    out = torch.full((8, n + extra, 72), 7.0, dtype=c.dt, device=DEV)
+    lse = torch.full((8, n + extra), 7.0, device=DEV)
+    o, l = kvattn.prompt_attention(
+        c.plan(), big[:, 1], kk[:, :, 8:72].transpose(0, 1),
+        vv[:, :, 16:80].transpose(0, 1), c.pages, c.table,
+        out=out[:, :, :64].transpose(0, 1), lse=lse.t())
+    assert o.data_ptr() == out.data_ptr()
+    assert torch.equal(o[:n], want) and torch.equal(l[:n], want_lse)
+    assert (out[:, n:] == 7).all() and (out[:, :, 64:] == 7).all()
+    assert (lse[:, n:] == 7).all()
+
+
+def test_contiguous_cache_as_one_page_each():
+    # a [sequences, heads, capacity, dim] static cache is a page a sequence
+    c = Case([1, 1, 1], [0, 70, 200], 8, 2, 128, "bf16", page=256, seed=12)
+    c.table[:] = torch.tensor([[2], [0], [1]], dtype=torch.int32)
+    check_forward(c, *c.run())
+
+
+def test_same_result_twice_and_on_other_streams_and_graphs():
+    c = Case([1] * 5, [3000, 10, 700, 5000, 129], 32, 8, 128, "bf16", seed=13)
+    plan = c.plan()
+    assert plan._info.merges > 0
+    want, want_lse = c.run(plan)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(c.run(plan))
+    torch.cuda.synchronize()
+    for o, l in got:
+        assert torch.equal(o, want) and torch.equal(l, want_lse)
+    graphs, outs = [], []
+    for s in streams[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(c.run(plan))
+        graphs.append(g)
+    for o, l in outs:
+        o.zero_()
+    for s, g in zip(streams, graphs):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, l in outs:
+        assert torch.equal(o, want) and torch.equal(l, want_lse)
+
+
+def test_offsets_beyond_32_bits():
+    # a pool whose last pages start more than 2^32 bytes in
+    heads, page, dim = 8, 64, 128
+    P = (1 << 32) // (2 * heads * page * dim * 2) + 40
+    pool = torch.zeros(P, 2, heads, page, dim, dtype=torch.bfloat16,
+                       device=DEV)
+    c = Case([1, 2], [600, 300], 16, heads, dim, "bf16", page=page, seed=14)
+    ids = torch.randperm(30, device=DEV)[:c.pool.shape[0]] + (P - 31)
+    pool[ids] = c.pool
+    c.pool = pool
+    c.table = torch.where(c.table >= 0, ids[c.table.clamp(min=0).long()]
+                          .to(torch.int32), c.table)
+    check_forward(c, *c.run())
+
+
+def test_empty_batches():
+    for new, cached in (([], []), ([0, 0], [5, 0])):
+        plan = kvattn.AttentionPlan(new, cached, q_heads=4, kv_heads=2,
+                                    head_dim=64, page_size=16, device=DEV)
+        q = torch.zeros(0, 4, 64, dtype=torch.float16, device=DEV)
+        k = torch.zeros(0, 2, 64, dtype=torch.float16, device=DEV)
+        pages = (torch.zeros(1, 2, 16, 64, dtype=torch.float16,
+                             device=DEV),) * 2
+        table = torch.zeros(len(new), 1, dtype=torch.int32, device=DEV)
+        out, lse = kvattn.prompt_attention(plan, q, k, k, pages, table)
+        assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
+def test_refusals():
+    c = Case([4, 2], [30, 5], 4, 2, 64, "fp16", seed=15)
+    plan, tplan = c.plan(), kvattn.AttentionPlan(
+        c.new, c.cached, q_heads=4, kv_heads=2, head_dim=64, page_size=16,
+        tree=True, device=DEV)
+    mask = torch.ones(6, 4, dtype=torch.bool, device=DEV)
+
+    def call(plan=plan, q=c.q, k=c.k, v=c.v, pages=c.pages, table=c.table,
+             **kw):
+        return kvattn.prompt_attention(plan, q, k, v, pages, table, **kw)
+    call()
+    for bad in (dict(q=c.q.float()), dict(q=c.q[:5]), dict(k=c.k[:, :1]),
+                dict(q=c.q[..., :32]), dict(k=c.k.bfloat16()),
+                dict(q=c.q.cpu()), dict(plan=tplan), dict(pages=None),
+                dict(table=None), dict(table=c.table.long()),
+                dict(table=c.table[:1]), dict(table=c.table[:, :1]),
+                dict(table=c.table.cpu()), dict(pages=(c.pages[0], None)),
+                dict(pages=(c.pages[0], c.pages[1][:, :, :8])),
+                dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                dict(scale=math.inf),
+                dict(out=torch.empty(6, 4, 64, device=DEV)),
+                dict(out=torch.empty(1, 4, 64, dtype=c.dt, device=DEV)
+                     .expand(6, 4, 64)),
+                dict(lse=torch.empty(6, 4, dtype=torch.float64, device=DEV)),
+                dict(plan=c.plan(kvattn.WeightsPlan))):
+        with pytest.raises((ValueError, TypeError)):
+            call(**bad)
+    flat = torch.zeros(6 * 4 * 64 + 1, dtype=c.dt, device=DEV)
+    with pytest.raises(ValueError, match="16-byte"):
+        call(q=flat[1:].view(6, 4, 64))
+    with pytest.raises(RuntimeError, match="backward"):
+        call(q=c.q.clone().requires_grad_())
+    with torch.no_grad():
+        call(q=c.q.clone().requires_grad_())
+    for bad in (None, mask[:5], mask[:, :3], mask.float(), mask.cpu()):
+        with pytest.raises(ValueError):
+            kvattn.tree_attention(tplan, c.q, c.k, c.v, bad, c.pages, c.table)
+    with pytest.raises(ValueError):
+        kvattn.tree_attention(plan, c.q, c.k, c.v, mask, c.pages, c.table)
+    for kw in (dict(new_lengths=[1.5]), dict(new_lengths=[[1]]),
+               dict(new_lengths=[1], cached_lengths=[1, 2]),
+               dict(new_lengths=[-1]), dict(device="cpu")):
+        a = dict(new_lengths=[1], q_heads=4, kv_heads=2, head_dim=64,
+                 page_size=16, device=DEV)
+        a.update(kw)
+        with pytest.raises((ValueError, TypeError)):
+            kvattn.AttentionPlan(a.pop("new_lengths"),
+                                 a.pop("cached_lengths", None), **a)
+
+
+# ----------------------------------------------------------------- weights
+def check_weights(case, lse, window, got, before):
+    for b, at, k, v, vis in case.sequences():
+        n, keys = case.new[b], case.new[b] + case.cached[b]
+        base = before[b, :, :keys].double() if before is not None else \
+            torch.zeros(case.G, keys, dtype=torch.float64, device=DEV)
+        g = got[b, :, :keys].double()
+        if n == 0:
+            assert torch.equal(g, base)
+            continue
+        s, d = case.scores(at, n, k, vis)
+        ll = lse[at:at + n].double().t()
+        first = max(0, n - window)
+        p = torch.exp(s - ll[..., None])[:, first:]
+        p = p.nan_to_num(0.0) if (ll == -math.inf).any() else p
+        # a weight's exponent: the score's error, and that of the 32-bit
+        # subtraction of lse (both scaled by log2 e and back: 4 roundings)
+        rel = d[:, first:, None] + 2.0 ** -22 * (
+            4 + 2 * ll[:, first:, None].abs() + s[:, first:].abs()
+            .nan_to_num(0, posinf=0))
+        w = p.reshape(case.G, -1, keys).sum(1)
+        tol = (p * rel).reshape(case.G, -1, keys).sum(1)
+        rows = p.shape[1] * case.H // case.G
+        # sums: 128 rows by themselves, then the chunks and the parts
+        tol = tol + w * 2.0 ** -24 * (128 + rows / 128 + 8) + \
+            base.abs() * 2.0 ** -24
+        want = base + w
+        want = torch.where(vis[first:].any(0) if n else vis, want, base)
+        bad = (g - want).abs() > tol + 1e-12
+        assert not bad.any(), (b, bad.nonzero()[:5].tolist(),
+                               float((g - want).abs().max()))
+
+
+@pytest.mark.parametrize("window", [None, 1, 33])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_weights(shape, dtype, window):
+    new, cached, H, G, D, page = SHAPES[shape]
+    c = Case(new, cached, H, G, D, dtype, page, seed=shape + 50)
+    out, lse = c.run()
+    width = max(a + b for a, b in zip(new, cached)) + 3
+    before = torch.rand(len(new), G, width, device=DEV)
+    plan = c.plan(kvattn.WeightsPlan, window=window)
+    w = kvattn.attention_weights(plan, c.q, c.k, lse, c.pages[0], c.table,
+                                 add_to=before)
+    check_weights(c, lse, window or 10 ** 9, w, before)
+    for b, (n, m) in enumerate(zip(new, cached)):
+        assert torch.equal(w[b, :, n + m:], before[b, :, n + m:])
+    # each query's weights sum to 1 over the keys it sees
+    if window is None:
+        w0 = kvattn.attention_weights(plan, c.q, c.k, lse, c.pages[0],
+                                      c.table)
+        assert w0.shape[2] == width - 3
+        check_weights(c, lse, 10 ** 9, w0, None)
+        for b, n in enumerate(new):
+            assert abs(float(w0[b].double().sum()) - n * H) < 1e-3 * n * H \
+                + 1e-6
+            assert (w0[b, :, n + cached[b]:] == 0).all()
+    assert kvattn.wait_timeouts() == 0
+
+
+def test_weights_in_place_leaves_the_rest():
+    c = Case([3, 1], [300, 20], 8, 2, 128, "fp16", seed=60)
+    out, lse = c.run()
+    plan = c.plan(kvattn.WeightsPlan)
+    args = (plan, c.q, c.k, lse, c.pages[0], c.table)
+    big = torch.rand(2, 4, 400, device=DEV)
+    acc = big[:, 1:3, 5:320]
+    keep = big.clone()
+    want = kvattn.attention_weights(*args, add_to=acc)
+    got = kvattn.attention_weights(*args, add_to=acc, out=acc)
+    assert got.data_ptr() == acc.data_ptr()
+    for b, n in enumerate([303, 21]):
+        assert torch.equal(acc[b, :, :n], want[b, :, :n])
+        assert torch.equal(acc[b, :, n:], keep[b, 1:3, 5 + n:320])
+    big[:, 1:3, 5:320] = keep[:, 1:3, 5:320]
+    assert torch.equal(big, keep)
+
+
+def test_weights_of_gone_pages_and_captured():
+    c = Case([40, 2], [200, 600], 4, 2, 64, "bf16", seed=61)
+    c.table[1, 2:5] = -1
+    c.table[0, 0] = c.pool.shape[0] + 3
+    out, lse = c.run()
+    plan = c.plan(kvattn.WeightsPlan, window=20)
+    before = torch.rand(2, 2, 700, device=DEV)
+    w = kvattn.attention_weights(plan, c.q, c.k, lse, c.pages[0], c.table,
+                                 add_to=before)
+    check_weights(c, lse, 20, w, before)
+    assert torch.equal(w[1, :, 32:80], before[1, :, 32:80])
+    assert torch.equal(w[0, :, :16], before[0, :, :16])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        w2 = kvattn.attention_weights(plan, c.q, c.k, lse, c.pages[0],
+                                      c.table, add_to=before)
+    w2.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(w, w2)
+
+
+def test_weights_refusals():
+    c = Case([4, 2], [30, 5], 4, 2, 64, "fp16", seed=62)
+    out, lse = c.run()
+    plan = c.plan(kvattn.WeightsPlan)
+    w = torch.zeros(2, 2, 34, device=DEV)
+
+    def call(plan=plan, lse=lse, kp=c.pages[0], **kw):
+        return kvattn.attention_weights(plan, c.q, c.k, lse, kp, c.table,
+                                        **kw)
+    call(add_to=w)
+    for bad in (dict(plan=c.plan()), dict(lse=lse.double()),
+                dict(lse=lse[:5]), dict(kp=None), dict(add_to=w[:, :, :33]),
+                dict(add_to=w.double()), dict(out=w[:1]),
+                dict(out=torch.zeros(1, 2, 34, device=DEV).expand(2, 2, 34)),
+                dict(out=w.transpose(1, 2)), dict(scale=0.0)):
+        with pytest.raises((ValueError, TypeError)):
+            call(**bad)
+    with pytest.raises(ValueError):
+        c.plan(kvattn.WeightsPlan, window=0)
