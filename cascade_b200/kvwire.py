@@ -259,19 +259,31 @@ def _sources(caches):
 
 
 def store_kv_caches(store, block_ids: Sequence, caches: Sequence,
-                    is_prefix=None):
+                    is_prefix=None, weights=None, budget=None, recent=0,
+                    sink=0):
     """KVCacheStore.store (kv_manager.py:116-127) for a batch, without host
     copies.  ``store``: a CascadeStore.  When every wire block fits the HBM
     pool as a raw payload, one store call (cascade_store_put_kv_batch)
     serialises each cache straight into its pool slot; otherwise the caches
     are serialised in one launch and put with put_batch.  Returns the
-    per-block put status codes."""
+    per-block put status codes.
+
+    With ``weights`` (the attention each token received, float32 [n, layers,
+    kv heads, seq] or [n, kv heads, seq]) the caches are first cut to
+    ``budget`` tokens per head by kvattn.evict_kv_caches: the stored blocks
+    are wire blocks of min(budget, seq) tokens."""
     import numpy as np
     if len(block_ids) != len(caches):
         raise ValueError("one id per cache")
+    if (weights is None) != (budget is None):
+        raise ValueError("weights and budget go together")
     n = len(caches)
     if n == 0:
         return []
+    if weights is not None:
+        from . import kvattn
+        caches = kvattn.cache_views(kvattn.evict_kv_caches(
+            caches, weights, budget, recent, sink)[0])
     L, H, S, D, dev, dt, src = _sources(caches)
     keys = np.frombuffer(b"".join(store._key(b) for b in block_ids),
                          dtype=np.uint8).copy()
@@ -291,6 +303,34 @@ def store_kv_caches(store, block_ids: Sequence, caches: Sequence,
                            return_status=True)[1]
 
 
+def load_kv_pages(store, block_ids: Sequence, layers: int, heads: int,
+                  seq: int, head_dim: int):
+    """load_kv_caches into one tensor of pages: (pages, found), pages FP16
+    [n, layers, 2 (K, V), heads, seq, head_dim] and found a bool array.
+    pages[:, l, 0] and pages[:, l, 1] are layer l's K and V pages for
+    cascade_b200.kvattn, page i being block_ids[i].  Pages whose id was not
+    found hold nothing: a page table must not name them."""
+    import numpy as np
+    import torch
+    n = len(block_ids)
+    dev = torch.device(f"cuda:{store._device}")
+    L, H, S, D = layers, heads, seq, head_dim
+    outs = torch.empty((n, L, 2, H, S, D), dtype=torch.float16, device=dev)
+    found = np.zeros(n, np.uint8)
+    if n == 0:
+        return outs, found.astype(bool)
+    views = [outs[i, l, kv] for i in range(n) for l in range(L)
+             for kv in range(2)]
+    dst = _descriptors(views, dev)
+    keys = np.frombuffer(b"".join(store._key(b) for b in block_ids),
+                         dtype=np.uint8).copy()
+    nf = ctypes.c_uint64(0)
+    check(_lib.load().cascade_store_get_kv_batch(
+        store._h, n, keys.ctypes.data, L, H, S, D, dst.data_ptr(),
+        found.ctypes.data, _stream(dev), ctypes.byref(nf)))
+    return outs, found.astype(bool)
+
+
 def load_kv_caches(store, block_ids: Sequence, layers: int, heads: int,
                    seq: int, head_dim: int) -> list:
     """KVCacheStore.load (kv_manager.py:135-156) for a batch of caches of a
@@ -299,24 +339,10 @@ def load_kv_caches(store, block_ids: Sequence, layers: int, heads: int,
     of the pool into fresh per-layer tensors.  Returns, per id, the tuple of
     (K, V) FP16 tensors [1, heads, seq, dim] per layer, or None when the
     store does not hold that id with the wire size of that shape."""
-    import numpy as np
-    import torch
-    n = len(block_ids)
-    if n == 0:
+    if len(block_ids) == 0:
         return []
-    dev = torch.device(f"cuda:{store._device}")
-    L, H, S, D = layers, heads, seq, head_dim
-    outs = torch.empty((n, L, 2, 1, H, S, D), dtype=torch.float16,
-                       device=dev)
-    views = [outs[i, l, kv, 0] for i in range(n) for l in range(L)
-             for kv in range(2)]
-    dst = _descriptors(views, dev)
-    keys = np.frombuffer(b"".join(store._key(b) for b in block_ids),
-                         dtype=np.uint8).copy()
-    found = np.zeros(n, np.uint8)
-    nf = ctypes.c_uint64(0)
-    check(_lib.load().cascade_store_get_kv_batch(
-        store._h, n, keys.ctypes.data, L, H, S, D, dst.data_ptr(),
-        found.ctypes.data, _stream(dev), ctypes.byref(nf)))
-    return [tuple((outs[i, l, 0], outs[i, l, 1]) for l in range(L))
-            if found[i] else None for i in range(n)]
+    outs, found = load_kv_pages(store, block_ids, layers, heads, seq,
+                                head_dim)
+    outs = outs.unsqueeze(3)
+    return [tuple((outs[i, l, 0], outs[i, l, 1]) for l in range(layers))
+            if found[i] else None for i in range(len(block_ids))]

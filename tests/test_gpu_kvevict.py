@@ -236,3 +236,101 @@ def test_evict_refusals():
               (kp, kp, t, n.long(), w), (kp, kp, t, n, w[:, :1])):
         with pytest.raises(ValueError):
             kvattn.evict_pages(*a, 4)
+
+
+# ------------------------------------------------------- a run of them all
+def _store(gib=1):
+    cfg = cc.CascadeConfig()
+    cfg.gpu_capacity_bytes = gib << 30
+    cfg.shm_capacity_bytes = 64 << 20
+    return cc.CascadeStore(cfg)
+
+
+def test_store_attend_weigh_evict_store_attend():
+    """A prefix in the store as 16-token blocks: load its pages, run a
+    prompt's rest and a draft tree over them, weigh the tokens, evict, store
+    the shorter cache, and attend over that."""
+    L, G, H, D, page = 2, 4, 16, 128, 16
+    n_blocks, tail = 12, 5                      # cached 11 * 16 + 5 tokens
+    cached = (n_blocks - 1) * page + tail
+    store = _store()
+    blocks = [tuple((torch.randn(1, G, page, D, device=DEV).half(),
+                     torch.randn(1, G, page, D, device=DEV).half())
+                    for _ in range(L)) for _ in range(n_blocks)]
+    ids = [f"prefix-{i}" for i in range(n_blocks)]
+    assert (np.asarray(kvwire.store_kv_caches(store, ids, blocks)) == 0).all()
+    order = [int(i) for i in torch.randperm(n_blocks)]
+    pages, found = kvwire.load_kv_pages(store, [ids[i] for i in order], L, G,
+                                        page, D)
+    assert found.all() and pages.shape == (n_blocks, L, 2, G, page, D)
+    table = torch.tensor([[order.index(i) for i in range(n_blocks)]],
+                         dtype=torch.int32, device=DEV)
+    missing, found = kvwire.load_kv_pages(store, ["no"], L, G, page, D)
+    assert not found.any()
+    new = 9
+    kw = dict(q_heads=H, kv_heads=G, head_dim=D, page_size=page, device=DEV)
+    plan = kvattn.AttentionPlan([new], [cached], **kw)
+    wplan = kvattn.WeightsPlan([new], [cached], window=4, **kw)
+    full, w_all = [], []
+    for l in range(L):
+        q, k, v = (torch.randn(new, h, D, device=DEV).half()
+                   for h in (H, G, G))
+        kv = pages[:, l, 0], pages[:, l, 1]
+        out, lse = kvattn.prompt_attention(plan, q, k, v, kv, table)
+        w = kvattn.attention_weights(wplan, q, k, lse, kv[0], table)
+        # the plain forms over the blocks that were stored
+        kk = torch.cat([b[l][0][0] for b in blocks], 1)[:, :cached]
+        vv = torch.cat([b[l][1][0] for b in blocks], 1)[:, :cached]
+        kk = torch.cat([kk, k.transpose(0, 1)], 1).double()
+        vv = torch.cat([vv, v.transpose(0, 1)], 1).double()
+        s = q.double().transpose(0, 1) @ kk.repeat_interleave(
+            H // G, 0).transpose(1, 2) / math.sqrt(D)
+        s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(
+            cached + 1), -math.inf)
+        p = s.softmax(-1)
+        ref = (p @ vv.repeat_interleave(H // G, 0)).transpose(0, 1)
+        # |v| <= 5.5; the weights and the output are rounded to fp16 once
+        assert (out.double() - ref).abs().max() < 2 * 2.0 ** -11 * 5.5
+        # a score is off by 128 2^-23 * 10 at most, a sum of weights is <= 16
+        wref = p[:, -4:].reshape(G, -1, cached + new).sum(1)
+        assert (w[0].double() - wref).abs().max() < 16 * 1.6e-4
+        full.append((kk[:, :cached].half(), vv[:, :cached].half()))
+        w_all.append(w[0, :, :cached])
+    # evict from the assembled cache while storing it
+    cache = tuple((k[None], v[None]) for k, v in full)
+    weights = torch.stack(w_all)[None]
+    budget = 64
+    st = kvwire.store_kv_caches(store, ["short"], [cache], weights=weights,
+                                budget=budget, recent=8, sink=2)
+    assert (np.asarray(st) == 0).all()
+    short = kvwire.load_kv_caches(store, ["short"], L, G, budget, D)[0]
+    kv, keep = kvattn.evict_kv_caches([cache], weights, budget, 8, 2)
+    assert (keep[..., :2] == torch.arange(2, device=DEV)).all()
+    for l in range(L):
+        assert torch.equal(short[l][0][0], kv[0, l, 0])
+        assert torch.equal(short[l][1][0], kv[0, l, 1])
+    # one page of the same layer, evicted in place of the gathered cache
+    k1, v1, keep1 = kvattn.evict_pages(
+        pages[:, 0, 0], pages[:, 0, 1], table,
+        torch.tensor([cached], dtype=torch.int32, device=DEV),
+        weights[:, 0].contiguous(), budget, 8, 2)
+    assert torch.equal(keep1, keep[:, 0]) and torch.equal(k1[0], kv[0, 0, 0])
+    # drafts over the short cache: it is one page of `budget` tokens
+    mask = torch.eye(3, dtype=torch.bool, device=DEV)
+    tplan = kvattn.AttentionPlan([3], [budget], q_heads=H, kv_heads=G,
+                                 head_dim=D, page_size=budget, tree=True,
+                                 device=DEV)
+    q, k, v = (torch.randn(3, h, D, device=DEV).half() for h in (H, G, G))
+    one = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    out, _ = kvattn.tree_attention(tplan, q, k, v, mask,
+                                   (short[0][0], short[0][1]), one)
+    for i in range(3):
+        kk = torch.cat([short[0][0][0], k[i][:, None]], 1).double()
+        vv = torch.cat([short[0][1][0], v[i][:, None]], 1).double()
+        s = (q[i].double().view(G, H // G, D) @ kk.transpose(1, 2)) \
+            / math.sqrt(D)
+        ref = (s.softmax(-1) @ vv).view(H, D)
+        assert (out[i].double() - ref).abs().max() < 2 * 2.0 ** -11 * 5.5
+    with pytest.raises(ValueError):
+        kvwire.store_kv_caches(store, ["x"], [cache], weights=weights)
+    store.close()
