@@ -46,7 +46,6 @@ struct Shape {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kQTiles = kDual ? 1 : 2;
   static constexpr int kSlots = D == 128 ? (kDual ? 6 : 5) : 12;
-  static constexpr int kPending = kSlots - 2 < 6 ? kSlots - 2 : 6;
   static constexpr int kSmem =
       (kQTiles + kSlots) * kTileBytes + (int)sizeof(Control);
   static_assert(kSlots <= kMaxSlots, "ring");
@@ -58,14 +57,6 @@ __device__ __forceinline__ int first_masked_tile(const Segment &s, int group,
                                                  int tree) {
   return (s.cached + (tree ? 0 : s.row0 / group + 1)) / kTile;
 }
-
-// The loader's queue of copies in flight: one cp.async group per tile.
-template <int N>
-struct Pending {
-  uint32_t bar[N];
-  uint32_t check[N];               // V tile to rid of inf and NaN, or 0
-  int n = 0;
-};
 
 // ------------------------------------------------------------------ kernel
 // Mathematics.  Row r of an item is (token i, head g of the group): s_rj =
@@ -101,10 +92,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < Sh::kSlots; ++i) {
-      mbar_init(smem_u32(&ct.full[i]), 4);
+      mbar_init(smem_u32(&ct.full[i]), 128 + 4);
       mbar_init(smem_u32(&ct.empty[i]), 1);
     }
-    mbar_init(smem_u32(&ct.q_full), 4);
+    mbar_init(smem_u32(&ct.q_full), 128 + 4);
     mbar_init(smem_u32(&ct.q_empty), 1);
     mbar_init(smem_u32(&ct.done), 1);
     for (int w = 0; w < 2; ++w) {
@@ -406,7 +397,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kRowsPer = 32 / kChunks;         // rows per warp step
     const int lw = warp - 8;
     const int chunk = lane % kChunks, sub_row = lane / kChunks;
-    Pending<Sh::kPending> pend;
     uint32_t item = 0, q_phase = 1;
 
     // Chunk `chunk` of row `row` of a tile, in the 128-byte swizzle.
@@ -414,74 +404,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       return (uint32_t)((chunk >> 3) * (kTile * 128) + row * 128 +
                         (((chunk & 7) ^ (row & 7)) << 4));
     };
-    auto signal = [&](uint32_t bar, uint32_t check) {
-      if (check) {
-        // A masked tile: a key some rows do not see must not reach them
-        // through 0 * inf, so inf and NaN go in as zeros (and are added
-        // back for the rows that see them in the epilogue).
-        const uint32_t ex = kBf16 ? 0x7f807f80u : 0x7c007c00u;
-        for (int i = 0; i < 32 / kRowsPer; ++i) {
-          const uint32_t at = check + place(lw * 32 + i * kRowsPer + sub_row);
-          uint32_t v[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(at)
+    // A V tile in which some row does not see every key: a key that a row
+    // does not see must not reach it through 0 * inf, so inf and NaN go in
+    // as zeros (and are added back for the rows that see them, in the
+    // epilogue).  Each thread looks at what it copied.
+    auto check_finite = [&](uint32_t dst) {
+      cp_async_wait_all();
+      const uint32_t ex = kBf16 ? 0x7f807f80u : 0x7c007c00u;
+      for (int i = 0; i < 32 / kRowsPer; ++i) {
+        const uint32_t at = dst + place(lw * 32 + i * kRowsPer + sub_row);
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                     : "r"(at)
+                     : "memory");
+        uint32_t bad = 0;
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = v[e] & ex;
+          uint32_t keep = 0;
+          if ((x & 0xffffu) != (ex & 0xffffu)) keep |= 0xffffu;
+          if ((x >> 16) != (ex >> 16)) keep |= 0xffff0000u;
+          bad |= ~keep;
+          v[e] &= keep;
+        }
+        if (bad) {
+          ct.bad_v = 1;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                        : "memory");
-          uint32_t bad = 0;
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = v[e] & ex;
-            uint32_t keep = 0;
-            if ((x & 0xffffu) != (ex & 0xffffu)) keep |= 0xffffu;
-            if ((x >> 16) != (ex >> 16)) keep |= 0xffff0000u;
-            bad |= ~keep;
-            v[e] &= keep;
-          }
-          if (bad) {
-            ct.bad_v = 1;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
-                         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
-                         : "memory");
-          }
         }
       }
       fence_async_proxy();
+    };
+    // A tile is full when every thread's copies have landed (128 arrivals
+    // by the copies themselves) and every warp's plain writes are released
+    // (4): no thread waits for its own copies, so as many tiles are in
+    // flight as there are free slots.
+    auto publish = [&](uint32_t bar) {
+      cp_async_arrive(bar);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
-    };
-    auto flush = [&]() {
-      cp_async_wait<0>();
-#pragma unroll
-      for (int i = 0; i < Sh::kPending; ++i)
-        if (i < pend.n) signal(pend.bar[i], pend.check[i]);
-      pend.n = 0;
-    };
-    // Waits for a free place; what is in flight is handed over first when
-    // that takes long, since the consumers may be waiting for it.
-    auto wait_free = [&](uint32_t bar, uint32_t parity) {
-      if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
-      flush();
-      mbar_wait(bar, parity, give_up);
-      __syncwarp();
-    };
-    auto push = [&](uint32_t bar, uint32_t check) {
-      cp_async_commit();
-      if (pend.n == Sh::kPending) {
-        cp_async_wait<Sh::kPending>();
-        signal(pend.bar[0], pend.check[0]);
-#pragma unroll
-        for (int i = 0; i + 1 < Sh::kPending; ++i) {
-          pend.bar[i] = pend.bar[i + 1];
-          pend.check[i] = pend.check[i + 1];
-        }
-        pend.n = Sh::kPending - 1;
-      }
-#pragma unroll
-      for (int i = 0; i < Sh::kPending; ++i)
-        if (i == pend.n) {
-          pend.bar[i] = bar;
-          pend.check[i] = check;
-        }
-      ++pend.n;
     };
     // One tile: lane `i` of the warp holds the address of its row i (0: the
     // row is not there and reads as zeros).
@@ -502,7 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t_all = kDual ? sg.t1 : max(sg.n0, sg.n1);
       const int masked_from = first_masked_tile(sg, a.group, a.tree);
       // Q
-      wait_free(smem_u32(&ct.q_empty), q_phase);
+      mbar_wait(smem_u32(&ct.q_empty), q_phase, give_up);
+      __syncwarp();
       q_phase ^= 1;
       for (int qt = 0; qt < Sh::kQTiles; ++qt) {
         const int r = qt * kTile + lw * 32 + lane;
@@ -516,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         copy_rows(sm_q + qt * Sh::kTileBytes, src);
       }
-      push(smem_u32(&ct.q_full), 0);
+      publish(smem_u32(&ct.q_full));
       // K and V tiles
       const int total = sg.cached + sg.n_new;
       auto page_at = [&](int t) {        // the page of this lane's key
@@ -545,25 +508,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         {
           const uint32_t slot = item % Sh::kSlots;
           const uint32_t ph = (item / Sh::kSlots) & 1;
-          wait_free(smem_u32(&ct.empty[slot]), ph ^ 1);
+          mbar_wait(smem_u32(&ct.empty[slot]), ph ^ 1, give_up);
+          __syncwarp();
           if (lane == 0) ct.valid[tile_no & 7][lw] = there;
           copy_rows(sm_ring + slot * Sh::kTileBytes, kp);
-          push(smem_u32(&ct.full[slot]), 0);
+          publish(smem_u32(&ct.full[slot]));
           ++item;
         }
         {
           const uint32_t slot = item % Sh::kSlots;
           const uint32_t ph = (item / Sh::kSlots) & 1;
           const uint32_t dst = sm_ring + slot * Sh::kTileBytes;
-          wait_free(smem_u32(&ct.empty[slot]), ph ^ 1);
+          mbar_wait(smem_u32(&ct.empty[slot]), ph ^ 1, give_up);
+          __syncwarp();
           copy_rows(dst, vp);
-          push(smem_u32(&ct.full[slot]), t >= masked_from ? dst : 0);
+          if (t >= masked_from) check_finite(dst);
+          publish(smem_u32(&ct.full[slot]));
           ++item;
         }
         ++tile_no;
       }
     }
-    flush();
+    cp_async_wait_all();
   } else {
     // ------------------------------------------------------------ MMA
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -575,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait_item = [&](uint32_t item) {
         const uint32_t slot = item % Sh::kSlots;
         mbar_wait(smem_u32(&ct.full[slot]), (item / Sh::kSlots) & 1, give_up);
+        fence_async_proxy();
         return slot;
       };
       for (int si = seg_begin; si < seg_end; ++si) {
@@ -603,6 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (--left == 0) tc_commit(smem_u32(&ct.q_empty));
         };
         mbar_wait(smem_u32(&ct.q_full), q_phase, give_up);
+        fence_async_proxy();
         q_phase ^= 1;
         if (kDual) {
           qk(t0, 0);

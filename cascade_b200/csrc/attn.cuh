@@ -113,14 +113,19 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src,
                "l"(src), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives on `bar` (one of its expected arrivals) once every cp.async that
+// this thread has issued so far has landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                   bar)
+               : "memory");
 }
-// Generic-proxy writes to shared memory become visible to tcgen05.mma.
+// Between generic-proxy writes to shared memory (cp.async among them) that
+// this thread made or has seen complete on an mbarrier, and tcgen05.mma
+// reading them.
 __device__ __forceinline__ void fence_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }

@@ -70,11 +70,11 @@ __global__ void __launch_bounds__(kWThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kKSlots; ++i) {
-      mbar_init(smem_u32(&ct.k_full[i]), 4);
+      mbar_init(smem_u32(&ct.k_full[i]), 128);
       mbar_init(smem_u32(&ct.k_empty[i]), 1);
     }
     for (int i = 0; i < kQSlots; ++i) {
-      mbar_init(smem_u32(&ct.q_full[i]), 4);
+      mbar_init(smem_u32(&ct.q_full[i]), 128 + 4);
       mbar_init(smem_u32(&ct.q_empty[i]), 9);   // the MMAs and 8 warps
     }
     for (int w = 0; w < 2; ++w)
@@ -169,47 +169,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
     // ------------------------------------------------------- loaders
     constexpr int kChunks = D / 8;
     constexpr int kRowsPer = 32 / kChunks;
-    constexpr int kPending = 3;
     const int lw = warp - 8;
     const int chunk = lane % kChunks, sub_row = lane / kChunks;
-    uint32_t pend[kPending];
-    int n_pend = 0;
     uint32_t k_no = 0, q_no = 0;
     auto place = [&](int row) {
       return (uint32_t)((chunk >> 3) * (kTile * 128) + row * 128 +
                         (((chunk & 7) ^ (row & 7)) << 4));
-    };
-    auto signal = [&](uint32_t bar) {
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    auto flush = [&]() {
-      cp_async_wait<0>();
-#pragma unroll
-      for (int i = 0; i < kPending; ++i)
-        if (i < n_pend) signal(pend[i]);
-      n_pend = 0;
-    };
-    auto wait_free = [&](uint32_t bar, uint32_t parity) {
-      if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
-      flush();
-      mbar_wait(bar, parity, give_up);
-      __syncwarp();
-    };
-    auto push = [&](uint32_t bar) {
-      cp_async_commit();
-      if (n_pend == kPending) {
-        cp_async_wait<kPending>();
-        signal(pend[0]);
-#pragma unroll
-        for (int i = 0; i + 1 < kPending; ++i) pend[i] = pend[i + 1];
-        n_pend = kPending - 1;
-      }
-#pragma unroll
-      for (int i = 0; i < kPending; ++i)
-        if (i == n_pend) pend[i] = bar;
-      ++n_pend;
     };
     auto copy_rows = [&](uint32_t dst, const char *row_ptr) {
 #pragma unroll
@@ -241,10 +206,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
       }
       {
         const uint32_t slot = k_no % kKSlots;
-        wait_free(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1);
+        mbar_wait(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1,
+                  give_up);
+        __syncwarp();
         copy_rows(sm_k + 2 * slot * kTileBytes, kp[0]);
         copy_rows(sm_k + (2 * slot + 1) * kTileBytes, kp[1]);
-        push(smem_u32(&ct.k_full[slot]));
+        cp_async_arrive(smem_u32(&ct.k_full[slot]));
         ++k_no;
       }
       for (int ch = sg.t0; ch < sg.t1; ++ch, ++q_no) {
@@ -262,14 +229,19 @@ __global__ void __launch_bounds__(kWThreads, 1)
           const float l = a.lse[at * a.l_tok + head * a.l_head];
           l2 = l == -INFINITY ? INFINITY : l * kLog2e;
         }
-        wait_free(smem_u32(&ct.q_empty[slot]), ((q_no / kQSlots) & 1) ^ 1);
+        mbar_wait(smem_u32(&ct.q_empty[slot]), ((q_no / kQSlots) & 1) ^ 1,
+                  give_up);
+        __syncwarp();
         ct.lse2[slot][r] = l2;
         // the MMA reads the rows up to the next multiple of 32
         if (lw * 32 < n) copy_rows(sm_q + slot * kTileBytes, src);
-        push(smem_u32(&ct.q_full[slot]));
+        // the copies arrive by themselves, the warp for what it wrote
+        cp_async_arrive(smem_u32(&ct.q_full[slot]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ct.q_full[slot]));
       }
     }
-    flush();
+    cp_async_wait_all();
   } else {
     // ------------------------------------------------------------ MMA
     if (lane == 0) {
@@ -279,6 +251,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         if (t0 >= t1) continue;
         const uint32_t ks = k_no % kKSlots;
         mbar_wait(smem_u32(&ct.k_full[ks]), (k_no / kKSlots) & 1, give_up);
+        fence_async_proxy();
         ++k_no;
         for (int ch = t0; ch < t1; ++ch, ++chunk_no) {
           const uint32_t buf = chunk_no & 1, slot = chunk_no % kQSlots;
@@ -286,6 +259,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
           const uint32_t idesc = mma_idesc(kBf16, n, false);
           mbar_wait(smem_u32(&ct.q_full[slot]), (chunk_no / kQSlots) & 1,
                     give_up);
+          fence_async_proxy();
           const uint32_t q = sm_q + slot * kTileBytes;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
