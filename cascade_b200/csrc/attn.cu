@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 8) {
     // ------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int w = warp >> 2;                       // warpgroup
     const int rt = (warp & 3) * 32 + lane;         // row of the tile
     const int r = (kDual ? 0 : w * kTile) + rt;    // row of the item
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     cp_async_wait_all();
   } else {
     // ------------------------------------------------------------ MMA
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12 && lane == 0) {
       constexpr uint32_t id_qk = mma_idesc(kBf16, kTile, false);
       constexpr uint32_t id_pv = mma_idesc(kBf16, D, true);
@@ -556,13 +556,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t it = base + 2 * (t - t0);
           const uint32_t slot = wait_item(it);
           tc_fence_after();
-          const uint32_t q = sm_q + (kDual ? 0 : w * Sh::kTileBytes);
-          const uint32_t k = sm_ring + slot * Sh::kTileBytes;
+          const uint64_t q =
+              tile_desc(pinned(sm_q + (kDual ? 0 : w * Sh::kTileBytes)), 0);
+          const uint64_t k =
+              tile_desc(pinned(sm_ring + slot * Sh::kTileBytes), 0);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
-            mma_ss(tmem + w * 128, tile_desc(q + off, 0),
-                   tile_desc(k + off, 0), id_qk, kk != 0);
+            mma_ss(tmem + w * 128, q + (off >> 4), k + (off >> 4), id_qk,
+                   kk != 0);
           }
           const bool last = kDual || w == (t < n1 ? 1 : 0);
           if (last) tc_commit(smem_u32(&ct.empty[slot]));
@@ -594,13 +596,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             else
               p_phase[0] ^= 1;
             tc_fence_after();
-            const uint32_t v = sm_ring + slot * Sh::kTileBytes;
+            const uint64_t v =
+                tile_desc(pinned(sm_ring + slot * Sh::kTileBytes),
+                          kTile * 128);
             const bool fresh = kDual ? t < t0 + 2 : t == t0;
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk)
               mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
-                     tile_desc(v + kk * 2048, kTile * 128), id_pv,
-                     !(fresh && kk == 0));
+                     v + kk * (2048 >> 4), id_pv, !(fresh && kk == 0));
             const bool last_use = kDual || w == (t < n1 ? 1 : 0);
             if (last_use) tc_commit(smem_u32(&ct.empty[slot]));
             const int t_next = t + (kDual ? 2 : 1);
@@ -680,7 +683,7 @@ int run_fwd(const FwdArgs &a, const cascade_attn_plan_info_t &p,
   using Sh = Shape<D, kDual>;
   auto *kernel = attn_fwd_kernel<D, kBf16, kDual>;
   // setmaxnreg hands the launch's registers from the loaders and the MMA
-  // warps to the softmax warps: 256 x 200 + 128 x 72 + 128 x 40 = 512 x 128.
+  // warps to the softmax warps: 256 x 192 + 128 x 72 + 128 x 56 = 512 x 128.
   // A launch with fewer would wait for ever, so it is refused.
   cudaFuncAttributes fa;
   CB_CUDA(cudaFuncGetAttributes(&fa, kernel));

@@ -179,6 +179,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b,
       : "memory");
 }
 
+// The same value, recomputed where it is used: descriptors made from it are
+// not kept in registers across loops.
+__device__ __forceinline__ uint32_t pinned(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+
 // Shared-memory matrix descriptor of a tile in the 128-byte swizzle: rows of
 // 64 16-bit values (128 bytes), 8-row groups 1024 bytes apart, further
 // 64-value column blocks `lbo` bytes apart (used when the rows run along K).
