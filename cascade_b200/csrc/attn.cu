@@ -33,6 +33,7 @@ struct Control {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t turn[2];
   uint64_t done;
   alignas(16) uint32_t valid[8][4];  // which keys of a tile there are
   float2 ml[2][kTile];             // two-tile form: each half's (max, sum)
@@ -93,15 +94,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < Sh::kSlots; ++i) {
       mbar_init(smem_u32(&ct.full[i]), 128 + 4);
-      mbar_init(smem_u32(&ct.empty[i]), 1);
+      mbar_init(smem_u32(&ct.empty[i]), kDual ? 1 : 2);
     }
     mbar_init(smem_u32(&ct.q_full), 128 + 4);
-    mbar_init(smem_u32(&ct.q_empty), 1);
-    mbar_init(smem_u32(&ct.done), 1);
+    mbar_init(smem_u32(&ct.q_empty), 2);
+    mbar_init(smem_u32(&ct.done), 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&ct.s_full[w]), 1);
       mbar_init(smem_u32(&ct.p_full[w]), 4);
       mbar_init(smem_u32(&ct.o_full[w]), 1);
+      mbar_init(smem_u32(&ct.turn[w]), 1);
     }
     ct.give_up = 0;
     ct.bad_v = 0;
@@ -157,13 +159,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) tc_ld32(x[i], tm_s + i * 32);
           const uint4 vw = *reinterpret_cast<const uint4 *>(
               ct.valid[(tiles_done + t - sg.t0) & 7]);
+          const bool partial =
+              (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu || t >= masked_from;
           tc_wait_ld();
 #pragma unroll
           for (int i = 0; i < 4; ++i) tc_hold(x[i]);
-          const bool partial =
-              (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu || t >= masked_from;
           if (partial) {
-            const uint32_t words[4] = {vw.x, vw.y, vw.z, vw.w};
+            const uint32_t there[4] = {vw.x, vw.y, vw.z, vw.w};
             uint32_t any = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = max(j0, sg.cached); j < e; ++j)
                   if (mrow[j - sg.cached]) vis |= 1u << (j - j0);
               }
-              vis &= words[i];
+              vis &= there[i];
               any |= vis;
 #pragma unroll
               for (int e = 0; e < 32; ++e)
@@ -188,23 +190,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           float mx[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v0 = __uint_as_float(x[i][0]);
-            float v1 = __uint_as_float(x[i][1]);
+            mx[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
 #pragma unroll
-            for (int e = 2; e < 32; e += 2) {
-              v0 = fmaxf(v0, __uint_as_float(x[i][e]));
-              v1 = fmaxf(v1, __uint_as_float(x[i][e + 1]));
-            }
-            mx[i] = fmaxf(v0, v1);
+            for (int e = 2; e < 32; ++e)
+              mx[i] = fmaxf(mx[i], __uint_as_float(x[i][e]));
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           // m == -inf: any finite top is growth
           if (__any_sync(0xffffffffu, top > m + grow)) {
             const float m_new = fmaxf(m, top);
             if (!first) {
-              const float f =
-                  m == -INFINITY ? (l == 0.f ? 1.f : 0.f)
-                                 : ex2((m - m_new) * a.c);
+              const float f = m == -INFINITY ? (l == 0.f ? 1.f : 0.f)
+                                             : ex2((m - m_new) * a.c);
               l *= f;
 #pragma unroll 1
               for (int i = 0; i < D / 16; ++i) {
@@ -448,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One tile: lane `i` of the warp holds the address of its row i (0: the
     // row is not there and reads as zeros).
     auto copy_rows = [&](uint32_t dst, const char *row_ptr) {
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < 32 / kRowsPer; ++i) {
         const int rl = i * kRowsPer + sub_row;
         const uint64_t p =
@@ -532,93 +529,113 @@ __global__ void __launch_bounds__(kThreads, 1)
     cp_async_wait_all();
   } else {
     // ------------------------------------------------------------ MMA
+    // One warp for each of the two chains S -> P -> O.  A tcgen05.mma holds
+    // its warp until the tensor pipe takes it, so whatever a warp does
+    // between two of them is time in which only the other warp's MMAs run.
+    // With two row tiles the warps take turns, a step's PV and next QK at a
+    // time: were their MMAs to interleave, both chains would fall into step,
+    // exponentials under exponentials and MMAs under MMAs (16384 tokens:
+    // 5.44 ms against 3.98).
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12 && lane == 0) {
+    if (warp < 14) {
+      const int w = uniform(warp - 12);
+      const uint32_t issue = lane == 0;
+      const uint32_t tm_s = uniform(tmem) + w * 128, tm_o = tm_s + 256;
+      const uint32_t q = tile_desc(
+          uniform(sm_q) + (kDual ? 0 : w * Sh::kTileBytes), 0);
+      const uint32_t ring = uniform(sm_ring);
       constexpr uint32_t id_qk = mma_idesc(kBf16, kTile, false);
       constexpr uint32_t id_pv = mma_idesc(kBf16, D, true);
-      uint32_t base = 0, q_phase = 0;
-      uint32_t p_phase[2] = {0, 0};
-      auto wait_item = [&](uint32_t item) {
-        const uint32_t slot = item % Sh::kSlots;
-        mbar_wait(smem_u32(&ct.full[slot]), (item / Sh::kSlots) & 1, give_up);
-        fence_async_proxy();
-        return slot;
-      };
-      for (int si = seg_begin; si < seg_end; ++si) {
+      constexpr int kStep = kDual ? 2 : 1;
+      uint32_t base = 0, q_phase = 0, p_phase = 0;
+      uint32_t turn_phase = w ^ 1;          // warp 0 has the first turn
+      const int seg_last = uniform(seg_end);
+      for (int si = uniform(seg_begin); si < seg_last; ++si) {
         const Segment *sp = segs + si;
-        const int t0 = sp->t0;
-        const int n0 = kDual ? sp->t1 : sp->n0, n1 = kDual ? sp->t1 : sp->n1;
-        const int t_all = max(n0, n1);
-        // steps in order: (tile t, buffer w); w = row tile, or, in the
-        // two-tile form, the parity of the key tile
-        int left = kDual ? t_all - t0 : max(n0 - t0, 0) + max(n1 - t0, 0);
-        auto qk = [&](int t, int w) {
-          const uint32_t it = base + 2 * (t - t0);
-          const uint32_t slot = wait_item(it);
-          tc_fence_after();
-          const uint64_t q =
-              tile_desc(pinned(sm_q + (kDual ? 0 : w * Sh::kTileBytes)), 0);
-          const uint64_t k =
-              tile_desc(pinned(sm_ring + slot * Sh::kTileBytes), 0);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
-            mma_ss(tmem + w * 128, q + (off >> 4), k + (off >> 4), id_qk,
-                   kk != 0);
-          }
-          const bool last = kDual || w == (t < n1 ? 1 : 0);
-          if (last) tc_commit(smem_u32(&ct.empty[slot]));
-          tc_commit(smem_u32(&ct.s_full[w]));
-          if (--left == 0) tc_commit(smem_u32(&ct.q_empty));
+        const int t0 = uniform(sp->t0);
+        const int n0 = uniform(kDual ? sp->t1 : sp->n0);
+        const int n1 = uniform(kDual ? sp->t1 : sp->n1);
+        const int t_all = max(n0, n1), n_end = w ? n1 : n0;
+        const int t_first = kDual ? t0 + w : t0;
+        auto full = [&](uint32_t item) {
+          return smem_u32(&ct.full[item % Sh::kSlots]);
         };
-        mbar_wait(smem_u32(&ct.q_full), q_phase, give_up);
-        fence_async_proxy();
+        auto phase = [&](uint32_t item) { return (item / Sh::kSlots) & 1; };
+        auto pass_turn = [&]() {
+          if (!kDual && issue) mbar_arrive(smem_u32(&ct.turn[w ^ 1]));
+        };
+        mbar_wait_warp(smem_u32(&ct.q_full), q_phase, give_up);
         q_phase ^= 1;
-        if (kDual) {
-          qk(t0, 0);
-          if (t0 + 1 < t_all) qk(t0 + 1, 1);
-        } else {
-          if (t0 < n0) qk(t0, 0);
-          if (t0 < n1) qk(t0, 1);
+        if (t_first < n_end) {
+          const uint32_t item = base + 2 * (t_first - t0);
+          const uint32_t slot = item % Sh::kSlots;
+          mbar_wait_warp(full(item), phase(item), give_up);
+          fence_async_proxy();
+          mma_rows<0, D / 16>(tm_s, q,
+                              tile_desc(ring + slot * Sh::kTileBytes, 0),
+                              id_qk, issue);
+          tc_commit(smem_u32(&ct.s_full[w]), issue);
+          tc_commit(smem_u32(&ct.empty[slot]), issue);
         }
-        for (int t = t0; t < t_all; ++t) {
-          const uint32_t it_v = base + 2 * (t - t0) + 1;
-#pragma unroll
-          for (int h = 0; h < (kDual ? 1 : 2); ++h) {
-            const int w = kDual ? (t - t0) & 1 : h;
-            const int n_end = w ? n1 : n0;
-            if (!kDual && t >= n_end) continue;
-            const uint32_t slot = wait_item(it_v);
-            mbar_wait(smem_u32(&ct.p_full[w]), w ? p_phase[1] : p_phase[0],
-                      give_up);
-            if (w)
-              p_phase[1] ^= 1;
-            else
-              p_phase[0] ^= 1;
-            tc_fence_after();
-            const uint64_t v =
-                tile_desc(pinned(sm_ring + slot * Sh::kTileBytes),
-                          kTile * 128);
-            const bool fresh = kDual ? t < t0 + 2 : t == t0;
-#pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
-              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
-                     v + kk * (2048 >> 4), id_pv, !(fresh && kk == 0));
-            const bool last_use = kDual || w == (t < n1 ? 1 : 0);
-            if (last_use) tc_commit(smem_u32(&ct.empty[slot]));
-            const int t_next = t + (kDual ? 2 : 1);
-            if (t_next < n_end)
-              qk(t_next, w);
-            else
-              tc_commit(smem_u32(&ct.o_full[w]));
+        for (int t = t_first; t < t_all; t += kStep) {
+          if (!kDual && t >= n_end) {
+            // A tile that only the other row tile needs: give it back, pass
+            // the turn on.
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t item = base + 2 * (t - t0) + h;
+              mbar_wait_warp(full(item), phase(item), give_up);
+              if (issue)
+                mbar_arrive(smem_u32(&ct.empty[item % Sh::kSlots]));
+            }
+            mbar_wait_warp(smem_u32(&ct.turn[w]), turn_phase, give_up);
+            turn_phase ^= 1;
+            pass_turn();
+            continue;
           }
+          const uint32_t v_item = base + 2 * (t - t0) + 1;
+          const uint32_t k_item = v_item + 2 * kStep - 1;
+          const uint32_t slot = v_item % Sh::kSlots;
+          const uint32_t k_slot = k_item % Sh::kSlots;
+          const bool more = t + kStep < n_end;
+          mbar_wait_warp(full(v_item), phase(v_item), give_up);
+          const uint32_t v =
+              tile_desc(ring + slot * Sh::kTileBytes, kTile * 128);
+          const uint32_t k = tile_desc(ring + k_slot * Sh::kTileBytes, 0);
+          const bool k_there =
+              more && __all_sync(0xffffffffu,
+                                 mbar_try(full(k_item), phase(k_item)));
+          fence_async_proxy();
+          mbar_wait_warp(smem_u32(&ct.p_full[w]), p_phase, give_up);
+          p_phase ^= 1;
+          if (!kDual) {
+            mbar_wait_warp(smem_u32(&ct.turn[w]), turn_phase, give_up);
+            turn_phase ^= 1;
+          }
+          tc_fence_after();
+          mma_keys<0, kTile / 16>(tm_o, tm_s, v, id_pv, t != t_first, issue);
+          if (!k_there) {
+            pass_turn();
+            if (!more) tc_commit(smem_u32(&ct.o_full[w]), issue);
+            tc_commit(smem_u32(&ct.empty[slot]), issue);
+            if (!more) continue;
+            mbar_wait_warp(full(k_item), phase(k_item), give_up);
+            fence_async_proxy();
+          }
+          mma_rows<0, D / 16>(tm_s, q, k, id_qk, issue);
+          if (k_there) {
+            pass_turn();
+            tc_commit(smem_u32(&ct.empty[slot]), issue);
+          }
+          tc_commit(smem_u32(&ct.s_full[w]), issue);
+          tc_commit(smem_u32(&ct.empty[k_slot]), issue);
         }
+        tc_commit(smem_u32(&ct.q_empty), issue);
         base += 2 * (t_all - t0);
       }
       // TMEM is freed only when no MMA is in flight.
-      tc_commit(smem_u32(&ct.done));
+      tc_commit(smem_u32(&ct.done), issue);
       int gave_up = 0;
-      mbar_wait(smem_u32(&ct.done), 0, &gave_up);
+      mbar_wait_warp(smem_u32(&ct.done), 0, &gave_up);
     }
     __syncwarp();
   }

@@ -106,6 +106,14 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity,
   mbar_wait_slow(bar, parity, give_up);
 }
 
+// The same for a whole warp, which stays converged.
+__device__ __forceinline__ void mbar_wait_warp(uint32_t bar, uint32_t parity,
+                                               volatile int *give_up) {
+  if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
+  mbar_wait_slow(bar, parity, give_up);
+  __syncwarp();
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src,
                                            uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(
@@ -151,47 +159,81 @@ __device__ __forceinline__ void tc_dealloc(uint32_t tmem, uint32_t cols) {
                "r"(cols)
                : "memory");
 }
-// Arrives on `bar` once every tcgen05.mma this thread issued has finished.
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 "
-      "[%0];" ::"r"(bar)
-      : "memory");
+// The MMA warp runs converged, with every value of its loops the same in all
+// lanes, and one lane issues: descriptors and addresses then stay in uniform
+// registers.  (Issued from a branch that one lane takes, each tcgen05.mma
+// first moves its operands there, which took longer than the MMA itself.)
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return __reduce_max_sync(0xffffffffu, x);
 }
 
-// D[128 x N] (+)= A[128 x 16] B[16 x N], A and B in shared memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b,
-                                       uint32_t idesc, bool accumulate) {
+// Arrives on `bar` once every tcgen05.mma the issuing lane issued is done.
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t issue) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster"
+      ".b64 [%0];\n\t}" ::"r"(bar),
+      "r"(issue)
       : "memory");
-}
-// The same with A in TMEM (two 16-bit values a column, one row a lane).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b,
-                                       uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(
-          d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-
-// The same value, recomputed where it is used: descriptors made from it are
-// not kept in registers across loops.
-__device__ __forceinline__ uint32_t pinned(uint32_t x) {
-  asm volatile("" : "+r"(x));
-  return x;
 }
 
 // Shared-memory matrix descriptor of a tile in the 128-byte swizzle: rows of
 // 64 16-bit values (128 bytes), 8-row groups 1024 bytes apart, further
 // 64-value column blocks `lbo` bytes apart (used when the rows run along K).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lbo >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// The lower word is made here; the upper one (the group stride, the
+// descriptor version and the swizzle) is the same for all tiles.
+__device__ __forceinline__ uint32_t tile_desc(uint32_t addr, uint32_t lbo) {
+  return ((addr & 0x3FFFF) >> 4) | ((lbo >> 4) << 16);
+}
+#define CB_DESC_HIGH "0x40004040"
+
+// D[128 x N] (+)= A[128 x 16] B[16 x N], A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b,
+                                       uint32_t idesc, uint32_t accumulate,
+                                       uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 da, {%1, " CB_DESC_HIGH "};\n\t"
+      "mov.b64 db, {%2, " CB_DESC_HIGH "};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(
+          d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+// The same with A in TMEM (two 16-bit values a column, one row a lane).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b,
+                                       uint32_t idesc, uint32_t accumulate,
+                                       uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 db, {%2, " CB_DESC_HIGH "};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, "
+      "p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+
+// S[128 x N] = A B^T over D columns: 16-column steps [kStep, kEnd) in turn.
+template <int kStep, int kEnd>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b,
+                                         uint32_t idesc, uint32_t issue) {
+#pragma unroll
+  for (int k = kStep; k < kEnd; ++k) {
+    const uint32_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+    mma_ss(d, a + off, b + off, idesc, k, issue);
+  }
+}
+// O[128 x N] (+)= P[128 x 128] V over the key steps [kStep, kEnd).
+template <int kStep, int kEnd>
+__device__ __forceinline__ void mma_keys(uint32_t d, uint32_t p, uint32_t v,
+                                         uint32_t idesc, bool accumulate,
+                                         uint32_t issue) {
+#pragma unroll
+  for (int k = kStep; k < kEnd; ++k)
+    mma_ts(d, p + k * 8, v + k * (2048 >> 4), idesc,
+           accumulate || k != kStep, issue);
 }
 
 // kind::f16 instruction descriptor: 128 x n, FP32 accumulator; `mn_b` when
@@ -223,13 +265,15 @@ __device__ __forceinline__ void tc_ld32(uint32_t (&x)[32], uint32_t addr) {
       : CB_R8(x, 0), CB_R8(x, 8), CB_R8(x, 16), CB_R8(x, 24)
       : "r"(addr));
 }
-__device__ __forceinline__ void tc_ld16(uint32_t (&x)[16], uint32_t addr) {
+__device__ __forceinline__ void tc_st32(uint32_t addr,
+                                        const uint32_t (&x)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15}, [%16];"
-      : CB_R8(x, 0), CB_R8(x, 8)
-      : "r"(addr));
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31};" ::CB_I8(x, 0),
+      CB_I8(x, 8), CB_I8(x, 16), CB_I8(x, 24), "r"(addr)
+      : "memory");
 }
 __device__ __forceinline__ void tc_st16(uint32_t addr,
                                         const uint32_t (&x)[16]) {
@@ -239,6 +283,14 @@ __device__ __forceinline__ void tc_st16(uint32_t addr,
       "%15};" ::CB_I8(x, 0),
       CB_I8(x, 8), "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t (&x)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : CB_R8(x, 0), CB_R8(x, 8)
+      : "r"(addr));
 }
 __device__ __forceinline__ void tc_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -250,6 +302,7 @@ __device__ __forceinline__ void tc_wait_st() {
 __device__ __forceinline__ void tc_hold(uint32_t (&x)[32]) {
   asm volatile("" : CB_K8(x, 0), CB_K8(x, 8), CB_K8(x, 16), CB_K8(x, 24));
 }
+
 __device__ __forceinline__ void tc_hold(uint32_t (&x)[16]) {
   asm volatile("" : CB_K8(x, 0), CB_K8(x, 8));
 }
@@ -258,6 +311,64 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Pairs of floats in one register pair: one instruction works on both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of a pair on the FMA pipe, for x <= 127 (x below -126, -inf among
+// them, gives 2^-126; NaN stays NaN).  The special-function unit does 16
+// exponentials a cycle and SM, which is what bounds a softmax beside
+// tcgen05; a share of them is done here instead.  x = i + f with i the
+// nearest integer (added to 1.5 2^23, its bits are the low ones) and f in
+// [-1/2, 1/2]; 2^f is the polynomial of degree 5 of least relative error
+// there (Remez exchange; 2.1e-7 with its coefficients and steps rounded to
+// FP32, no more than ex2.approx is off).
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+  float lo, hi;
+  unpair(x, lo, hi);
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(lo));        // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(hi));
+  x = pair(lo, hi);
+  const uint64_t t = add2(x, pair(12582912.f, 12582912.f));
+  const uint64_t i = add2(t, pair(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(i, pair(-1.f, -1.f), x);
+  constexpr float c0 = 0x1.000002p+0f, c1 = 0x1.62e428p-1f,
+                  c2 = 0x1.ebf918p-3f, c3 = 0x1.c6b6e4p-5f,
+                  c4 = 0x1.3d0c52p-7f, c5 = 0x1.5c08e6p-10f;
+  uint64_t p = fma2(pair(c5, c5), f, pair(c4, c4));
+  p = fma2(p, f, pair(c3, c3));
+  p = fma2(p, f, pair(c2, c2));
+  p = fma2(p, f, pair(c1, c1));
+  p = fma2(p, f, pair(c0, c0));
+  unpair(t, lo, hi);
+  const float e0 =
+      __uint_as_float((__float_as_uint(lo) << 23) + 0x3f800000u);
+  const float e1 =
+      __uint_as_float((__float_as_uint(hi) << 23) + 0x3f800000u);
+  return mul2(p, pair(e0, e1));
 }
 
 // Two floats to two 16-bit values in one word, to nearest even.

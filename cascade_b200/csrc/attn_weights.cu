@@ -244,44 +244,44 @@ __global__ void __launch_bounds__(kWThreads, 1)
     cp_async_wait_all();
   } else {
     // ------------------------------------------------------------ MMA
-    if (lane == 0) {
+    {
+      const uint32_t issue = lane == 0;
+      const uint32_t tm = uniform(tmem), sk = uniform(sm_k);
+      const uint32_t sq = uniform(sm_q);
       uint32_t k_no = 0, chunk_no = 0;
-      for (int si = seg_begin; si < seg_end; ++si) {
-        const int t0 = segs[si].t0, t1 = segs[si].t1, rows = segs[si].rows;
+      for (int si = uniform(seg_begin); si < (int)uniform(seg_end); ++si) {
+        const int t0 = uniform(segs[si].t0), t1 = uniform(segs[si].t1);
+        const int rows = uniform(segs[si].rows);
         if (t0 >= t1) continue;
         const uint32_t ks = k_no % kKSlots;
-        mbar_wait(smem_u32(&ct.k_full[ks]), (k_no / kKSlots) & 1, give_up);
+        mbar_wait_warp(smem_u32(&ct.k_full[ks]), (k_no / kKSlots) & 1, give_up);
         fence_async_proxy();
         ++k_no;
         for (int ch = t0; ch < t1; ++ch, ++chunk_no) {
           const uint32_t buf = chunk_no & 1, slot = chunk_no % kQSlots;
           const int n = min(kTile, (rows - ch * kTile + 31) / 32 * 32);
           const uint32_t idesc = mma_idesc(kBf16, n, false);
-          mbar_wait(smem_u32(&ct.q_full[slot]), (chunk_no / kQSlots) & 1,
+          mbar_wait_warp(smem_u32(&ct.q_full[slot]), (chunk_no / kQSlots) & 1,
                     give_up);
           fence_async_proxy();
-          const uint32_t q = sm_q + slot * kTileBytes;
+          const uint32_t q = tile_desc(sq + slot * kTileBytes, 0);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            mbar_wait(smem_u32(&ct.s_empty[w][buf]),
+            mbar_wait_warp(smem_u32(&ct.s_empty[w][buf]),
                       ((chunk_no >> 1) & 1) ^ 1, give_up);
             tc_fence_after();
-            const uint32_t k = sm_k + (2 * ks + w) * kTileBytes;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
-              mma_ss(tmem + w * 256 + buf * 128, tile_desc(k + off, 0),
-                     tile_desc(q + off, 0), idesc, kk != 0);
-            }
-            tc_commit(smem_u32(&ct.s_full[w][buf]));
+            mma_rows<0, D / 16>(tm + w * 256 + buf * 128,
+                        tile_desc(sk + (2 * ks + w) * kTileBytes, 0), q,
+                        idesc, issue);
+            tc_commit(smem_u32(&ct.s_full[w][buf]), issue);
           }
-          tc_commit(smem_u32(&ct.q_empty[slot]));
+          tc_commit(smem_u32(&ct.q_empty[slot]), issue);
         }
-        tc_commit(smem_u32(&ct.k_empty[ks]));
+        tc_commit(smem_u32(&ct.k_empty[ks]), issue);
       }
-      tc_commit(smem_u32(&ct.done));
+      tc_commit(smem_u32(&ct.done), issue);
       int gave_up = 0;
-      mbar_wait(smem_u32(&ct.done), 0, &gave_up);
+      mbar_wait_warp(smem_u32(&ct.done), 0, &gave_up);
     }
     __syncwarp();
   }
