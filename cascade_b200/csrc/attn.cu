@@ -455,12 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
 
-    uint32_t tile_no = 0;
-    for (int si = seg_begin; si < seg_end; ++si) {
-      const Segment sg = segs[si];
-      const int t_all = kDual ? sg.t1 : max(sg.n0, sg.n1);
-      const int masked_from = first_masked_tile(sg, a.group, a.tree);
-      // Q
+    auto load_q = [&](const Segment &sg) {
       mbar_wait(smem_u32(&ct.q_empty), q_phase, give_up);
       __syncwarp();
       q_phase ^= 1;
@@ -477,6 +472,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         copy_rows(sm_q + qt * Sh::kTileBytes, src);
       }
       publish(smem_u32(&ct.q_full));
+    };
+
+    uint32_t tile_no = 0;
+    for (int si = seg_begin; si < seg_end; ++si) {
+      const Segment sg = segs[si];
+      const int t_all = kDual ? sg.t1 : max(sg.n0, sg.n1);
+      const int masked_from = first_masked_tile(sg, a.group, a.tree);
       // K and V tiles
       const int total = sg.cached + sg.n_new;
       auto page_at = [&](int t) {        // the page of this lane's key
@@ -485,6 +487,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int page = page_at(sg.t0);
       for (int t = sg.t0; t < t_all; ++t) {
+        // Q goes behind the segment's first two tiles: it has to wait until
+        // the segment before is through with its own, they do not.
+        if (t == min(sg.t0 + 2, t_all - 1)) load_q(sg);
         const int key = t * kTile + lw * 32 + lane;
         const char *kp = nullptr, *vp = nullptr;
         if (key < sg.cached) {

@@ -23,10 +23,11 @@ struct Segment {      // one CTA's consecutive work on one item
   int row0;           // first row of the item (row = token * group + head)
   int t0, t1;         // attention: key tiles; weights: row chunks
   int part;           // partial slot, or -1 when the item is whole
-  int n0, n1;         // attention: end of the key tiles of either row tile
+  int n0, n1;         // attention: end of the key tiles of either row tile;
+                      // weights: n0 pairs of key tiles
   int rows;           // attention: rows of the item
-  int key0;           // weights: first key of the item
-  int fill;           // weights: the item ends its sequence's keys
+  int key0;           // weights: first key
+  int fill;           // weights: the segment ends its sequence's keys
   int pad[2];
 };
 static_assert(sizeof(Segment) == 64, "segments are 16 ints");

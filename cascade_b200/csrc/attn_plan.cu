@@ -200,6 +200,10 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
       !fwd || (int64_t)max_new * group > kTile ? 2 * kTile : kTile;
   p.row_tile = row_tile;
 
+  // Weights of at most 128 rows a sequence: keys stream by the rows.
+  const bool by_keys =
+      !fwd && (int64_t)std::min(max_new, p.window) * group <= kTile;
+
   std::vector<Item> items;
   int64_t count = 0, tok0 = 0;
   for (int b = 0; b < p.batch; ++b) {
@@ -244,7 +248,16 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
         it.seg.rows = w * group;
         const int chunks = (int)div_up((uint64_t)it.seg.rows, kTile);
         const int keys = c + n;
+        if (by_keys) {
+          // one chunk of rows at most: a unit is a pair of key tiles
+          it.seg.t0 = 0;
+          it.seg.t1 = std::max(1, (int)div_up(keys, row_tile));
+          it.seg.n1 = chunks;
+          items.push_back(it);
+          continue;
+        }
         int key = 0;
+        it.seg.n0 = 1;
         do {
           // rows of tokens before key - cached see none of these keys
           const int64_t first =
@@ -274,12 +287,12 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
                       std::min<int64_t>(row_tile, (int64_t)max_new * group);
   } else {
     const int64_t rows = (int64_t)std::min(max_new, p.window) * group;
-    cost.unit = 200 + 1000.0 * std::min<int64_t>(rows, kTile) / kTile;
-    cost.unit_bytes = 0;
-    cost.segment = 1500;
-    cost.part_bytes = 8.0 * row_tile;
+    cost.unit = by_keys ? 400 + 800.0 * rows / kTile : 1200;
+    cost.unit_bytes = by_keys ? 2 * tile_bytes : 0;
+    cost.segment = by_keys ? 500 : 1500;
+    cost.part_bytes = by_keys ? 0 : 8.0 * row_tile;
   }
-  cost.merge = 3500;
+  cost.merge = by_keys ? 0 : 3500;        // runs of keys need no merge
 
   std::vector<std::vector<Segment>> best;
   std::vector<Merge> merges;
@@ -311,6 +324,10 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
       }
     }
     if (n_best) best = equal_runs(items, n_best, cost, fwd, &merges, &parts);
+    if (by_keys) {
+      merges.clear();
+      parts = 0;
+    }
   }
   size_t segments = 0;
   for (const auto &v : best) segments += v.size();
@@ -338,6 +355,14 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
       if (fwd) {
         s.n0 = std::max(s.t0, std::min(s.n0, s.t1));
         s.n1 = std::max(s.t0, std::min(s.n1, s.t1));
+      } else if (by_keys) {
+        // from units to keys, pairs and the one chunk
+        s.key0 = s.t0 * row_tile;
+        s.n0 = s.t1 - s.t0;
+        s.fill = s.t1 * row_tile >= s.n_new + s.cached;
+        s.t0 = 0;
+        s.t1 = s.n1;
+        s.part = -1;
       }
       out[at++] = s;
     }

@@ -8,7 +8,7 @@ namespace {
 
 constexpr int kWThreads = 416;     // 2 x 4 summing warps, 4 loaders, MMA
 constexpr int kKeys = 2 * kTile;   // keys of an item
-constexpr int kKSlots = 2, kQSlots = 3;
+constexpr int kKSlots = 4, kQSlots = 3;   // tiles of 128 keys, of 128 rows
 
 struct WeightArgs {
   KvSource kv;
@@ -38,7 +38,7 @@ struct WControl {
 
 template <int D>
 constexpr int weights_smem() {
-  return (2 * kKSlots + kQSlots) * kTile * D * 2 + (int)sizeof(WControl);
+  return (kKSlots + kQSlots) * kTile * D * 2 + (int)sizeof(WControl);
 }
 static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
 
@@ -47,20 +47,21 @@ static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
 // K Q^T, with 128 keys as the rows of a tcgen05 tile: a thread owns one key
 // and adds along its own row, so the sum over the rows of all heads of a
 // group needs no reduction across threads and no atomics, and its order is
-// fixed.  256 keys stay resident while chunks of up to 128 query rows
-// stream by; a decode step's few rows are one chunk of N = 16, 32, ...
-// columns, and the keys stream.  Key j is seen by the rows of tokens from j
-// on, so a thread's mask is one row number.  A chunk's sum is taken by
-// itself before it joins the total.
+// fixed.  Two warpgroups take 128 keys each (a pair).  With many query rows
+// a segment is one pair that stays resident while chunks of 128 rows stream
+// by; with up to 128 rows (a decode step, a short window) it is a run of
+// pairs that stream by one resident chunk of N = 32, 64, ... columns.  Key j
+// is seen by the rows of tokens from j on, so a thread's mask is one row
+// number.  A chunk's sum is taken by itself before it joins the total.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kWThreads, 1)
     attn_weights_kernel(const __grid_constant__ WeightArgs a) {
   constexpr int kTileBytes = kTile * D * 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sm_k = smem_u32(smem);
-  const uint32_t sm_q = sm_k + 2 * kKSlots * kTileBytes;
+  const uint32_t sm_q = sm_k + kKSlots * kTileBytes;
   WControl &ct = *reinterpret_cast<WControl *>(
-      smem + (2 * kKSlots + kQSlots) * kTileBytes);
+      smem + (kKSlots + kQSlots) * kTileBytes);
   volatile int *give_up = &ct.give_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -101,69 +102,73 @@ __global__ void __launch_bounds__(kWThreads, 1)
     const int w = warp >> 2;
     const int kt = w * kTile + (warp & 3) * 32 + lane;   // key of the item
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
-    uint32_t chunk_no = 0;
+    uint32_t step = 0, q_no = 0;
     for (int si = seg_begin; si < seg_end; ++si) {
       const Segment sg = segs[si];
       const int total = sg.cached + sg.n_new;
-      const int key = sg.key0 + kt;
-      bool there = key < total;
-      if (there && key < sg.cached) there = page_of(a.kv, sg.b, key) >= 0;
-      const int64_t wi = (int64_t)sg.hk;
-      float prev = 0.f;
-      if (key < total && a.before != nullptr)
-        prev = a.before[sg.b * a.b_seq + wi * a.b_head + key];
-      // rows from `from` on see this key
-      const int64_t from =
-          (int64_t)(key - sg.cached - sg.row0) * a.group;
-      float sum = 0.f;
-      for (int ch = sg.t0; ch < sg.t1; ++ch, ++chunk_no) {
-        const uint32_t buf = chunk_no & 1, slot = chunk_no % kQSlots;
-        const int n = min(kTile, sg.rows - ch * kTile);
-        mbar_wait(smem_u32(&ct.s_full[w][buf]), (chunk_no >> 1) & 1, give_up);
-        tc_fence_after();
-        const float4 *l4 = reinterpret_cast<const float4 *>(ct.lse2[slot]);
-        const int64_t hidden = from - (int64_t)ch * kTile;
-        const bool whole = __all_sync(0xffffffffu, hidden <= 0);
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      const int64_t hk = sg.hk;
+      const float *before =
+          a.before != nullptr ? a.before + sg.b * a.b_seq + hk * a.b_head
+                              : nullptr;
+      float *out = a.out + sg.b * a.o_seq + hk * a.o_head;
+      for (int pair = 0; pair < sg.n0; ++pair) {
+        const int key = sg.key0 + pair * kKeys + kt;
+        bool there = key < total;
+        if (there && key < sg.cached) there = page_of(a.kv, sg.b, key) >= 0;
+        float prev = 0.f;
+        if (key < total && before != nullptr) prev = before[key];
+        // rows from `from` on see this key
+        const int64_t from =
+            (int64_t)(key - sg.cached - sg.row0) * a.group;
+        float sum = 0.f;
+        for (int ch = sg.t0; ch < sg.t1; ++ch, ++step) {
+          const uint32_t buf = step & 1;
+          const uint32_t slot = (q_no + ch - sg.t0) % kQSlots;
+          const int n = min(kTile, sg.rows - ch * kTile);
+          mbar_wait(smem_u32(&ct.s_full[w][buf]), (step >> 1) & 1, give_up);
+          tc_fence_after();
+          const float4 *l4 = reinterpret_cast<const float4 *>(ct.lse2[slot]);
+          const int64_t hidden = from - (int64_t)ch * kTile;
+          const bool whole = __all_sync(0xffffffffu, hidden <= 0);
+          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll 1
-        for (int i = 0; i < n; i += 32) {
-          uint32_t x[32];
-          tc_ld32(x, tm + buf * 128 + i);
-          tc_wait_ld();
-          tc_hold(x);
-          if (!whole || i + 32 > n) {
+          for (int i = 0; i < n; i += 32) {
+            uint32_t x[32];
+            tc_ld32(x, tm + buf * 128 + i);
+            tc_wait_ld();
+            tc_hold(x);
+            if (!whole || i + 32 > n) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;  // -inf
-          }
+              for (int e = 0; e < 32; ++e)
+                if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;  // -inf
+            }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 l = l4[i / 4 + e];
-            s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
-            s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
-            s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
-            s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
+            for (int e = 0; e < 8; ++e) {
+              const float4 l = l4[i / 4 + e];
+              s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
+              s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
+              s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
+              s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
+            }
           }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(smem_u32(&ct.s_empty[w][buf]));
+            if (pair + 1 == sg.n0) mbar_arrive(smem_u32(&ct.q_empty[slot]));
+          }
+          sum += (s0 + s1) + (s2 + s3);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(smem_u32(&ct.s_empty[w][buf]));
-          mbar_arrive(smem_u32(&ct.q_empty[slot]));
-        }
-        sum += (s0 + s1) + (s2 + s3);
+        if (!there) sum = 0.f;
+        if (sg.part >= 0)
+          a.part[(int64_t)sg.part * kKeys + kt] = sum;
+        else if (key < total)
+          out[key] = prev + sum;
       }
-      if (!there) sum = 0.f;
-      if (sg.part >= 0)
-        a.part[(int64_t)sg.part * kKeys + kt] = sum;
-      else if (key < total)
-        a.out[sg.b * a.o_seq + wi * a.o_head + key] = prev + sum;
+      q_no += sg.t1 - sg.t0;
       if (sg.fill && a.fill)
         for (int k = total + kt; k < a.width; k += kKeys)
-          a.out[sg.b * a.o_seq + wi * a.o_head + k] =
-              a.before != nullptr
-                  ? a.before[sg.b * a.b_seq + wi * a.b_head + k]
-                  : 0.f;
+          out[k] = before != nullptr ? before[k] : 0.f;
     }
   } else if (warp < 12) {
     // ------------------------------------------------------- loaders
@@ -186,60 +191,71 @@ __global__ void __launch_bounds__(kWThreads, 1)
         cp_async16(dst + place(lw * 32 + rl), src, p ? 16 : 0);
       }
     };
+    // lse of row r of chunk ch (in powers of two), and its Q row
+    auto row_at = [&](const Segment &sg, int ch, const char **src) {
+      const int r = lw * 32 + lane, row = ch * kTile + r;
+      *src = nullptr;
+      if (row >= sg.rows) return INFINITY;    // a row that counts for nothing
+      const int tok = row / a.group;
+      const int64_t head = sg.hk * a.group + row - tok * a.group;
+      const int64_t at = (int64_t)sg.tok0 + sg.row0 + tok;
+      *src = a.q + at * a.q_tok + head * a.q_head;
+      const float l = a.lse[at * a.l_tok + head * a.l_head];
+      return l == -INFINITY ? INFINITY : l * kLog2e;
+    };
+    auto load_chunk = [&](const Segment &sg, int ch) {
+      const uint32_t slot = q_no % kQSlots;
+      const char *src;
+      const float l2 = row_at(sg, ch, &src);
+      mbar_wait(smem_u32(&ct.q_empty[slot]), ((q_no / kQSlots) & 1) ^ 1,
+                give_up);
+      __syncwarp();
+      ct.lse2[slot][lw * 32 + lane] = l2;
+      // the MMA reads the rows up to the next multiple of 32
+      if (ch * kTile + lw * 32 < sg.rows)
+        copy_rows(sm_q + slot * kTileBytes, src);
+      // the copies arrive by themselves, the warp for what it wrote
+      cp_async_arrive(smem_u32(&ct.q_full[slot]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ct.q_full[slot]));
+      ++q_no;
+    };
     for (int si = seg_begin; si < seg_end; ++si) {
       const Segment sg = segs[si];
       if (sg.t0 >= sg.t1) continue;
       const int total = sg.cached + sg.n_new;
-      const char *kp[2] = {nullptr, nullptr};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = sg.key0 + h * kTile + lw * 32 + lane;
+      auto page_at = [&](int tile) {
+        const int key = sg.key0 + tile * kTile + lw * 32 + lane;
+        return key < sg.cached ? page_of(a.kv, sg.b, key) : -1;
+      };
+      const int tiles = 2 * sg.n0;
+      // pages of the next two tiles are looked up ahead
+      int page[2] = {page_at(0), page_at(1)};
+      for (int tile = 0; tile < tiles; ++tile) {
+        const int key = sg.key0 + tile * kTile + lw * 32 + lane;
+        const char *kp = nullptr;
         if (key < sg.cached) {
-          const int page = page_of(a.kv, sg.b, key);
-          if (page >= 0)
-            kp[h] = a.kv.kp + page * a.kv.kp_page + sg.hk * a.kv.kp_head +
-                    (key % a.kv.page) * a.kv.kp_tok;
+          if (page[0] >= 0)
+            kp = a.kv.kp + page[0] * a.kv.kp_page + sg.hk * a.kv.kp_head +
+                 (key % a.kv.page) * a.kv.kp_tok;
         } else if (key < total) {
-          kp[h] = a.kv.k + (int64_t)(sg.tok0 + key - sg.cached) * a.kv.k_tok +
-                  sg.hk * a.kv.k_head;
+          kp = a.kv.k + (int64_t)(sg.tok0 + key - sg.cached) * a.kv.k_tok +
+               sg.hk * a.kv.k_head;
         }
-      }
-      {
+        page[0] = page[1];
+        if (tile + 2 < tiles) page[1] = page_at(tile + 2);
         const uint32_t slot = k_no % kKSlots;
         mbar_wait(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1,
                   give_up);
         __syncwarp();
-        copy_rows(sm_k + 2 * slot * kTileBytes, kp[0]);
-        copy_rows(sm_k + (2 * slot + 1) * kTileBytes, kp[1]);
+        copy_rows(sm_k + slot * kTileBytes, kp);
         cp_async_arrive(smem_u32(&ct.k_full[slot]));
         ++k_no;
+        // the first chunk goes behind the first pair: its slot may still
+        // have to be freed, theirs are free already
+        if (tile == 1) load_chunk(sg, sg.t0);
       }
-      for (int ch = sg.t0; ch < sg.t1; ++ch, ++q_no) {
-        const uint32_t slot = q_no % kQSlots;
-        const int n = min(kTile, sg.rows - ch * kTile);
-        const int r = lw * 32 + lane;
-        const char *src = nullptr;
-        float l2 = INFINITY;                  // a row that counts for nothing
-        if (r < n) {
-          const int row = ch * kTile + r;
-          const int tok = row / a.group;
-          const int64_t head = sg.hk * a.group + row - tok * a.group;
-          const int64_t at = (int64_t)sg.tok0 + sg.row0 + tok;
-          src = a.q + at * a.q_tok + head * a.q_head;
-          const float l = a.lse[at * a.l_tok + head * a.l_head];
-          l2 = l == -INFINITY ? INFINITY : l * kLog2e;
-        }
-        mbar_wait(smem_u32(&ct.q_empty[slot]), ((q_no / kQSlots) & 1) ^ 1,
-                  give_up);
-        __syncwarp();
-        ct.lse2[slot][r] = l2;
-        // the MMA reads the rows up to the next multiple of 32
-        if (lw * 32 < n) copy_rows(sm_q + slot * kTileBytes, src);
-        // the copies arrive by themselves, the warp for what it wrote
-        cp_async_arrive(smem_u32(&ct.q_full[slot]));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ct.q_full[slot]));
-      }
+      for (int ch = sg.t0 + 1; ch < sg.t1; ++ch) load_chunk(sg, ch);
     }
     cp_async_wait_all();
   } else {
@@ -248,36 +264,43 @@ __global__ void __launch_bounds__(kWThreads, 1)
       const uint32_t issue = lane == 0;
       const uint32_t tm = uniform(tmem), sk = uniform(sm_k);
       const uint32_t sq = uniform(sm_q);
-      uint32_t k_no = 0, chunk_no = 0;
-      for (int si = uniform(seg_begin); si < (int)uniform(seg_end); ++si) {
+      uint32_t k_no = 0, step = 0, q_no = 0;
+      const int seg_last = uniform(seg_end);
+      for (int si = uniform(seg_begin); si < seg_last; ++si) {
         const int t0 = uniform(segs[si].t0), t1 = uniform(segs[si].t1);
-        const int rows = uniform(segs[si].rows);
+        const int rows = uniform(segs[si].rows), pairs = uniform(segs[si].n0);
         if (t0 >= t1) continue;
-        const uint32_t ks = k_no % kKSlots;
-        mbar_wait_warp(smem_u32(&ct.k_full[ks]), (k_no / kKSlots) & 1, give_up);
-        fence_async_proxy();
-        ++k_no;
-        for (int ch = t0; ch < t1; ++ch, ++chunk_no) {
-          const uint32_t buf = chunk_no & 1, slot = chunk_no % kQSlots;
-          const int n = min(kTile, (rows - ch * kTile + 31) / 32 * 32);
-          const uint32_t idesc = mma_idesc(kBf16, n, false);
-          mbar_wait_warp(smem_u32(&ct.q_full[slot]), (chunk_no / kQSlots) & 1,
-                    give_up);
-          fence_async_proxy();
-          const uint32_t q = tile_desc(sq + slot * kTileBytes, 0);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            mbar_wait_warp(smem_u32(&ct.s_empty[w][buf]),
-                      ((chunk_no >> 1) & 1) ^ 1, give_up);
-            tc_fence_after();
-            mma_rows<0, D / 16>(tm + w * 256 + buf * 128,
-                        tile_desc(sk + (2 * ks + w) * kTileBytes, 0), q,
-                        idesc, issue);
-            tc_commit(smem_u32(&ct.s_full[w][buf]), issue);
+        for (int pair = 0; pair < pairs; ++pair, k_no += 2) {
+          for (int ch = t0; ch < t1; ++ch, ++step) {
+            const uint32_t buf = step & 1, qi = q_no + ch - t0;
+            const uint32_t slot = qi % kQSlots;
+            const int n = min(kTile, (rows - ch * kTile + 31) / 32 * 32);
+            const uint32_t idesc = mma_idesc(kBf16, n, false);
+            const uint32_t q = tile_desc(sq + slot * kTileBytes, 0);
+            if (pair == 0)
+              mbar_wait_warp(smem_u32(&ct.q_full[slot]), (qi / kQSlots) & 1,
+                             give_up);
+#pragma unroll 1
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t ks = (k_no + w) % kKSlots;
+              if (ch == t0)
+                mbar_wait_warp(smem_u32(&ct.k_full[ks]),
+                               ((k_no + w) / kKSlots) & 1, give_up);
+              fence_async_proxy();
+              mbar_wait_warp(smem_u32(&ct.s_empty[w][buf]),
+                             ((step >> 1) & 1) ^ 1, give_up);
+              tc_fence_after();
+              mma_rows<0, D / 16>(tm + w * 256 + buf * 128,
+                                  tile_desc(sk + ks * kTileBytes, 0), q,
+                                  idesc, issue);
+              tc_commit(smem_u32(&ct.s_full[w][buf]), issue);
+              if (ch + 1 == t1) tc_commit(smem_u32(&ct.k_empty[ks]), issue);
+            }
+            if (pair + 1 == pairs)
+              tc_commit(smem_u32(&ct.q_empty[slot]), issue);
           }
-          tc_commit(smem_u32(&ct.q_empty[slot]), issue);
         }
-        tc_commit(smem_u32(&ct.k_empty[ks]), issue);
+        q_no += t1 - t0;
       }
       tc_commit(smem_u32(&ct.done), issue);
       int gave_up = 0;

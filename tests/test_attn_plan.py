@@ -62,6 +62,29 @@ def units(kind, new, cached, group, kv_heads, row_tile, tree, window):
     return out
 
 
+def check_key_runs(segs, info, new, cached, group, kv_heads, window, tok0):
+    """Weights of few rows: each segment is a run of key pairs."""
+    assert info.merges == info.parts == info.workspace_bytes == 0
+    runs = {}
+    for s in segs:
+        t0_, n, c, b, h, first, a, z, part, pairs, _, rows, key0, fill = (
+            int(x) for x in s[:14])
+        w = min(n, window)
+        assert (t0_, n, c) == (tok0[b], new[b], cached[b])
+        assert (first, rows, part) == (n - w, w * group, -1)
+        assert (a, z) == (0, -(-rows // TILE)) and z <= 1 and pairs >= 1
+        assert fill == (key0 + 256 * pairs >= n + c)
+        runs.setdefault((b, h), []).append((key0, key0 + 256 * pairs))
+    assert set(runs) == {(b, h) for b in range(len(new))
+                         for h in range(kv_heads)}
+    for (b, h), r in runs.items():
+        r.sort()
+        assert r[0][0] == 0
+        assert all(x[1] == y[0] for x, y in zip(r, r[1:]))
+        keys = new[b] + cached[b]
+        assert r[-1][1] >= keys and r[-1][0] < max(keys, 1)
+
+
 CASES = [
     ([1], [0]), ([1], [1000]), ([1] * 64, [6000 + 31 * i for i in range(64)]),
     ([16384], [0]), ([64] * 8, [4096] * 8), ([5, 0, 300, 1, 129], [0] * 5),
@@ -90,6 +113,10 @@ def test_every_unit_is_in_one_segment(kind, case, heads, kv_heads, dim, tree,
                  tree and kind == kvattn.FORWARD, window)
     got, parts = {}, {}
     tok0 = np.concatenate([[0], np.cumsum(new)])
+    most = max(new or [0])
+    if kind == kvattn.WEIGHTS and min(most, window) * group <= TILE:
+        return check_key_runs(segs, info, new, cached, group, kv_heads,
+                              window, tok0)
     for s in segs:
         t0_, n, c, b, h, row0, a, z, part, n0, n1, rows, key0, fill = (
             int(x) for x in s[:14])
