@@ -25,6 +25,7 @@ struct FwdArgs {
   const int32_t *plan;
   float *part_o, *part_lse;        // [slot][row tile rows][D], [slot][rows]
   int ctas, group, tree;
+  int out32;                       // rows of out are 32-byte aligned
   float scale, c;                  // c = scale * log2(e)
 };
 
@@ -47,6 +48,7 @@ struct Shape {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kQTiles = kDual ? 1 : 2;
   static constexpr int kSlots = D == 128 ? (kDual ? 6 : 5) : 12;
+  static constexpr int kAhead = kDual ? 2 : 1;
   static constexpr int kSmem =
       (kQTiles + kSlots) * kTileBytes + (int)sizeof(Control);
   static_assert(kSlots <= kMaxSlots, "ring");
@@ -179,6 +181,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               vis &= there[i];
               any |= vis;
+              // most 32-key pieces of a masked tile are seen whole
+              if (__all_sync(0xffffffffu, vis == 0xffffffffu)) continue;
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!((vis >> e) & 1)) x[i][e] = 0xff800000u;  // -inf
@@ -357,22 +361,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
             }
+            uint32_t v[8];
             if (sg.part >= 0) {
-              float4 *dst = reinterpret_cast<float4 *>(
-                  a.part_o + prow * D + col);
+              float *dst = a.part_o + prow * D + col;
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2],
-                                     o[4 * e + 3]);
+              for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  v[e] = __float_as_uint(o[8 * i + e]);
+                store32(dst + 8 * i, v, true);
+              }
             } else {
-              uint4 *dst = reinterpret_cast<uint4 *>(orow + col * 2);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                dst[e] = make_uint4(
-                    pack16<kBf16>(o[8 * e], o[8 * e + 1]),
-                    pack16<kBf16>(o[8 * e + 2], o[8 * e + 3]),
-                    pack16<kBf16>(o[8 * e + 4], o[8 * e + 5]),
-                    pack16<kBf16>(o[8 * e + 6], o[8 * e + 7]));
+              for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  v[e] = pack16<kBf16>(o[16 * i + 2 * e],
+                                       o[16 * i + 2 * e + 1]);
+                store32(orow + col * 2 + 32 * i, v, a.out32);
+              }
             }
           }
         }
@@ -487,9 +494,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int page = page_at(sg.t0);
       for (int t = sg.t0; t < t_all; ++t) {
-        // Q goes behind the segment's first two tiles: it has to wait until
+        // Q goes behind a tile or two of its segment: it has to wait until
         // the segment before is through with its own, they do not.
-        if (t == min(sg.t0 + 2, t_all - 1)) load_q(sg);
+        if (t == (si == seg_begin ? sg.t0
+                                  : min(sg.t0 + Sh::kAhead, t_all - 1)))
+          load_q(sg);
         const int key = t * kTile + lw * 32 + lane;
         const char *kp = nullptr, *vp = nullptr;
         if (key < sg.cached) {
@@ -776,6 +785,9 @@ extern "C" int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
   a.ctas = p.ctas;
   a.group = p.q_heads / p.kv_heads;
   a.tree = p.tree;
+  a.out32 = (((uintptr_t)args->out | (uint64_t)a.o_tok |
+              (uint64_t)a.o_head) &
+             31) == 0;
   a.scale = args->scale;
   a.c = args->scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -308,6 +308,22 @@ __device__ __forceinline__ void tc_hold(uint32_t (&x)[16]) {
   asm volatile("" : CB_K8(x, 0), CB_K8(x, 8));
 }
 
+// 32 bytes of one thread: one full sector, where the address allows it.
+__device__ __forceinline__ void store32(void *dst, const uint32_t (&v)[8],
+                                        bool aligned) {
+  if (aligned) {
+    asm volatile(
+        "st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+        "r"(v[6]), "r"(v[7])
+        : "memory");
+  } else {
+    uint4 *d = static_cast<uint4 *>(dst);
+    d[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    d[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

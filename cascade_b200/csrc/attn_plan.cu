@@ -17,9 +17,9 @@ int check_args(const cascade_attn_plan_info_t &p,
   CB_CHECK(p.segments == 0 || a.plan, CASCADE_ERR_INVALID,
            "null pointer argument");
   CB_CHECK(((uintptr_t)a.plan & 15) == 0 &&
-               ((uintptr_t)a.workspace & 15) == 0,
+               ((uintptr_t)a.workspace & 31) == 0,
            CASCADE_ERR_INVALID,
-           "the plan and the workspace must be 16-byte aligned");
+           "the plan must be 16-byte, the workspace 32-byte aligned");
   CB_CHECK(std::isfinite(a.scale) && a.scale > 0.f, CASCADE_ERR_INVALID,
            "scale must be finite and above 0");
   uint64_t bits = (uintptr_t)a.q | (uintptr_t)a.k;

@@ -221,7 +221,7 @@ typedef struct {
   int32_t width;       /* weights: keys of a row; >= the longest sequence */
   int32_t fill;        /* weights: 1 = positions behind a sequence's end are
                           written too (before's value, or 0) */
-  void *workspace;     /* device, info.workspace_bytes, 16-byte aligned */
+  void *workspace;     /* device, info.workspace_bytes, 32-byte aligned */
   uint64_t workspace_bytes;
 } cascade_attn_args_t;
 
