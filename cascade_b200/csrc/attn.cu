@@ -159,17 +159,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t x[4][32];
 #pragma unroll
           for (int i = 0; i < 4; ++i) tc_ld32(x[i], tm_s + i * 32);
-          const uint4 vw = *reinterpret_cast<const uint4 *>(
-              ct.valid[(tiles_done + t - sg.t0) & 7]);
-          const bool partial =
-              (vw.x & vw.y & vw.z & vw.w) != 0xffffffffu || t >= masked_from;
-          tc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tc_hold(x[i]);
-          if (partial) {
-            const uint32_t there[4] = {vw.x, vw.y, vw.z, vw.w};
+          const uint32_t *there = ct.valid[(tiles_done + t - sg.t0) & 7];
+          const uint4 vw = *reinterpret_cast<const uint4 *>(there);
+          if ((vw.x & vw.y & vw.z & vw.w) != 0xffffffffu || t >= masked_from) {
+            // What a row does not see becomes -inf in TMEM, 32 keys at a
+            // time: a loop, because unrolled its code would push the hot
+            // loops out of the instruction cache.
+            tc_wait_ld();
             uint32_t any = 0;
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < 4; ++i) {
               const int j0 = t * kTile + i * 32;
               const int nvis = min(max(lim - j0, 0), 32);
@@ -183,14 +181,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               any |= vis;
               // most 32-key pieces of a masked tile are seen whole
               if (__all_sync(0xffffffffu, vis == 0xffffffffu)) continue;
+              uint32_t z[32];
+              tc_ld32(z, tm_s + i * 32);
+              tc_wait_ld();
+              tc_hold(z);
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (!((vis >> e) & 1)) x[i][e] = 0xff800000u;  // -inf
+                if (!((vis >> e) & 1)) z[e] = 0xff800000u;
+              tc_st32(tm_s + i * 32, z);
             }
+            tc_wait_st();
             seen |= any != 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tc_ld32(x[i], tm_s + i * 32);
           } else {
             seen = true;
           }
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tc_hold(x[i]);
           float mx[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
