@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *give_up = &ct.give_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  let_next_start();
   if (sm_q & 1023) {               // the swizzle needs 1024-byte alignment
     if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1u);
     return;
@@ -676,7 +677,8 @@ template <int D, bool kBf16>
 __global__ void __launch_bounds__(256)
     attn_merge_kernel(const __grid_constant__ FwdArgs a, const Merge *merges,
                       int slot_rows) {
-  const Merge mg = merges[blockIdx.y];
+  const Merge mg = merges[blockIdx.y];   // the plan is not the kernel's
+  wait_for_previous();
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (r >= mg.rows) return;
@@ -725,12 +727,17 @@ int run_fwd(const FwdArgs &a, const cascade_attn_plan_info_t &p,
   // setmaxnreg hands the launch's registers from the loaders and the MMA
   // warps to the softmax warps: 256 x 192 + 128 x 72 + 128 x 56 = 512 x 128.
   // A launch with fewer would wait for ever, so it is refused.
-  cudaFuncAttributes fa;
-  CB_CUDA(cudaFuncGetAttributes(&fa, kernel));
-  CB_CHECK(fa.numRegs == 128, CASCADE_ERR_UNSUPPORTED,
-           "attention kernel built with an unexpected register count");
-  CB_CUDA(cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+  static std::atomic<uint64_t> done{0};
+  OncePerDevice once(&done);
+  if (once.pending()) {
+    cudaFuncAttributes fa;
+    CB_CUDA(cudaFuncGetAttributes(&fa, kernel));
+    CB_CHECK(fa.numRegs == 128, CASCADE_ERR_UNSUPPORTED,
+             "attention kernel built with an unexpected register count");
+    CB_CUDA(cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+    once.set();
+  }
   kernel<<<p.ctas, kThreads, Sh::kSmem, s>>>(a);
   count_launches(1);
   CB_CUDA(cudaGetLastError());
@@ -738,10 +745,9 @@ int run_fwd(const FwdArgs &a, const cascade_attn_plan_info_t &p,
     const Merge *merges = reinterpret_cast<const Merge *>(
         a.plan + seg_offset(p.ctas) + (int64_t)p.segments * 16);
     const dim3 grid((unsigned)div_up(p.merge_rows, 8), (unsigned)p.merges);
-    attn_merge_kernel<D, kBf16>
-        <<<grid, 256, 0, s>>>(a, merges, Sh::kQTiles * kTile);
+    CB_CUDA(launch_early(attn_merge_kernel<D, kBf16>, grid, dim3(256), 0, s,
+                         a, merges, Sh::kQTiles * kTile));
     count_launches(1);
-    CB_CUDA(cudaGetLastError());
   }
   return CASCADE_OK;
 }

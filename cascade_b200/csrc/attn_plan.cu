@@ -406,3 +406,8 @@ extern "C" int cascade_attn_plan(cascade_attn_plan_info_t *info,
     return CASCADE_ERR_NOMEM;
   }
 }
+
+extern "C" void cascade_attn_struct_sizes(size_t *plan_info, size_t *args) {
+  if (plan_info) *plan_info = sizeof(cascade_attn_plan_info_t);
+  if (args) *args = sizeof(cascade_attn_args_t);
+}

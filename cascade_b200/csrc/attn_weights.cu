@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
   volatile int *give_up = &ct.give_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  let_next_start();
   if (sm_k & 1023) {
     if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1u);
     return;
@@ -320,7 +321,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
 __global__ void __launch_bounds__(kKeys)
     weights_merge_kernel(const __grid_constant__ WeightArgs a,
                          const Merge *merges) {
-  const Merge mg = merges[blockIdx.x];
+  const Merge mg = merges[blockIdx.x];   // the plan is not the kernel's
+  wait_for_previous();
   const int key = mg.key0 + threadIdx.x;
   if (key >= mg.rows) return;
   float sum = 0.f;
@@ -337,8 +339,13 @@ int run_weights(const WeightArgs &a, const cascade_attn_plan_info_t &p,
                 cudaStream_t s) {
   auto *kernel = attn_weights_kernel<D, kBf16>;
   constexpr int smem = weights_smem<D>();
-  CB_CUDA(cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done{0};
+  OncePerDevice once(&done);
+  if (once.pending()) {
+    CB_CUDA(cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    once.set();
+  }
   kernel<<<p.ctas, kWThreads, smem, s>>>(a);
   count_launches(1);
   CB_CUDA(cudaGetLastError());
@@ -346,9 +353,9 @@ int run_weights(const WeightArgs &a, const cascade_attn_plan_info_t &p,
     const Segment *segs =
         reinterpret_cast<const Segment *>(a.plan + seg_offset(p.ctas));
     const Merge *merges = reinterpret_cast<const Merge *>(segs + p.segments);
-    weights_merge_kernel<<<p.merges, kKeys, 0, s>>>(a, merges);
+    CB_CUDA(launch_early(weights_merge_kernel, dim3(p.merges), dim3(kKeys), 0,
+                         s, a, merges));
     count_launches(1);
-    CB_CUDA(cudaGetLastError());
   }
   return CASCADE_OK;
 }

@@ -50,6 +50,7 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 // above that weight, and the lowest positions of those equal to it.
 __global__ void __launch_bounds__(kSelThreads)
     evict_select_kernel(const __grid_constant__ SelectArgs a) {
+  let_next_start();
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks();
   const int rank = (int)cluster.block_rank();
@@ -201,70 +202,106 @@ __global__ void __launch_bounds__(kSelThreads)
 }
 
 // ------------------------------------------------------------------ gather
-constexpr int kGatherTensors = 1024;   // descriptors of one launch
 constexpr int kGThreads = 256;
+constexpr int kGRows = 8;          // rows in flight per thread
 
+// The descriptors travel as kernel parameters, so a call needs no copy to
+// the device: 1024 of them (24 KiB) at most, or 16 in the small form, whose
+// launch is cheaper.
+template <int kTensors>
 struct GatherArgs {
-  const int32_t *keep;             // [items][heads][kept]
+  const int32_t *keep;             // [items / layers][heads][kept]
   char *out;                       // [items][2][heads][kept][row bytes]
   const int32_t *table;            // paged sources: [items][table_row]
-  int64_t table_row, stride_page;  // the latter in elements
-  int64_t table_cols;
-  int32_t page, pages, seq;        // seq: tokens of an unpaged source
-  int32_t heads, kept, row_bytes, elem, vec;
-  int32_t item0, shared_keep, layers;
-  cascade_kv_tensor_t t[kGatherTensors];
+  int64_t table_row, stride_page;  // the latter in bytes
+  int32_t table_cols, page, pages;
+  int32_t seq;                     // tokens of an unpaged source
+  int32_t heads, kept, per_row;    // vectors of a row
+  int32_t item0, layers;
+  cascade_kv_tensor_t t[kTensors]; // strides in bytes
 };
 
-// One thread copies one vector of one kept row; a block takes the rows of
-// one head of one tensor.  Each row of head_dim values is contiguous, so a
-// row's bytes move as full sectors whatever the row's neighbours do.
-template <typename V>
+// One thread copies one vector of each of kGRows kept rows; a block takes
+// rows of one head of one tensor.  Bound by HBM: a row of head_dim values is
+// contiguous, so its bytes move as full sectors wherever it lies.
+template <typename V, int kTensors>
 __global__ void __launch_bounds__(kGThreads)
-    evict_gather_kernel(const __grid_constant__ GatherArgs a) {
+    evict_gather_kernel(const __grid_constant__ GatherArgs<kTensors> a) {
   const int head = blockIdx.y % a.heads, ti = blockIdx.y / a.heads;
   const int item = a.item0 + (ti >> 1);
   const cascade_kv_tensor_t t = a.t[ti];
-  const int per_row = a.row_bytes / (int)sizeof(V);
   const int32_t *keep =
-      a.keep + ((int64_t)(a.shared_keep ? item / a.layers : item) * a.heads +
-                head) * a.kept;
+      a.keep + ((int64_t)(item / a.layers) * a.heads + head) * a.kept;
   const char *base = reinterpret_cast<const char *>(t.ptr) +
-                     (int64_t)head * t.stride_head * a.elem;
-  V *out = reinterpret_cast<V *>(
-      a.out + (((int64_t)(2 * a.item0 + ti)) * a.heads + head) * a.kept *
-                  (int64_t)a.row_bytes);
-  const int64_t units = (int64_t)a.kept * per_row;
-  constexpr int kPer = 4;
-  const int64_t first =
-      (int64_t)blockIdx.x * kGThreads * kPer + threadIdx.x;
-  V v[kPer];
+                     (int64_t)head * t.stride_head;
+  V *out = reinterpret_cast<V *>(a.out) +
+           (((int64_t)2 * a.item0 + ti) * a.heads + head) * a.kept *
+               (int64_t)a.per_row;
+  // threads of a row, rows of a step (a long row takes several steps)
+  const int width = min(a.per_row, kGThreads);
+  const int step = kGThreads / width;
+  const int row_in = threadIdx.x / width, c0 = threadIdx.x - row_in * width;
+  const int64_t r0 = (int64_t)blockIdx.x * step * kGRows + row_in;
+  if (row_in >= step) return;
+  wait_for_previous();             // which may be what chose the rows
+  const char *src[kGRows];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t u = first + i * kGThreads;
-    v[i] = V{};
-    if (u >= units) continue;
-    const int r = (int)(u / per_row), c = (int)(u - (int64_t)r * per_row);
+  for (int i = 0; i < kGRows; ++i) {
+    const int64_t r = r0 + i * step;
+    src[i] = nullptr;
+    if (r >= a.kept) continue;
     const int pos = keep[r];
-    const char *src = nullptr;
     if (a.table != nullptr) {
       if (pos >= 0 && pos / a.page < a.table_cols) {
         const int id =
             a.table[(int64_t)item * a.table_row + pos / a.page];
         if (id >= 0 && id < a.pages)
-          src = base + (id * a.stride_page +
-                        (int64_t)(pos % a.page) * t.stride_seq) * a.elem;
+          src[i] = base + id * a.stride_page +
+                   (int64_t)(pos % a.page) * t.stride_seq;
       }
     } else if (pos >= 0 && pos < a.seq) {
-      src = base + (int64_t)pos * t.stride_seq * a.elem;
+      src[i] = base + (int64_t)pos * t.stride_seq;
     }
-    if (src != nullptr) v[i] = reinterpret_cast<const V *>(src)[c];
   }
+  for (int c = c0; c < a.per_row; c += width) {
+    V v[kGRows];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t u = first + i * kGThreads;
-    if (u < units) out[u] = v[i];
+    for (int i = 0; i < kGRows; ++i)
+      v[i] = src[i] ? __ldcs(reinterpret_cast<const V *>(src[i]) + c) : V{};
+#pragma unroll
+    for (int i = 0; i < kGRows; ++i) {
+      const int64_t r = r0 + i * step;
+      if (r < a.kept) __stcs(out + r * a.per_row + c, v[i]);
+    }
   }
+}
+
+template <int kTensors>
+int run_gather(GatherArgs<kTensors> &a, const cascade_kv_tensor_t *src,
+               uint32_t tensors, uint32_t elem, int vec, uint32_t step_max,
+               unsigned blocks, cudaStream_t s) {
+  if (step_max > (uint32_t)kTensors) step_max = kTensors;
+  for (uint32_t t0 = 0; t0 < tensors; t0 += step_max) {
+    const uint32_t n = tensors - t0 < step_max ? tensors - t0 : step_max;
+    a.item0 = (int)(t0 / 2);
+    for (uint32_t i = 0; i < n; ++i) {
+      a.t[i] = src[t0 + i];
+      a.t[i].stride_head *= elem;
+      a.t[i].stride_seq *= elem;
+    }
+    const dim3 grid(blocks, n * a.heads), block(kGThreads);
+    if (vec == 16)
+      CB_CUDA(launch_early(evict_gather_kernel<uint4, kTensors>, grid, block,
+                           0, s, a));
+    else if (vec == 4)
+      CB_CUDA(launch_early(evict_gather_kernel<uint32_t, kTensors>, grid,
+                           block, 0, s, a));
+    else
+      CB_CUDA(launch_early(evict_gather_kernel<uint16_t, kTensors>, grid,
+                           block, 0, s, a));
+    count_launches(1);
+  }
+  return CASCADE_OK;
 }
 
 }  // namespace
@@ -312,9 +349,14 @@ extern "C" int cascade_kv_evict_select(
   const int64_t per = (int64_t)div_up(div_up(width, 32), ranks) * 32;
   size_t smem = sizeof(SelectShared);
   if (per <= kHeld) smem += (size_t)per * 4;
-  CB_CUDA(cudaFuncSetAttribute(evict_select_kernel,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(sizeof(SelectShared) + kHeld * 4)));
+  static std::atomic<uint64_t> done{0};
+  OncePerDevice once(&done);
+  if (once.pending()) {
+    CB_CUDA(cudaFuncSetAttribute(evict_select_kernel,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)(sizeof(SelectShared) + kHeld * 4)));
+    once.set();
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * ranks));
   cfg.blockDim = dim3(kSelThreads);
@@ -353,55 +395,47 @@ extern "C" int cascade_kv_evict_gather(
            "null pointer argument");
   CB_CHECK(!d_table || (page > 0 && table_cols >= 0), CASCADE_ERR_INVALID,
            "a page table needs a page size");
-  static thread_local GatherArgs a;
-  a.keep = d_keep;
-  a.out = static_cast<char *>(d_out);
-  a.table = d_table;
-  a.table_row = table_row;
-  a.table_cols = table_cols;
-  a.stride_page = stride_page;
-  a.page = (int)(page ? page : 1);
-  a.pages = (int)pages;
-  a.seq = (int)seq;
-  a.heads = (int)heads;
-  a.kept = (int)kept;
-  a.row_bytes = (int)(head_dim * elem_bytes);
-  a.elem = (int)elem_bytes;
-  a.shared_keep = layers > 1;
-  a.layers = (int)layers;
   // 16-byte vectors when every row starts on a 16-byte boundary, else
   // elements one by one.
-  uint64_t bits = (uintptr_t)d_out | (uint64_t)a.row_bytes |
+  const uint64_t row_bytes = (uint64_t)head_dim * elem_bytes;
+  uint64_t bits = (uintptr_t)d_out | row_bytes |
                   (uint64_t)(d_table ? stride_page * elem_bytes : 0);
-  for (uint32_t i = 0; i < items * 2; ++i) {
+  const uint32_t tensors = items * 2;
+  for (uint32_t i = 0; i < tensors; ++i) {
     CB_CHECK(src[i].ptr || (d_table ? pages == 0 : seq == 0),
              CASCADE_ERR_INVALID, "null pointer argument");
     bits |= src[i].ptr | (uint64_t)(src[i].stride_head * elem_bytes) |
             (uint64_t)(src[i].stride_seq * elem_bytes);
   }
   const int vec = bits & 15 ? (int)elem_bytes : 16;
-  const uint64_t units = (uint64_t)kept * (a.row_bytes / vec);
-  const uint64_t blocks = div_up(units, kGThreads * 4);
-  CB_CHECK(blocks <= INT32_MAX, CASCADE_ERR_INVALID, "kept is too large");
-  const uint32_t step_max = 65535 / heads < (uint32_t)kGatherTensors
-                                ? (65535 / heads) & ~1u
-                                : (uint32_t)kGatherTensors;
+  const uint32_t per_row = (uint32_t)(row_bytes / vec);
+  const uint32_t rows =
+      kGThreads / (per_row < kGThreads ? per_row : kGThreads) * kGRows;
+  const unsigned blocks = (unsigned)div_up(kept, rows);
+  const uint32_t step_max = (65535 / heads) & ~1u;
   CB_CHECK(step_max >= 2, CASCADE_ERR_INVALID, "too many heads");
+  auto fill = [&](auto &a) {
+    a.keep = d_keep;
+    a.out = static_cast<char *>(d_out);
+    a.table = d_table;
+    a.table_row = table_row;
+    a.table_cols = (int)(table_cols < INT32_MAX ? table_cols : INT32_MAX);
+    a.stride_page = stride_page * elem_bytes;
+    a.page = (int)(page ? page : 1);
+    a.pages = (int)pages;
+    a.seq = (int)seq;
+    a.heads = (int)heads;
+    a.kept = (int)kept;
+    a.per_row = (int)per_row;
+    a.layers = (int)layers;
+  };
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (uint32_t t0 = 0; t0 < items * 2; t0 += step_max) {
-    const uint32_t n =
-        items * 2 - t0 < step_max ? items * 2 - t0 : step_max;
-    a.item0 = (int)(t0 / 2);
-    for (uint32_t i = 0; i < n; ++i) a.t[i] = src[t0 + i];
-    const dim3 grid((unsigned)blocks, n * heads);
-    if (vec == 16)
-      evict_gather_kernel<uint4><<<grid, kGThreads, 0, s>>>(a);
-    else if (elem_bytes == 4)
-      evict_gather_kernel<uint32_t><<<grid, kGThreads, 0, s>>>(a);
-    else
-      evict_gather_kernel<uint16_t><<<grid, kGThreads, 0, s>>>(a);
-    count_launches(1);
-    CB_CUDA(cudaGetLastError());
+  if (tensors <= 16) {
+    GatherArgs<16> a;
+    fill(a);
+    return run_gather(a, src, tensors, elem_bytes, vec, step_max, blocks, s);
   }
-  return CASCADE_OK;
+  static thread_local GatherArgs<1024> a;
+  fill(a);
+  return run_gather(a, src, tensors, elem_bytes, vec, step_max, blocks, s);
 }

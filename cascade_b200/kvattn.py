@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 from . import _lib, kvwire
 from ._lib import check
@@ -55,25 +56,11 @@ class _PlanInfo(ctypes.Structure):
                                       ("workspace_bytes", _u64)]
 
 
-class _Args(ctypes.Structure):
-    """cascade_attn_args_t."""
-    _fields_ = [("dtype", _i32), ("pages", _i32), ("scale", _f32),
-                ("add", _i32), ("plan", _vp), ("q", _vp), ("k", _vp),
-                ("v", _vp)] + [(n, _i64) for n in (
-                    "q_tok", "q_head", "k_tok", "k_head", "v_tok",
-                    "v_head")] + [("k_pages", _vp), ("v_pages", _vp)] + [
-                        (n, _i64) for n in (
-                            "kp_page", "kp_head", "kp_tok", "vp_page",
-                            "vp_head", "vp_tok")] + [
-        ("table", _vp), ("table_row", _i64), ("mask", _vp),
-        ("mask_row", _i64), ("out", _vp), ("out_tok", _i64),
-        ("out_head", _i64), ("lse", _vp), ("lse_tok", _i64),
-        ("lse_head", _i64), ("before", _vp), ("before_seq", _i64),
-        ("before_head", _i64), ("weights", _vp), ("weights_seq", _i64),
-        ("weights_head", _i64), ("width", _i32), ("fill", _i32),
-        ("workspace", _vp), ("workspace_bytes", _u64)]
+# cascade_attn_args_t, in the order of _pack_args' arguments
+_ARGS = struct.Struct("@iifi4P6q2P6qPqPqPqqPqqPqqPqqiiPQ")
 
 
+_lib.register("cascade_attn_struct_sizes", None, [_vp, _vp])
 _lib.register("cascade_attn_plan", _int, [_vp, _vp, _vp, _vp, _sz])
 _lib.register("cascade_attn_forward", _int, [_vp, _vp, _vp])
 _lib.register("cascade_attn_weights", _int, [_vp, _vp, _vp])
@@ -148,6 +135,8 @@ class _Plan:
         self.head_dim, self.page_size = info.head_dim, info.page_size
         self.max_new, self.max_cached = info.max_new, info.max_cached
         self.max_keys, self.tree = info.max_keys, bool(info.tree)
+        self._heads = q_heads, kv_heads, head_dim
+        self._ptr, self._lib = self._buf.data_ptr(), _lib.load()
 
 
 class AttentionPlan(_Plan):
@@ -179,21 +168,28 @@ class WeightsPlan(_Plan):
 
 
 # ------------------------------------------------------------------ checks
-def _dtype(q):
+def _dtype_code(q):
     import torch
-    codes = {torch.float16: 0, torch.bfloat16: 1}
-    if q.dtype not in codes:
-        raise TypeError(f"q must be float16 or bfloat16, not {q.dtype}")
-    return codes[q.dtype]
+    if q.dtype is torch.float16:
+        return 0
+    if q.dtype is torch.bfloat16:
+        return 1
+    raise TypeError(f"q must be float16 or bfloat16, not {q.dtype}")
 
 
 def _strides(t):
     """Element strides with 0 for dimensions of one element, whose stride
     torch leaves arbitrary."""
-    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape, t.stride()))
 
 
 def _rows(name, t, shape, dtype, device):
+    """(address, strides) of a tensor of 16-bit rows."""
+    p, st = t.data_ptr(), t.stride()
+    if (t.shape == shape and t.dtype is dtype and t.device == device
+            and st[-1] == 1 and not (p | st[0] * 2 | st[1] * 2
+                                     | st[-2] * 2) & 15):
+        return p, st
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} must have shape {shape}; got "
                          f"{tuple(t.shape)}")
@@ -203,18 +199,18 @@ def _rows(name, t, shape, dtype, device):
     st = _strides(t)
     if st[-1] not in (0, 1):
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    align = 16 // t.element_size()
-    if t.data_ptr() % 16 or any(s % align for s in st[:-1]):
+    if p % 16 or any(s % 8 for s in st[:-1]):
         raise ValueError(f"{name}: rows must start on 16-byte boundaries")
-    return t.data_ptr(), st
+    return p, st
 
 
 def _no_grad(*tensors):
     import torch
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the attention operators have no backward pass: "
-                           "call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the attention operators have no backward "
+                                   "pass: call them under torch.no_grad()")
 
 
 def _writable(name, t):
@@ -222,47 +218,13 @@ def _writable(name, t):
         raise ValueError(f"{name} must not be an expanded tensor")
 
 
-def _common(plan, kind, q, k, v, k_pages, v_pages, page_table, scale):
-    """The arguments that both kinds of call share."""
-    if plan._info.kind != kind:
-        raise ValueError("the plan is of the other kind: AttentionPlan for "
-                         "attention, WeightsPlan for attention_weights")
-    dev, n = plan.device, plan.tokens
-    H, G, D = plan.q_heads, plan.kv_heads, plan.head_dim
-    if q.dim() != 3 or q.shape[0] < n:
-        raise ValueError(f"q must be [>= {n} tokens, {H}, {D}]; got "
-                         f"{tuple(q.shape)}")
-    rows = q.shape[0]
-    a = _Args(dtype=_dtype(q))
+def _scale(scale, dim):
     if scale is None:
-        a.scale = 1.0 / math.sqrt(D)
-    else:
-        a.scale = scale
-        if not (math.isfinite(scale) and a.scale > 0.0
-                and math.isfinite(a.scale)):
-            raise ValueError("scale must be finite and above 0")
-    a.q, st = _rows("q", q, (rows, H, D), q.dtype, dev)
-    a.q_tok, a.q_head = st[:2]
-    a.k, st = _rows("k", k, (rows, G, D), q.dtype, dev)
-    a.k_tok, a.k_head = st[:2]
-    if v is not None:
-        a.v, st = _rows("v", v, (rows, G, D), q.dtype, dev)
-        a.v_tok, a.v_head = st[:2]
-    if plan.max_cached:
-        if k_pages is None or page_table is None:
-            raise ValueError("the plan has cached tokens: pages and "
-                             "page_table are needed")
-        shape = (k_pages.shape[0], G, plan.page_size, D)
-        a.pages = shape[0]
-        a.k_pages, st = _rows("k_pages", k_pages, shape, q.dtype, dev)
-        a.kp_page, a.kp_head, a.kp_tok = st[:3]
-        if v_pages is not None:
-            a.v_pages, st = _rows("v_pages", v_pages, shape, q.dtype, dev)
-            a.vp_page, a.vp_head, a.vp_tok = st[:3]
-        a.table, a.table_row = _table(page_table, plan.batch,
-                                      plan._info.table_cols, dev)
-    a.plan = plan._buf.data_ptr()
-    return a
+        return dim ** -0.5
+    if not (math.isfinite(scale) and scale > 0.0
+            and 0.0 < ctypes.c_float(scale).value < math.inf):
+        raise ValueError("scale must be finite and above 0")
+    return scale
 
 
 def _table(page_table, batch, cols, dev):
@@ -271,33 +233,80 @@ def _table(page_table, batch, cols, dev):
             or page_table.shape[1] < cols):
         raise ValueError(f"page_table must be [{batch}, >= {cols}]; got "
                          f"{tuple(page_table.shape)}")
-    if page_table.dtype != torch.int32 or page_table.device != dev:
+    if page_table.dtype is not torch.int32 or page_table.device != dev:
         raise ValueError(f"page_table must be int32 on {dev}")
-    st = _strides(page_table)
-    if st[1] not in (0, 1):
+    st = page_table.stride()
+    if page_table.shape[1] > 1 and st[1] != 1:
         raise ValueError("page_table: rows must be contiguous")
-    return page_table.data_ptr(), st[0]
+    return page_table.data_ptr(), st[0] if batch > 1 else 0
 
 
-def _launch(plan, a, fn):
-    """Runs fn on the current stream of the plan's device."""
+_NO_KV = (0,) * 4
+
+
+def _call(plan, kind, fn, q, k, v, k_pages, v_pages, page_table, scale, add,
+          mask, out, lse, before, weights):
+    """Checks the arguments that both kinds of call share and runs fn on the
+    current stream of the plan's device.  mask: (address, stride); out, lse,
+    before: (address, strides); weights: (address, strides, width, fill)."""
     import torch
-    dev = plan.device
+    if plan._info.kind != kind:
+        raise ValueError("the plan is of the other kind: AttentionPlan for "
+                         "attention, WeightsPlan for attention_weights")
+    dev, dt = plan.device, q.dtype
+    rows, (H, G, D) = q.shape[0], plan._heads
+    if rows < plan.tokens:
+        raise ValueError(f"q must be [>= {plan.tokens} tokens, {H}, {D}]; "
+                         f"got {tuple(q.shape)}")
+    code = _dtype_code(q)
+    qp, qs = _rows("q", q, (rows, H, D), dt, dev)
+    kp, ks = _rows("k", k, (rows, G, D), dt, dev)
+    vp, vs = (0, _NO_KV) if v is None else _rows("v", v, (rows, G, D), dt,
+                                                 dev)
+    P = pkp = pvp = tp = trow = 0
+    pks = pvs = _NO_KV
+    if plan.max_cached:
+        if k_pages is None or page_table is None:
+            raise ValueError("the plan has cached tokens: pages and "
+                             "page_table are needed")
+        P = k_pages.shape[0]
+        shape = (P, G, plan.page_size, D)
+        pkp, pks = _rows("k_pages", k_pages, shape, dt, dev)
+        if v is not None:
+            if v_pages is None:
+                raise ValueError("pages is a pair (k_pages, v_pages)")
+            pvp, pvs = _rows("v_pages", v_pages, shape, dt, dev)
+        tp, trow = _table(page_table, plan.batch, plan._info.table_cols, dev)
+    scale = _scale(scale, D)
     if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            return _launch(plan, a, fn)
-    stream = torch.cuda.current_stream(dev)
-    if stream != plan._stream:
-        # the plan's memory must not be handed out while this call reads it
-        plan._buf.record_stream(stream)
-    size = plan._info.workspace_bytes
-    if size:
+        guard = torch.cuda.device(dev)
+    else:
+        guard = None
+    if guard is not None:
+        guard.__enter__()
+    try:
+        stream = torch.cuda.current_stream(dev)
+        if stream != plan._stream:
+            # the plan's memory must not be handed out while this call reads
+            plan._buf.record_stream(stream)
+        size = plan._info.workspace_bytes
         # freed on return: the allocator hands it out again only to work
         # ordered behind this call on the same stream
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        a.workspace = ws.data_ptr()
-        a.workspace_bytes = size
-    check(fn(plan._ref, ctypes.byref(a), stream.cuda_stream))
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        args = _ARGS.pack(
+            code, P, scale, add, plan._ptr, qp, kp, vp, qs[0], qs[1], ks[0],
+            ks[1], vs[0], vs[1], pkp, pvp, pks[0], pks[1], pks[2], pvs[0],
+            pvs[1], pvs[2], tp, trow, mask[0], mask[1], out[0], out[1][0],
+            out[1][1], lse[0], lse[1][0], lse[1][1], before[0], before[1][0],
+            before[1][1], weights[0], weights[1][0], weights[1][1],
+            weights[2], weights[3], ws.data_ptr() if size else 0, size)
+        check(fn(plan._ref, args, stream.cuda_stream))
+    finally:
+        if guard is not None:
+            guard.__exit__(None, None, None)
+
+
+_NONE = (0, (0, 0))
 
 
 # --------------------------------------------------------------- attention
@@ -305,38 +314,40 @@ def _forward(plan, q, k, v, mask, pages, page_table, scale, out, lse):
     import torch
     k_pages, v_pages = pages if pages is not None else (None, None)
     _no_grad(q, k, v, k_pages, v_pages)
-    if pages is not None and v_pages is None:
-        raise ValueError("pages is a pair (k_pages, v_pages)")
-    a = _common(plan, FORWARD, q, k, v, k_pages, v_pages, page_table, scale)
-    dev, shape = plan.device, (q.shape[0], plan.q_heads, plan.head_dim)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, q heads, dim]; got "
+                         f"{tuple(q.shape)}")
+    dev, rows = plan.device, q.shape[0]
+    H, _, D = plan._heads
+    mp = (0, 0)
     if mask is not None:
-        if (mask.dim() != 2 or mask.shape[0] != shape[0]
+        if (mask.dim() != 2 or mask.shape[0] != rows
                 or mask.shape[1] < plan.max_new):
-            raise ValueError(f"mask must be [{shape[0]}, >= {plan.max_new}]; "
+            raise ValueError(f"mask must be [{rows}, >= {plan.max_new}]; "
                              f"got {tuple(mask.shape)}")
-        if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev:
+        if (mask.dtype is not torch.bool and mask.dtype is not torch.uint8
+                ) or mask.device != dev:
             raise ValueError(f"mask must be bool or uint8 on {dev}")
-        st = _strides(mask)
-        if st[1] not in (0, 1) or (st[1] == 0 and mask.shape[1] > 1):
+        if mask.shape[1] > 1 and mask.stride(1) != 1:
             raise ValueError("mask: rows must be contiguous")
-        a.mask, a.mask_row = mask.data_ptr(), st[0]
+        mp = mask.data_ptr(), mask.stride(0)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
+        op = out.data_ptr(), (H * D, D)
     else:
         _writable("out", out)
-    a.out, st = _rows("out", out, shape, q.dtype, dev)
-    a.out_tok, a.out_head = st[:2]
+        op = _rows("out", out, (rows, H, D), q.dtype, dev)
     if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+        lse = torch.empty((rows, H), dtype=torch.float32, device=dev)
+        lp = lse.data_ptr(), (H, 1)
     else:
         _writable("lse", lse)
-        if (tuple(lse.shape) != shape[:2] or lse.dtype != torch.float32
+        if (tuple(lse.shape) != (rows, H) or lse.dtype != torch.float32
                 or lse.device != dev):
-            raise ValueError(f"lse must be float32 {shape[:2]} on {dev}")
-    a.lse = lse.data_ptr()
-    a.lse_tok, a.lse_head = _strides(lse)
-    if plan.tokens:
-        _launch(plan, a, _lib.load().cascade_attn_forward)
+            raise ValueError(f"lse must be float32 {(rows, H)} on {dev}")
+        lp = lse.data_ptr(), _strides(lse)
+    _call(plan, FORWARD, plan._lib.cascade_attn_forward, q, k, v, k_pages,
+          v_pages, page_table, scale, 0, mp, op, lp, _NONE, (0, (0, 0), 0, 0))
     return out, lse
 
 
@@ -371,6 +382,20 @@ def tree_attention(plan, q, k, v, mask, pages=None, page_table=None, *,
     return _forward(plan, q, k, v, mask, pages, page_table, scale, out, lse)
 
 
+def _weight_rows(name, t, plan):
+    import torch
+    if (t.dim() != 3 or t.shape[0] != plan.batch
+            or t.shape[1] != plan.kv_heads or t.shape[2] < plan.max_keys):
+        raise ValueError(
+            f"{name} must be [{plan.batch}, {plan.kv_heads}, >= "
+            f"{plan.max_keys}]; got {tuple(t.shape)}")
+    if t.dtype is not torch.float32 or t.device != plan.device:
+        raise ValueError(f"{name} must be float32 on {plan.device}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return t.data_ptr(), t.stride()
+
+
 def attention_weights(plan, q, k, lse, k_pages=None, page_table=None, *,
                       scale=None, add_to=None, out=None):
     """The attention weight that every token received: out[b, kv head, j] =
@@ -384,45 +409,32 @@ def attention_weights(plan, q, k, lse, k_pages=None, page_table=None, *,
     add_to's values (or 0).  In a given out those are left as they were."""
     import torch
     _no_grad(q, k, lse, k_pages, add_to)
-    a = _common(plan, WEIGHTS, q, k, None, k_pages, None, page_table, scale)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, q heads, dim]; got "
+                         f"{tuple(q.shape)}")
     dev = plan.device
-    if (tuple(lse.shape) != (q.shape[0], plan.q_heads)
-            or lse.dtype != torch.float32 or lse.device != dev):
+    if (lse.dim() != 2 or lse.shape[0] != q.shape[0]
+            or lse.shape[1] != plan.q_heads
+            or lse.dtype is not torch.float32 or lse.device != dev):
         raise ValueError("lse must be float32 "
                          f"{(q.shape[0], plan.q_heads)} on {dev}")
-    a.lse = lse.data_ptr()
-    a.lse_tok, a.lse_head = _strides(lse)
-
-    def rows(name, t):
-        if (t.dim() != 3 or tuple(t.shape[:2]) != (plan.batch, plan.kv_heads)
-                or t.shape[2] < plan.max_keys):
-            raise ValueError(
-                f"{name} must be [{plan.batch}, {plan.kv_heads}, >= "
-                f"{plan.max_keys}]; got {tuple(t.shape)}")
-        if t.dtype != torch.float32 or t.device != dev:
-            raise ValueError(f"{name} must be float32 on {dev}")
-        st = _strides(t)
-        if st[2] not in (0, 1) or (st[2] == 0 and t.shape[2] > 1):
-            raise ValueError(f"{name}: rows must be contiguous")
-        return t.data_ptr(), st
-
+    lp = lse.data_ptr(), lse.stride()
+    bp, add, fill = _NONE, 0, 0
+    if add_to is not None:
+        bp, add = _weight_rows("add_to", add_to, plan), 1
     if out is None:
-        width = plan.max_keys if add_to is None else add_to.shape[-1]
+        width = plan.max_keys if add_to is None else add_to.shape[2]
         out = torch.empty((plan.batch, plan.kv_heads, width),
                           dtype=torch.float32, device=dev)
-        a.fill = 1
+        wp, fill = (out.data_ptr(), out.stride()), 1
     else:
         _writable("out", out)
-    a.weights, st = rows("out", out)
-    a.weights_seq, a.weights_head = st[:2]
-    a.width = out.shape[2]
-    if add_to is not None:
-        a.before, st = rows("add_to", add_to)
-        a.before_seq, a.before_head = st[:2]
-        a.width = min(a.width, add_to.shape[2])
-        a.add = 1
-    if out.numel():
-        _launch(plan, a, _lib.load().cascade_attn_weights)
+        wp = _weight_rows("out", out, plan)
+        width = out.shape[2] if add_to is None else min(out.shape[2],
+                                                        add_to.shape[2])
+    _call(plan, WEIGHTS, plan._lib.cascade_attn_weights, q, k, None, k_pages,
+          None, page_table, scale, add, (0, 0), _NONE, lp, bp,
+          (wp[0], wp[1], width, fill))
     return out
 
 
@@ -458,7 +470,7 @@ def select_kept(weights, budget, recent=0, sink=0, lengths=None):
     keep = torch.empty(lead + [budget], dtype=torch.int32, device=dev)
     pad = 3 - len(lead)
     dims = (_i64 * 3)(*(lead + [1] * pad))
-    strides = (_i64 * 3)(*(st[:-1] + [0] * pad))
+    strides = (_i64 * 3)(*(st[:-1] + (0,) * pad))
     with torch.cuda.device(dev):
         check(_lib.load().cascade_kv_evict_select(
             weights.data_ptr(), dims, strides, weights.shape[-1],
@@ -480,7 +492,17 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     n = len(caches)
     if n == 0:
         raise ValueError("no caches to evict from")
-    desc, (L, H, S, D, dev, dt) = _cache_descriptors(caches)
+    tensors, L = [], 0
+    for c in caches:
+        pairs = kvwire.extract_kv_pairs(c)
+        if L not in (0, len(pairs)):
+            raise ValueError("every cache must have the same layers")
+        L = len(pairs)
+        for kv in pairs:
+            tensors += kv
+    if not tensors:
+        raise ValueError("a KV cache needs at least one layer")
+    desc, (H, S, D, dev, dt) = _descriptors(tensors)
     lead = (n, L, H) if weights.dim() == 4 else (n, H)
     if tuple(weights.shape) != lead + (S,) or weights.device != dev:
         raise ValueError(f"weights must be {lead + (S,)} on {dev}; got "
@@ -501,32 +523,40 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     return kv, keep
 
 
-def _cache_descriptors(caches):
-    """(host descriptor rows, geometry) of n caches of one shape."""
+def _descriptors(tensors):
+    """Host cascade_kv_tensor_t rows of [1, heads, seq, dim] or [heads, seq,
+    dim] tensors of one shape, dtype and device, and those."""
     import numpy as np
-    tensors, geo = [], None
-    for c in caches:
-        pairs = kvwire.extract_kv_pairs(c)
-        if geo is None:
-            geo = kvwire._geometry(pairs)
-        elif len(pairs) != geo[0]:
-            raise ValueError("every cache must have one shape, dtype and "
-                             "device")
-        for kv in pairs:
-            tensors += kv
-    L, H, S, D, dev, dt = geo
+    t0 = tensors[0]
+    shape, dt, dev = t0.shape, t0.dtype, t0.device
+    if dev.type != "cuda" or dt.itemsize not in (2, 4):
+        raise ValueError("KV tensors are CUDA tensors of 2- or 4-byte values")
+    if len(shape) not in (3, 4) or (len(shape) == 4 and shape[0] != 1):
+        raise ValueError("KV tensors are [1, heads, seq, dim]; got "
+                         f"{tuple(shape)}")
+    H, S, D = shape[-3:]
+    other = (1, H, S, D) if len(shape) == 3 else (H, S, D)
     rows = np.empty((len(tensors), 3), dtype=np.int64)
-    shapes = ((1, H, S, D), (H, S, D))
-    for i, t in enumerate(tensors):
-        if t.shape not in shapes or t.dtype != dt or t.device != dev:
-            raise ValueError("every cache must have one shape, dtype and "
+    strides = []
+    for t in tensors:
+        if (t.shape != shape and t.shape != other) or t.dtype is not dt \
+                or t.device != dev:
+            raise ValueError("every K and V must have one shape, dtype and "
                              "device")
-        st = t.stride()
-        if D > 1 and st[-1] != 1:
-            raise ValueError("head_dim must be contiguous (stride 1)")
-        rows[i] = (t.data_ptr(), st[-3] if H > 1 else 0,
-                   st[-2] if S > 1 else 0)
-    return rows, geo
+        strides.append(t.stride()[-3:])
+    rows[:, 0] = [t.data_ptr() for t in tensors]
+    if strides.count(strides[0]) == len(strides):
+        rows[:, 1:] = strides[0][:2]
+        strides = strides[:1]
+    else:
+        rows[:, 1:] = [s[:2] for s in strides]
+    if D > 1 and any(s[2] != 1 for s in strides):
+        raise ValueError("head_dim must be contiguous (stride 1)")
+    if H == 1:
+        rows[:, 1] = 0
+    if S == 1:
+        rows[:, 2] = 0
+    return rows, (H, S, D, dev, dt)
 
 
 def cache_views(kv):

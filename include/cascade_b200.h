@@ -238,6 +238,9 @@ int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
 int cascade_attn_weights(const cascade_attn_plan_info_t *plan,
                          const cascade_attn_args_t *args, void *stream);
 
+/* sizeof of the two structs above, for bindings to check. */
+void cascade_attn_struct_sizes(size_t *plan_info, size_t *args);
+
 /* Which tokens of a cache to keep: per row of weights (three leading
  * dimensions, strides in elements, `width` contiguous weights) the first
  * `sink` tokens, the last `recent`, and those of the largest weights, ties

@@ -195,11 +195,34 @@ def test_refusals(kw, text):
     assert e.value.code == 1
 
 
+def test_struct_layouts():
+    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+    _lib.load().cascade_attn_struct_sizes(ctypes.byref(a), ctypes.byref(b))
+    assert a.value == ctypes.sizeof(kvattn._PlanInfo)
+    assert b.value == kvattn._ARGS.size
+
+
+class Args:
+    """cascade_attn_args_t by field names."""
+    NAMES = ("dtype pages scale add plan q k v q_tok q_head k_tok k_head "
+             "v_tok v_head k_pages v_pages kp_page kp_head kp_tok vp_page "
+             "vp_head vp_tok table table_row mask mask_row out out_tok "
+             "out_head lse lse_tok lse_head before before_seq before_head "
+             "weights weights_seq weights_head width fill workspace "
+             "workspace_bytes").split()
+
+    def __init__(self, **kw):
+        self.__dict__.update(dict.fromkeys(self.NAMES, 0), **kw)
+
+    def pack(self):
+        return kvattn._ARGS.pack(*(getattr(self, n) for n in self.NAMES))
+
+
 def test_launches_refuse_bad_arguments():
     L = _lib.load()
     info, _ = make(kvattn.FORWARD, [4], [10])
-    args = kvattn._Args(scale=1.0)
-    call = lambda fn, i, a: fn(ctypes.byref(i), ctypes.byref(a), None)
+    args = Args(scale=1.0)
+    call = lambda fn, i, a: fn(ctypes.byref(i), a.pack(), None)
     assert L.cascade_attn_forward(None, None, None) == 1
     assert call(L.cascade_attn_weights, info, args) == 1       # wrong kind
     assert call(L.cascade_attn_forward, info, args) == 1       # no plan
