@@ -10,11 +10,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kDigit = 8, kBins = 1 << kDigit;
-constexpr int kHeld = 40960;       // weights of a slice held in shared memory
-
 struct SelectArgs {
   const float *w;
   int64_t stride[3];               // elements, of the three row dimensions
@@ -22,14 +17,6 @@ struct SelectArgs {
   const int32_t *lengths;          // per i0, or null: all `width`
   int width, budget, recent, sink;
   int32_t *keep;                   // [rows][budget]
-};
-
-struct SelectShared {
-  uint32_t hist[kBins * 32];       // one counter per bin and lane
-  uint32_t bins[2][kBins];         // this CTA's totals, read by the cluster
-  uint32_t above[kSelWarps], equal[kSelWarps];
-  uint32_t cta[2];                 // (above, equal) of this CTA's slice
-  uint32_t digit, left;
 };
 
 // Unsigned integers in the order of the weights: -0 equals 0, and NaN ranks
@@ -41,22 +28,31 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One cluster per row of weights; each CTA takes one slice of the row.  The
-// need-th largest weight is found digit by digit (4 x 8 bits): every lane of
-// a warp counts into its own column of the histogram, so equal weights (a
-// row of zeros, the common case after a long prompt) cost no more than
-// different ones; the counts of the cluster's CTAs are added over
-// distributed shared memory.  Then one ordered pass writes the positions
-// above that weight, and the lowest positions of those equal to it.
-__global__ void __launch_bounds__(kSelThreads)
+// One cluster per row of weights; each CTA takes one slice of the row, each
+// warp consecutive weights of that, kept in registers (kKeys a lane; 0: a
+// row too long for that is read again, from L2, in every round).  The
+// need-th largest weight is built from the top, a bit a round: the weights
+// that reach the longer prefix are counted, and the counts added up over the
+// CTA and, through distributed shared memory, the cluster.  The search ends
+// when a prefix has exactly the weights wanted.  Equal weights (a row of
+// zeros, the common case after a long prompt) cost what different ones do;
+// histograms in shared memory took longer (112 us for 1024 rows of 8192),
+// since their atomics pass about one lane a cycle.  Then one ordered pass
+// writes the positions above the weight found, and the lowest positions of
+// those equal to it.  Bound by the compares: 2 instructions a weight and
+// round, 20 to 32 rounds.
+template <int kThreads, int kKeys>
+__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : 1)
     evict_select_kernel(const __grid_constant__ SelectArgs a) {
+  constexpr int kWarps = kThreads / 32;
   let_next_start();
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks();
   const int rank = (int)cluster.block_rank();
-  extern __shared__ __align__(16) uint8_t raw[];
-  SelectShared &sh = *reinterpret_cast<SelectShared *>(raw);
-  float *held = reinterpret_cast<float *>(raw + sizeof(SelectShared));
+  __shared__ uint32_t warp_sum[2][kWarps];
+  __shared__ uint2 warp_count[2][kWarps];
+  __shared__ uint32_t cta_sum[2];
+  __shared__ uint32_t cta_total[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.x / ranks;
   const int i2 = (int)(row % a.dim2);
@@ -68,142 +64,147 @@ __global__ void __launch_bounds__(kSelThreads)
   int len = a.width;
   if (a.lengths != nullptr) len = min(max(a.lengths[i0], 0), a.width);
   const int kept = min(len, a.budget);
-  for (int i = kept + rank * kSelThreads + tid; i < a.budget;
-       i += ranks * kSelThreads)
+  for (int i = kept + rank * kThreads + tid; i < a.budget;
+       i += ranks * kThreads)
     keep[i] = -1;
   if (len <= a.budget) {           // the same for the whole cluster
-    for (int i = rank * kSelThreads + tid; i < len; i += ranks * kSelThreads)
+    for (int i = rank * kThreads + tid; i < len; i += ranks * kThreads)
       keep[i] = i;
     return;
   }
   // candidates are [sink, len - recent); the rest is kept anyway
   const int lo = a.sink, hi = len - a.recent;
   const int n = hi - lo;
-  int need = a.budget - a.sink - a.recent;
-  for (int i = rank * kSelThreads + tid; i < lo; i += ranks * kSelThreads)
+  const uint32_t need = a.budget - a.sink - a.recent;
+  for (int i = rank * kThreads + tid; i < lo; i += ranks * kThreads)
     keep[i] = i;
-  for (int i = rank * kSelThreads + tid; i < a.recent;
-       i += ranks * kSelThreads)
+  for (int i = rank * kThreads + tid; i < a.recent; i += ranks * kThreads)
     keep[a.budget - a.recent + i] = hi + i;
   if (need == 0) return;
 
-  // this CTA's slice, in whole warps' worths of candidates
-  const int per = (int)div_up(div_up(n, 32), ranks) * 32;
-  const int s0 = min(n, rank * per), s1 = min(n, s0 + per);
-  const float *src = w + lo + s0;
-  const int m = s1 - s0;
-  const bool in_smem = per <= kHeld;
-  if (in_smem) {
-    for (int i = tid; i < m; i += kSelThreads) held[i] = src[i];
-    src = held;
+  // this warp's candidates: per_warp consecutive ones, lane after lane
+  const int per_warp =
+      (int)div_up(div_up((uint64_t)n, 32), (uint64_t)ranks * kWarps) * 32;
+  const int64_t first = ((int64_t)rank * kWarps + warp) * per_warp;
+  const int begin = (int)(first < n ? first : n);
+  const int end = begin + per_warp < n ? begin + per_warp : n;
+  // order_of is above 0, so 0 stands for a candidate that is not there
+  auto fetch = [&](int i) -> uint32_t {
+    return i < end ? order_of(w[lo + i]) : 0u;
+  };
+  uint32_t key[kKeys > 0 ? kKeys : 1];
+  if (kKeys > 0) {
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) key[k] = fetch(begin + k * 32 + lane);
   }
 
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= kDigit) {
-    for (int i = tid; i < kBins * 32; i += kSelThreads) sh.hist[i] = 0;
-    __syncthreads();
-    const uint32_t high = shift == 24 ? 0 : 0xffffffffu << (shift + 8);
-    for (int i = tid; i < m; i += kSelThreads) {
-      const uint32_t u = order_of(src[i]);
-      if ((u & high) == prefix)
-        atomicAdd(&sh.hist[((u >> shift) & 255) * 32 + lane], 1u);
+  uint32_t least = 0;              // the need-th largest, so far
+#pragma unroll 1
+  for (int bit = 31, round = 0; bit >= 0; --bit, round ^= 1) {
+    const uint32_t t = least | (1u << bit);
+    uint32_t c = 0;
+    if (kKeys > 0) {
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) c += key[k] >= t;
+    } else {
+      for (int i = begin + lane; i < end; i += 32) c += fetch(i) >= t;
     }
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) warp_sum[round][warp] = c;
     __syncthreads();
-    uint32_t *bins = sh.bins[(shift >> 3) & 1];
-    if (tid < kBins) {
-      uint32_t c = 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) c += sh.hist[tid * 32 + ((i + tid) & 31)];
-      bins[tid] = c;
+    c = __reduce_add_sync(0xffffffffu,
+                          lane < kWarps ? warp_sum[round][lane] : 0u);
+    if (ranks > 1) {
+      if (tid == 0) cta_sum[round] = c;
+      cluster.sync();
+      c = __reduce_add_sync(
+          0xffffffffu,
+          lane < ranks ? *cluster.map_shared_rank(&cta_sum[round], lane)
+                       : 0u);
     }
-    cluster.sync();
-    if (warp == 0) {
-      // bins from the top, eight a lane: lane 0 holds 255..248
-      uint32_t c[8], own = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        c[e] = 0;
-        for (int r = 0; r < ranks; ++r)
-          c[e] += cluster.map_shared_rank(bins, r)[255 - (lane * 8 + e)];
-        own += c[e];
-      }
-      uint32_t incl = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      uint32_t before = incl - own;
-      if (before < (uint32_t)need && incl >= (uint32_t)need) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (before < (uint32_t)need && before + c[e] >= (uint32_t)need) {
-            sh.digit = 255 - (lane * 8 + e);
-            sh.left = need - before;
-            break;
-          }
-          before += c[e];
-        }
-      }
+    if (c >= need) least = t;
+    if (c == need) {               // these and no others: all above t - 1
+      least = t - 1;
+      break;
     }
-    __syncthreads();
-    prefix |= sh.digit << shift;
-    need = (int)sh.left;           // still to take among this digit's
   }
-  // now: everything above `prefix`, and the first `need` equal to it
-  const int warp_per = (int)div_up(div_up(m, 32), kSelWarps) * 32;
-  const int b0 = min(m, warp * warp_per), b1 = min(m, b0 + warp_per);
+  // now: everything above `least`, and the first ones equal to it
   uint32_t above = 0, equal = 0;
-  for (int i = b0; i < b1; i += 32) {
-    const uint32_t u = i + lane < b1 ? order_of(src[i + lane]) : 0;
-    const bool there = i + lane < b1;
-    above += __popc(__ballot_sync(0xffffffffu, there && u > prefix));
-    equal += __popc(__ballot_sync(0xffffffffu, there && u == prefix));
+  auto tally = [&](uint32_t u) {
+    above += __popc(__ballot_sync(0xffffffffu, u > least));
+    equal += __popc(__ballot_sync(0xffffffffu, u == least));
+  };
+  if (kKeys > 0) {
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) tally(key[k]);
+  } else {
+    for (int i = begin; i < end; i += 32) tally(fetch(i + lane));
   }
-  if (lane == 0) {
-    sh.above[warp] = above;
-    sh.equal[warp] = equal;
-  }
+  __syncthreads();                 // the counts of the last round are read
+  if (lane == 0) warp_count[0][warp] = make_uint2(above, equal);
   __syncthreads();
-  if (tid == 0) {
-    uint32_t x = 0, y = 0;
-    for (int i = 0; i < kSelWarps; ++i) {
-      const uint32_t cx = sh.above[i], cy = sh.equal[i];
-      sh.above[i] = x;
-      sh.equal[i] = y;
-      x += cx;
-      y += cy;
+  if (warp == 0) {
+    uint2 v = lane < kWarps ? warp_count[0][lane] : make_uint2(0u, 0u);
+    uint32_t x = v.x, y = v.y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t px = __shfl_up_sync(0xffffffffu, x, o);
+      const uint32_t py = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) {
+        x += px;
+        y += py;
+      }
     }
-    sh.cta[0] = x;
-    sh.cta[1] = y;
+    if (lane < kWarps) warp_count[1][lane] = make_uint2(x - v.x, y - v.y);
+    if (lane == 31) {
+      cta_total[0] = x;
+      cta_total[1] = y;
+    }
   }
-  cluster.sync();
-  uint32_t x = sh.above[warp], y = sh.equal[warp];
-  for (int r = 0; r < rank; ++r) {
-    const uint32_t *o = cluster.map_shared_rank(sh.cta, r);
-    x += o[0];
-    y += o[1];
+  if (ranks > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  uint32_t x = warp_count[1][warp].x, y = warp_count[1][warp].y;
+  uint32_t all_above = cta_total[0];
+  if (ranks > 1) {
+    uint32_t vx = 0, vy = 0, va = 0;
+    if (lane < ranks) {
+      const uint32_t *o = cluster.map_shared_rank(cta_total, lane);
+      va = o[0];
+      if (lane < rank) {
+        vx = va;
+        vy = o[1];
+      }
+    }
+    x += __reduce_add_sync(0xffffffffu, vx);
+    y += __reduce_add_sync(0xffffffffu, vy);
+    all_above = __reduce_add_sync(0xffffffffu, va);
   }
-  for (int i = b0; i < b1; i += 32) {
-    const bool there = i + lane < b1;
-    const uint32_t u = there ? order_of(src[i + lane]) : 0;
+  const uint32_t equals = need - all_above;   // how many of the equal ones
+  auto write = [&](uint32_t u, int i) {
     const uint32_t below = (1u << lane) - 1;
-    const uint32_t gt = __ballot_sync(0xffffffffu, there && u > prefix);
-    const uint32_t eq = __ballot_sync(0xffffffffu, there && u == prefix);
+    const uint32_t gt = __ballot_sync(0xffffffffu, u > least);
+    const uint32_t eq = __ballot_sync(0xffffffffu, u == least);
     const uint32_t my_eq = y + __popc(eq & below);
-    // kept before this one: all above, and the equal ones up to `need`
-    const uint32_t at = x + __popc(gt & below) + min(my_eq, (uint32_t)need);
-    if (there && (u > prefix || (u == prefix && my_eq < (uint32_t)need)))
-      keep[a.sink + at] = lo + s0 + i + lane;
+    const uint32_t at = x + __popc(gt & below) + min(my_eq, equals);
+    if (u > least || (u == least && my_eq < equals))
+      keep[a.sink + at] = lo + i;
     x += __popc(gt);
     y += __popc(eq);
+  };
+  if (kKeys > 0) {
+#pragma unroll
+    for (int k = 0; k < kKeys; ++k) write(key[k], begin + k * 32 + lane);
+  } else {
+    for (int i = begin; i < end; i += 32) write(fetch(i + lane), i + lane);
   }
-  cluster.sync();                  // the slices' totals are read remotely
+  if (ranks > 1) cluster.sync();   // the others read this CTA's totals
 }
 
 // ------------------------------------------------------------------ gather
 constexpr int kGThreads = 256;
-constexpr int kGRows = 8;          // rows in flight per thread
+constexpr int kGRows = 4;          // rows in flight per thread
 
 // The descriptors travel as kernel parameters, so a call needs no copy to
 // the device: 1024 of them (24 KiB) at most, or 16 in the small form, whose
@@ -267,11 +268,11 @@ __global__ void __launch_bounds__(kGThreads)
     V v[kGRows];
 #pragma unroll
     for (int i = 0; i < kGRows; ++i)
-      v[i] = src[i] ? __ldcs(reinterpret_cast<const V *>(src[i]) + c) : V{};
+      v[i] = src[i] ? reinterpret_cast<const V *>(src[i])[c] : V{};
 #pragma unroll
     for (int i = 0; i < kGRows; ++i) {
       const int64_t r = r0 + i * step;
-      if (r < a.kept) __stcs(out + r * a.per_row + c, v[i]);
+      if (r < a.kept) out[r * a.per_row + c] = v[i];
     }
   }
 }
@@ -320,7 +321,7 @@ extern "C" int cascade_kv_evict_select(
                (int64_t)recent + sink <= budget,
            CASCADE_ERR_INVALID,
            "budget must be above 0 and at least recent + sink");
-  const int64_t big = (int64_t)1 << 28;
+  const int64_t big = (int64_t)1 << 27;
   CB_CHECK(dims[0] <= big && dims[1] <= big && dims[2] <= big &&
                dims[0] * dims[1] <= big && dims[0] * dims[1] * dims[2] <= big,
            CASCADE_ERR_INVALID, "too many rows of weights");
@@ -339,37 +340,33 @@ extern "C" int cascade_kv_evict_select(
   a.recent = recent;
   a.sink = sink;
   a.keep = d_keep;
-  // One CTA reads about 4096 weights a microsecond, so a row is spread over
-  // more CTAs while SMs are idle and each still has that much to do; a
-  // slice that does not fit shared memory is read from L2 in every pass.
-  int ranks = 1;
-  while (ranks < 8 && rows * ranks * 2 <= 2 * sm_count() &&
-         width / (ranks * 2) >= 2048)
-    ranks *= 2;
-  const int64_t per = (int64_t)div_up(div_up(width, 32), ranks) * 32;
-  size_t smem = sizeof(SelectShared);
-  if (per <= kHeld) smem += (size_t)per * 4;
-  static std::atomic<uint64_t> done{0};
-  OncePerDevice once(&done);
-  if (once.pending()) {
-    CB_CUDA(cudaFuncSetAttribute(evict_select_kernel,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)(sizeof(SelectShared) + kHeld * 4)));
-    once.set();
+  // 8192 weights fit one CTA's registers at 16 a lane.  Longer rows are
+  // spread over clusters of such CTAs while there are SMs for them, else
+  // over CTAs of 1024 lanes of 32; beyond 8 of those they stay in L2.
+  int64_t ranks = 1;
+  while (ranks * 8192 < width) ranks *= 2;
+  auto *kernel = evict_select_kernel<512, 16>;
+  int threads = 512;
+  if (ranks > 8 || (ranks > 1 && rows * ranks > 2 * sm_count())) {
+    threads = 1024;
+    ranks = 1;
+    while (ranks * 32768 < width) ranks *= 2;
+    kernel = ranks <= 8 ? evict_select_kernel<1024, 32>
+                        : evict_select_kernel<1024, 0>;
+    if (ranks > 8) ranks = 8;
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * ranks));
-  cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(threads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CB_CUDA(cudaLaunchKernelEx(&cfg, evict_select_kernel, a));
+  CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   count_launches(1);
   return CASCADE_OK;
 }
