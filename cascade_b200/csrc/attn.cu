@@ -1,6 +1,6 @@
 // Attention over KV caches: causal prompts and trees of drafted tokens, with
 // grouped heads, over cached tokens in pages followed by new packed tokens.
-#include <cfloat>
+#include <type_traits>
 
 #include "attn.cuh"
 #include "kernels.cuh"
@@ -43,14 +43,25 @@ struct Control {
   int bad_v;                       // a masked tile held inf or NaN
 };
 
-template <int D, bool kDual>
+// Three forms of the kernel, by the rows of an item.
+enum Form {
+  kTwoRows,      // up to 256: two row tiles take turns on each key tile
+  kTwoKeys,      // up to 128: one row tile, two key tiles at a time
+  kFewRows,      // up to 16: the same, and the four warps of a warpgroup
+};               // share out a key tile's columns
+
+template <int D, int kForm>
 struct Shape {
+  static constexpr bool kDual = kForm != kTwoRows;
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kQTiles = kDual ? 1 : 2;
-  static constexpr int kSlots = D == 128 ? (kDual ? 6 : 5) : 12;
+  // the form for few rows joins its warps' results in one tile's room
+  static constexpr int kJoin = kForm == kFewRows ? 1 : 0;
+  static constexpr int kSlots =
+      D == 128 ? (kDual ? 6 - kJoin : 5) : 12 - kJoin;
   static constexpr int kAhead = kDual ? 2 : 1;
   static constexpr int kSmem =
-      (kQTiles + kSlots) * kTileBytes + (int)sizeof(Control);
+      (kQTiles + kSlots + kJoin) * kTileBytes + (int)sizeof(Control);
   static_assert(kSlots <= kMaxSlots, "ring");
   static_assert(kSmem <= 232448, "shared memory of one SM");
 };
@@ -59,6 +70,65 @@ struct Shape {
 __device__ __forceinline__ int first_masked_tile(const Segment &s, int group,
                                                  int tree) {
   return (s.cached + (tree ? 0 : s.row0 / group + 1)) / kTile;
+}
+
+// A row's maximum grows to m_new: its sum and its row of O follow.
+template <int D>
+__device__ __forceinline__ void raise_maximum(float &m, float &l, float m_new,
+                                              bool first, float c,
+                                              uint32_t tm_o) {
+  if (!first) {
+    const float f = m == -INFINITY ? (l == 0.f ? 1.f : 0.f)
+                                   : ex2((m - m_new) * c);
+    l *= f;
+#pragma unroll 1
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t o[16];
+      tc_ld16(o, tm_o + i * 16);
+      tc_wait_ld();
+      tc_hold(o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+      tc_st16(tm_o + i * 16, o);
+    }
+  }
+  m = m_new;
+}
+
+// The part of one value of O that zeros stood in for: a row of V that a
+// masked tile had cleared of inf and NaN gives them back to rows that see it.
+template <bool kBf16>
+__device__ __forceinline__ float cleared(uint16_t bits) {
+  constexpr uint16_t ex = kBf16 ? 0x7f80 : 0x7c00;
+  constexpr uint16_t mant = kBf16 ? 0x007f : 0x03ff;
+  if ((bits & ex) != ex) return 0.f;
+  return (bits & mant) ? NAN : (bits & 0x8000) ? -INFINITY : INFINITY;
+}
+
+// Adds those of the segment's masked tiles [from, to) to kN columns.
+template <bool kBf16, int kN>
+__device__ __forceinline__ void give_back(float (&o)[kN], const KvSource &kv,
+                                          const Segment &sg, int from, int to,
+                                          int lim, const uint8_t *mrow,
+                                          int col) {
+  const int end = min(to * kTile, sg.cached + sg.n_new);
+  for (int j = from * kTile; j < end; ++j) {
+    const char *vp;
+    if (j < sg.cached) {
+      const int id = page_of(kv, sg.b, j);
+      if (id < 0) continue;
+      vp = kv.vp + id * kv.vp_page + sg.hk * kv.vp_head +
+           (j % kv.page) * kv.vp_tok;
+    } else {
+      if (mrow != nullptr ? !mrow[j - sg.cached] : j >= lim) continue;
+      vp = kv.v + (int64_t)(sg.tok0 + j - sg.cached) * kv.v_tok +
+           sg.hk * kv.v_head;
+    }
+#pragma unroll
+    for (int e = 0; e < kN; ++e)
+      o[e] += cleared<kBf16>(reinterpret_cast<const uint16_t *>(vp)[col + e]);
+  }
 }
 
 // ------------------------------------------------------------------ kernel
@@ -77,15 +147,17 @@ __device__ __forceinline__ int first_masked_tile(const Segment &s, int group,
 // take turns (one's MMAs run under the other's exponentials).  Up to 128
 // rows (decode): one row tile, and the two warpgroups take alternate key
 // tiles, each with its own m, l and O, joined in the epilogue.
-template <int D, bool kBf16, bool kDual>
+template <int D, bool kBf16, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_fwd_kernel(const __grid_constant__ FwdArgs a) {
-  using Sh = Shape<D, kDual>;
+    attn_fwd_kernel(const __grid_constant__ FwdArgs a,
+                    const __grid_constant__ TileMaps maps) {
+  using Sh = Shape<D, kForm>;
+  constexpr bool kDual = Sh::kDual, kFew = kForm == kFewRows;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sm_q = smem_u32(smem);
   const uint32_t sm_ring = sm_q + Sh::kQTiles * Sh::kTileBytes;
   Control &ct = *reinterpret_cast<Control *>(
-      smem + (Sh::kQTiles + Sh::kSlots) * Sh::kTileBytes);
+      smem + (Sh::kQTiles + Sh::kSlots + Sh::kJoin) * Sh::kTileBytes);
   volatile int *give_up = &ct.give_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -127,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int w = warp >> 2;                       // warpgroup
     const int rt = (warp & 3) * 32 + lane;         // row of the tile
-    const int r = (kDual ? 0 : w * kTile) + rt;    // row of the item
+    // row of the item: in the form for few rows every warp has them all
+    const int r = kFew ? lane : (kDual ? 0 : w * kTile) + rt;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tm_s = lane_base + w * 128;
     const uint32_t tm_o = lane_base + 256 + w * 128;
@@ -155,7 +228,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = t_first; t < n_end; t += kDual ? 2 : 1) {
         mbar_wait(smem_u32(&ct.s_full[w]), s_phase, give_up);
         s_phase ^= 1;
-        if (warp_on) {
+        if constexpr (kFew) {
+          // This warp's 32 of the tile's 128 keys.  Its rows of P are zero
+          // at the other warps' keys, so its rows of O are the part of its
+          // own: eight parts of each row are joined in the epilogue.
+          const int part = warp & 3;
+          tc_fence_after();
+          uint32_t x[32];
+          tc_ld32(x, tm_s + part * 32);
+          uint32_t vis = ct.valid[(tiles_done + t - sg.t0) & 7][part];
+          if (t >= masked_from) {
+            const int j0 = t * kTile + part * 32;
+            const int nvis = min(max(lim - j0, 0), 32);
+            uint32_t own = nvis == 32 ? 0xffffffffu : (1u << nvis) - 1;
+            if (mrow != nullptr && j0 + 32 > sg.cached) {
+              const int e = min(j0 + 32, sg.cached + sg.n_new);
+              for (int j = max(j0, sg.cached); j < e; ++j)
+                if (mrow[j - sg.cached]) own |= 1u << (j - j0);
+            }
+            vis &= own;
+          }
+          seen |= vis != 0;
+          tc_wait_ld();
+          tc_hold(x);
+          if (!__all_sync(0xffffffffu, vis == 0xffffffffu)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((vis >> e) & 1)) x[e] = 0xff800000u;    // -inf
+          }
+          float t0 = __uint_as_float(x[0]), t1 = __uint_as_float(x[1]);
+#pragma unroll
+          for (int e = 2; e < 32; e += 2) {
+            t0 = fmaxf(t0, __uint_as_float(x[e]));
+            t1 = fmaxf(t1, __uint_as_float(x[e + 1]));
+          }
+          const float top = fmaxf(t0, t1);
+          if (__any_sync(0xffffffffu, top > m + grow))
+            raise_maximum<D>(m, l, fmaxf(m, top), first, a.c, tm_o);
+          first = false;
+          const float mc = m == -INFINITY ? 0.f : m * a.c;
+          float s0 = 0.f, s1 = 0.f;
+          uint32_t p[16], none[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float y0 = ex2(fmaf(__uint_as_float(x[2 * e]), a.c, -mc));
+            const float y1 =
+                ex2(fmaf(__uint_as_float(x[2 * e + 1]), a.c, -mc));
+            s0 += y0;
+            s1 += y1;
+            p[e] = pack16<kBf16>(y0, y1);
+            none[e] = 0;
+          }
+          l += s0 + s1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i == part)
+              tc_st16(tm_s + i * 16, p);
+            else
+              tc_st16(tm_s + i * 16, none);
+          tc_wait_st();
+          tc_fence_before();
+        } else if (warp_on) {
           tc_fence_after();
           uint32_t x[4][32];
 #pragma unroll
@@ -211,26 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           // m == -inf: any finite top is growth
-          if (__any_sync(0xffffffffu, top > m + grow)) {
-            const float m_new = fmaxf(m, top);
-            if (!first) {
-              const float f = m == -INFINITY ? (l == 0.f ? 1.f : 0.f)
-                                             : ex2((m - m_new) * a.c);
-              l *= f;
-#pragma unroll 1
-              for (int i = 0; i < D / 16; ++i) {
-                uint32_t o[16];
-                tc_ld16(o, tm_o + i * 16);
-                tc_wait_ld();
-                tc_hold(o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tc_st16(tm_o + i * 16, o);
-              }
-            }
-            m = m_new;
-          }
+          if (__any_sync(0xffffffffu, top > m + grow))
+            raise_maximum<D>(m, l, fmaxf(m, top), first, a.c, tm_o);
           first = false;
           const float mc = m == -INFINITY ? 0.f : m * a.c;
           float s0 = 0.f, s1 = 0.f;
@@ -259,6 +374,139 @@ __global__ void __launch_bounds__(kThreads, 1)
       tiles_done += t_all - sg.t0;
 
       // ---------------------------------------------------- epilogue
+      if constexpr (kFew) {
+        const int part = warp & 3;
+        const bool steps = n_end > t_first;
+        const bool steps2 = w ? true : sg.t1 > sg.t0 + 1;
+        ct.ml[w][rt] = make_float2(m, seen && l == 0.f ? -1.f : l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        float mm = -INFINITY, lsum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          mm = fmaxf(mm, ct.ml[i >> 2][(i & 3) * 32 + lane].x);
+        const float mc = mm == -INFINITY ? 0.f : mm * a.c;
+        float f1 = 0.f, f2 = 0.f;          // factors of this warp's two parts
+        seen = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 ml = ct.ml[i >> 2][(i & 3) * 32 + lane];
+          const float li = ml.y == -1.f ? 0.f : ml.y;
+          seen |= ml.y != 0.f;
+          // a part whose maximum is -inf holds no weight (or NaN)
+          const float f = ml.x == -INFINITY ? (li == 0.f ? 0.f : li)
+                                            : ex2(ml.x * a.c - mc);
+          lsum += li * f;
+          if ((i & 3) == part) {
+            if ((i >> 2) == w)
+              f1 = f;
+            else
+              f2 = f;
+          }
+        }
+        if (steps) {
+          mbar_wait(smem_u32(&ct.o_full[w]), o_phase, give_up);
+          o_phase ^= 1;
+        }
+        if (steps2) {
+          mbar_wait(smem_u32(&ct.o_full[w ^ 1]), o_phase2, give_up);
+          o_phase2 ^= 1;
+        }
+        tc_fence_after();
+        const bool empty = lsum == 0.f;
+        const float inv = empty ? 0.f : 1.f / lsum;
+        const float fill = part == 0 && empty && seen ? NAN : 0.f;
+        f1 *= inv;
+        f2 *= inv;
+        if (!steps || empty) f1 = 0.f;
+        if (!steps2 || empty) f2 = 0.f;
+        // Each warpgroup joins half of the columns: [part][row][column],
+        // 16-byte pieces permuted by the row so that lanes hit all banks.
+        constexpr int kCols = D / 2, kPieces = kCols / 4;
+        float4 *join = reinterpret_cast<float4 *>(
+                           smem + (1 + Sh::kSlots) * Sh::kTileBytes) +
+                       w * 4 * 16 * kPieces;
+#pragma unroll 1
+        for (int col = 0; col < kCols; col += 32) {
+          float o[32];
+          uint32_t u[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = fill;
+          if (steps) {
+            tc_ld32(u, tm_o + w * kCols + col);
+            tc_wait_ld();
+            tc_hold(u);
+            if (f1 != 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
+            }
+          }
+          if (steps2) {
+            tc_ld32(u, lane_base + 256 + (w ^ 1) * 128 + w * kCols + col);
+            tc_wait_ld();
+            tc_hold(u);
+            if (f2 != 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
+            }
+          }
+          if (row_on) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              join[(part * 16 + lane) * kPieces +
+                   ((col / 4 + e) ^ (lane & (kPieces - 1)))] =
+                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2],
+                              o[4 * e + 3]);
+          }
+        }
+        if (row_on && part == 0 && w == 0) {
+          const float lse =
+              empty ? -INFINITY : mm * a.scale + logf(lsum);
+          if (sg.part >= 0)
+            a.part_lse[(int64_t)sg.part * kTile + lane] = lse;
+          else
+            a.lse[(int64_t)(sg.tok0 + tok) * a.l_tok +
+                  (int64_t)head * a.l_head] = lse;
+        }
+        tc_fence_before();
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + w) : "memory");
+        for (int i = threadIdx.x & 127; i < sg.rows * kPieces; i += 128) {
+          const int row = i / kPieces, piece = i % kPieces;
+          float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 v = join[(q * 16 + row) * kPieces +
+                                  (piece ^ (row & (kPieces - 1)))];
+            o[0] += v.x;
+            o[1] += v.y;
+            o[2] += v.z;
+            o[3] += v.w;
+          }
+          const int col = w * kCols + piece * 4;
+          const int tk = (sg.row0 + row) / a.group;
+          const int hd = sg.hk * a.group + (sg.row0 + row) - tk * a.group;
+          if (ct.bad_v)
+            give_back<kBf16>(
+                o, a.kv, sg, max(sg.t0, masked_from), sg.t1,
+                a.tree ? sg.cached : sg.cached + tk + 1,
+                a.tree ? a.mask + (int64_t)(sg.tok0 + tk) * a.mask_row
+                       : nullptr,
+                col);
+          if (sg.part >= 0)
+            *reinterpret_cast<float4 *>(
+                a.part_o + ((int64_t)sg.part * kTile + row) * D + col) =
+                make_float4(o[0], o[1], o[2], o[3]);
+          else
+            *reinterpret_cast<uint2 *>(
+                a.out + (int64_t)(sg.tok0 + tk) * a.o_tok +
+                (int64_t)hd * a.o_head + col * 2) =
+                make_uint2(pack16<kBf16>(o[0], o[1]),
+                           pack16<kBf16>(o[2], o[3]));
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        continue;
+      }
       const bool steps = n_end > t_first;
       bool steps2 = false;                 // the other half's, two-tile form
       float m2 = -INFINITY, l2 = 0.f;
@@ -338,39 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (row_on) {
-            if (fix) {
-              // Masked tiles went in with inf and NaN as zeros; rows that
-              // see such a value get it back here.
-              const int jend = min(n_end * kTile, sg.cached + sg.n_new);
-              const int last = kDual ? min(sg.t1 * kTile,
-                                           sg.cached + sg.n_new)
-                                     : jend;
-              for (int j = max(sg.t0, masked_from) * kTile; j < last; ++j) {
-                const char *vp;
-                if (j < sg.cached) {
-                  const int id = page_of(a.kv, sg.b, j);
-                  if (id < 0) continue;
-                  vp = a.kv.vp + id * a.kv.vp_page + sg.hk * a.kv.vp_head +
-                       (j % a.kv.page) * a.kv.vp_tok;
-                } else {
-                  if (mrow != nullptr ? !mrow[j - sg.cached] : j >= lim)
-                    continue;
-                  vp = a.kv.v + (int64_t)(sg.tok0 + j - sg.cached) *
-                                    a.kv.v_tok +
-                       sg.hk * a.kv.v_head;
-                }
-                for (int e = 0; e < 32; ++e) {
-                  const uint16_t bits =
-                      reinterpret_cast<const uint16_t *>(vp)[col + e];
-                  const uint16_t ex = kBf16 ? 0x7f80 : 0x7c00;
-                  if ((bits & ex) != ex) continue;
-                  const uint16_t mant = kBf16 ? 0x007f : 0x03ff;
-                  o[e] += (bits & mant) ? NAN
-                          : (bits & 0x8000) ? -INFINITY
-                                            : INFINITY;
-                }
-              }
-            }
+            if (fix)
+              give_back<kBf16>(o, a.kv, sg, max(sg.t0, masked_from),
+                               kDual ? sg.t1 : n_end, lim, mrow, col);
             uint32_t v[8];
             if (sg.part >= 0) {
               float *dst = a.part_o + prow * D + col;
@@ -477,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       q_phase ^= 1;
       for (int qt = 0; qt < Sh::kQTiles; ++qt) {
-        const int r = qt * kTile + lw * 32 + lane;
+        const int r = kFew ? lane : qt * kTile + lw * 32 + lane;
         const char *src = nullptr;
         if (r < sg.rows) {
           const int tok = (sg.row0 + r) / a.group;
@@ -524,28 +742,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           kp = a.kv.k + n * a.kv.k_tok + sg.hk * a.kv.k_head;
           vp = a.kv.v + n * a.kv.v_tok + sg.hk * a.kv.v_head;
         }
+        const int this_page = page;
         if (t + 1 < t_all) page = page_at(t + 1);
         const uint32_t there = __ballot_sync(0xffffffffu, kp != nullptr);
-        {
+        // Tiles of one kind that every row sees whole go by TMA.
+        const bool by_page = maps.pages_ok && (t + 1) * kTile <= sg.cached;
+        const bool by_new = maps.new_ok && t * kTile >= sg.cached &&
+                            (t + 1) * kTile <= total && t < masked_from;
+        const int tok = sg.tok0 + t * kTile - sg.cached + lw * 32;
+        const int off = key % a.kv.page;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h, ++item) {        // K, V
           const uint32_t slot = item % Sh::kSlots;
           const uint32_t ph = (item / Sh::kSlots) & 1;
-          mbar_wait(smem_u32(&ct.empty[slot]), ph ^ 1, give_up);
-          __syncwarp();
-          if (lane == 0) ct.valid[tile_no & 7][lw] = there;
-          copy_rows(sm_ring + slot * Sh::kTileBytes, kp);
-          publish(smem_u32(&ct.full[slot]));
-          ++item;
-        }
-        {
-          const uint32_t slot = item % Sh::kSlots;
-          const uint32_t ph = (item / Sh::kSlots) & 1;
+          const uint32_t bar = smem_u32(&ct.full[slot]);
           const uint32_t dst = sm_ring + slot * Sh::kTileBytes;
           mbar_wait(smem_u32(&ct.empty[slot]), ph ^ 1, give_up);
           __syncwarp();
-          copy_rows(dst, vp);
-          if (t >= masked_from) check_finite(dst);
-          publish(smem_u32(&ct.full[slot]));
-          ++item;
+          if (h == 0 && lane == 0) ct.valid[tile_no & 7][lw] = there;
+          if (by_page) {
+            fetch_pages<D>(dst + lw * 32 * 128, maps, h ? &maps.vp : &maps.kp,
+                           this_page, off, a.kv.pages, sg.hk, bar, 33);
+          } else if (by_new) {
+            fetch_new<D>(dst + lw * 32 * 128, h ? &maps.v : &maps.k, tok,
+                         sg.hk, bar, 33);
+          } else {
+            copy_rows(dst, h ? vp : kp);
+            if (h == 1 && t >= masked_from) check_finite(dst);
+            publish(bar);
+          }
         }
         ++tile_no;
       }
@@ -719,11 +944,11 @@ __global__ void __launch_bounds__(256)
                          : top + logf(total);
 }
 
-template <int D, bool kBf16, bool kDual>
-int run_fwd(const FwdArgs &a, const cascade_attn_plan_info_t &p,
-            cudaStream_t s) {
-  using Sh = Shape<D, kDual>;
-  auto *kernel = attn_fwd_kernel<D, kBf16, kDual>;
+template <int D, bool kBf16, int kForm>
+int run_fwd(const FwdArgs &a, const TileMaps &maps,
+            const cascade_attn_plan_info_t &p, cudaStream_t s) {
+  using Sh = Shape<D, kForm>;
+  auto *kernel = attn_fwd_kernel<D, kBf16, kForm>;
   // setmaxnreg hands the launch's registers from the loaders and the MMA
   // warps to the softmax warps: 256 x 192 + 128 x 72 + 128 x 56 = 512 x 128.
   // A launch with fewer would wait for ever, so it is refused.
@@ -738,7 +963,7 @@ int run_fwd(const FwdArgs &a, const cascade_attn_plan_info_t &p,
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
     once.set();
   }
-  kernel<<<p.ctas, kThreads, Sh::kSmem, s>>>(a);
+  kernel<<<p.ctas, kThreads, Sh::kSmem, s>>>(a, maps);
   count_launches(1);
   CB_CUDA(cudaGetLastError());
   if (p.merges > 0) {
@@ -807,19 +1032,25 @@ extern "C" int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
   a.c = args->scale * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = args->dtype == CASCADE_KV_BF16;
-  const bool dual = p.row_tile == kTile;
-  if (p.head_dim == 128) {
-    if (dual)
-      return bf ? run_fwd<128, true, true>(a, p, s)
-                : run_fwd<128, false, true>(a, p, s);
-    return bf ? run_fwd<128, true, false>(a, p, s)
-              : run_fwd<128, false, false>(a, p, s);
-  }
-  if (dual)
-    return bf ? run_fwd<64, true, true>(a, p, s)
-              : run_fwd<64, false, true>(a, p, s);
-  return bf ? run_fwd<64, true, false>(a, p, s)
-            : run_fwd<64, false, false>(a, p, s);
+  TileMaps maps;
+  make_maps(*args, p, true, &maps);
+  const int form = p.row_tile > kTile ? kTwoRows
+                   : (int64_t)p.max_new * a.group > 16 ? kTwoKeys
+                                                       : kFewRows;
+  auto run = [&](auto d, auto b) {
+    constexpr int kD = decltype(d)::value;
+    constexpr bool kB = decltype(b)::value;
+    return form == kTwoRows   ? run_fwd<kD, kB, kTwoRows>(a, maps, p, s)
+           : form == kTwoKeys ? run_fwd<kD, kB, kTwoKeys>(a, maps, p, s)
+                              : run_fwd<kD, kB, kFewRows>(a, maps, p, s);
+  };
+  using std::integral_constant;
+  integral_constant<int, 128> d128;
+  integral_constant<int, 64> d64;
+  std::true_type yes;
+  std::false_type no;
+  if (p.head_dim == 128) return bf ? run(d128, yes) : run(d128, no);
+  return bf ? run(d64, yes) : run(d64, no);
 }
 
 extern "C" int cascade_diag_attn_timeouts(uint64_t *count) {

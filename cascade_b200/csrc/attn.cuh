@@ -3,8 +3,7 @@
 // host-side plan hands to the kernels.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include <cuda.h>
 
 #include "common.cuh"
 
@@ -420,6 +419,90 @@ void fill_source(const cascade_attn_args_t &a,
                  const cascade_attn_plan_info_t &p, KvSource *s);
 
 unsigned int *weights_timeouts_symbol();
+
+// Tensor maps for tiles that TMA can fetch: 64 columns of up to 32 rows of
+// one head, in the 128-byte swizzle.  A warp fetches its 32 rows of a tile
+// with a few instructions and nothing waits in registers or in the load/store
+// unit, whose queue of cp.async bounded a decode step at 5.1 TB/s.
+struct TileMaps {
+  CUtensorMap kp, vp;              // [page][head][token of the page][d]
+  CUtensorMap k, v;                // [token][head][d]
+  int pages_ok, new_ok;            // whether they can be used
+  int box;                         // rows of a page that one fetch takes
+};
+
+// Fills `m` for the call's tensors (the V maps where `with_v`).  Pages of 8,
+// 16, 32 or a multiple of 32 tokens can be fetched so; what has strides that
+// a tensor map does not take is left to cp.async.
+int make_maps(const cascade_attn_args_t &a, const cascade_attn_plan_info_t &p,
+              bool with_v, TileMaps *m);
+
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+               "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                   bar),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap *map,
+                                          int x, int y, int z, int w,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx"
+      "::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_rows3(uint32_t dst, const CUtensorMap *map,
+                                          int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx"
+      "::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// One warp's 32 rows of a tile of cached tokens: this lane's key is on page
+// `page` (-1: none, which reads as zeros) at token `off`.  Arrives on `bar`
+// like `plain` arrivals of the cp.async form.
+template <int D>
+__device__ __forceinline__ void fetch_pages(uint32_t dst, const TileMaps &m,
+                                            const CUtensorMap *map, int page,
+                                            int off, int pages, int hk,
+                                            uint32_t bar, uint32_t plain) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kHalves = D / 64;
+  if (lane == 0) {
+    mbar_expect(bar, 32 * D * 2);
+    mbar_arrive_n(bar, plain - 1);
+  }
+  __syncwarp();
+  const int piece = lane / kHalves, half = lane % kHalves;
+  const int row = piece * m.box;
+  const int pg = __shfl_sync(0xffffffffu, page, row & 31);
+  const int tok = __shfl_sync(0xffffffffu, off, row & 31);
+  if (row < 32)
+    tma_rows4(dst + half * (kTile * 128) + row * 128, map, half * 64, tok, hk,
+              pg < 0 ? pages : pg, bar);
+}
+// The same for new tokens from packed token `tok` on.
+template <int D>
+__device__ __forceinline__ void fetch_new(uint32_t dst, const CUtensorMap *map,
+                                          int tok, int hk, uint32_t bar,
+                                          uint32_t plain) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    mbar_expect(bar, 32 * D * 2);
+    mbar_arrive_n(bar, plain - 1);
+  }
+  __syncwarp();
+  if (lane < D / 64)
+    tma_rows3(dst + lane * (kTile * 128), map, lane * 64, hk, tok, bar);
+}
 
 // Page of cached token `key` of sequence b, or -1 when the table names none.
 __device__ __forceinline__ int page_of(const KvSource &s, int b, int key) {

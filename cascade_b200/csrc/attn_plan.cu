@@ -1,6 +1,7 @@
 // The host side of the attention operators: plans (which CTA does which part
 // of a batch) and the checks of a call's arguments.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -65,6 +66,83 @@ void fill_source(const cascade_attn_args_t &a,
   s->table_row = a.table_row;
   s->page = p.page_size > 0 ? p.page_size : 1;
   s->pages = a.pages;
+}
+
+namespace {
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+
+EncodeTiled encode_tiled() {
+  static std::atomic<EncodeTiled> cached{nullptr};
+  EncodeTiled fn = cached.load(std::memory_order_acquire);
+  if (fn == nullptr) {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000,
+                                         cudaEnableDefault, &found) ==
+            cudaSuccess &&
+        found == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(p);
+    cached.store(fn, std::memory_order_release);
+  }
+  return fn;
+}
+
+// A map of 64 x rows boxes; sizes and strides (in elements) from the second
+// dimension on.  False when the driver does not take them.
+bool encode(CUtensorMap *m, const void *base, int head_dim, int rank,
+            const int64_t *size, const int64_t *stride, int box_dim, int rows,
+            int dtype) {
+  cuuint64_t dims[4] = {(cuuint64_t)head_dim}, bytes[3];
+  cuuint32_t box[4] = {64, 1, 1, 1}, step[4] = {1, 1, 1, 1};
+  for (int i = 0; i + 1 < rank; ++i) {
+    // a dimension of one element is never stepped along
+    const int64_t s = size[i] == 1 ? head_dim : stride[i];
+    if (size[i] <= 0 || size[i] > (1ll << 31) || s <= 0 ||
+        s >= (1ll << 38))
+      return false;
+    dims[i + 1] = (cuuint64_t)size[i];
+    bytes[i] = (cuuint64_t)s * 2;
+  }
+  box[box_dim] = (cuuint32_t)rows;
+  const EncodeTiled fn = encode_tiled();
+  return fn != nullptr &&
+         fn(m,
+            dtype == CASCADE_KV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+            (cuuint32_t)rank, const_cast<void *>(base), dims, bytes, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+int make_maps(const cascade_attn_args_t &a, const cascade_attn_plan_info_t &p,
+              bool with_v, TileMaps *m) {
+  std::memset(m, 0, sizeof(*m));
+  const int page = p.page_size;
+  if (p.max_cached >= kTile && a.pages > 0 &&
+      (page == 8 || page == 16 || (page > 0 && page % 32 == 0))) {
+    m->box = page < 32 ? page : 32;
+    const int64_t size[3] = {page, p.kv_heads, a.pages};
+    const int64_t ks[3] = {a.kp_tok, a.kp_head, a.kp_page};
+    const int64_t vs[3] = {a.vp_tok, a.vp_head, a.vp_page};
+    m->pages_ok =
+        encode(&m->kp, a.k_pages, p.head_dim, 4, size, ks, 1, m->box,
+               a.dtype) &&
+        (!with_v || encode(&m->vp, a.v_pages, p.head_dim, 4, size, vs, 1,
+                           m->box, a.dtype));
+  }
+  if (p.max_new >= kTile) {
+    const int64_t size[2] = {p.kv_heads, p.tokens};
+    const int64_t ks[2] = {a.k_head, a.k_tok}, vs[2] = {a.v_head, a.v_tok};
+    m->new_ok =
+        encode(&m->k, a.k, p.head_dim, 3, size, ks, 2, 32, a.dtype) &&
+        (!with_v ||
+         encode(&m->v, a.v, p.head_dim, 3, size, vs, 2, 32, a.dtype));
+  }
+  return CASCADE_OK;
 }
 
 namespace {

@@ -55,7 +55,8 @@ static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
 // number.  A chunk's sum is taken by itself before it joins the total.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kWThreads, 1)
-    attn_weights_kernel(const __grid_constant__ WeightArgs a) {
+    attn_weights_kernel(const __grid_constant__ WeightArgs a,
+                        const __grid_constant__ TileMaps maps) {
   constexpr int kTileBytes = kTile * D * 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sm_k = smem_u32(smem);
@@ -243,14 +244,29 @@ __global__ void __launch_bounds__(kWThreads, 1)
           kp = a.kv.k + (int64_t)(sg.tok0 + key - sg.cached) * a.kv.k_tok +
                sg.hk * a.kv.k_head;
         }
+        const int this_page = page[0], off = key % a.kv.page;
+        const int key0 = sg.key0 + tile * kTile;
+        const bool by_page = maps.pages_ok && key0 + kTile <= sg.cached;
+        const bool by_new =
+            maps.new_ok && key0 >= sg.cached && key0 + kTile <= total;
         page[0] = page[1];
         if (tile + 2 < tiles) page[1] = page_at(tile + 2);
         const uint32_t slot = k_no % kKSlots;
         mbar_wait(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1,
                   give_up);
         __syncwarp();
-        copy_rows(sm_k + slot * kTileBytes, kp);
-        cp_async_arrive(smem_u32(&ct.k_full[slot]));
+        const uint32_t bar = smem_u32(&ct.k_full[slot]);
+        const uint32_t dst = sm_k + slot * kTileBytes;
+        if (by_page) {
+          fetch_pages<D>(dst + lw * 32 * 128, maps, &maps.kp, this_page, off,
+                         a.kv.pages, sg.hk, bar, 32);
+        } else if (by_new) {
+          fetch_new<D>(dst + lw * 32 * 128, &maps.k,
+                       sg.tok0 + key0 - sg.cached + lw * 32, sg.hk, bar, 32);
+        } else {
+          copy_rows(dst, kp);
+          cp_async_arrive(bar);
+        }
         ++k_no;
         // the first chunk goes behind the first pair: its slot may still
         // have to be freed, theirs are free already
@@ -335,8 +351,8 @@ __global__ void __launch_bounds__(kKeys)
 }
 
 template <int D, bool kBf16>
-int run_weights(const WeightArgs &a, const cascade_attn_plan_info_t &p,
-                cudaStream_t s) {
+int run_weights(const WeightArgs &a, const TileMaps &maps,
+                const cascade_attn_plan_info_t &p, cudaStream_t s) {
   auto *kernel = attn_weights_kernel<D, kBf16>;
   constexpr int smem = weights_smem<D>();
   static std::atomic<uint64_t> done{0};
@@ -346,7 +362,7 @@ int run_weights(const WeightArgs &a, const cascade_attn_plan_info_t &p,
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     once.set();
   }
-  kernel<<<p.ctas, kWThreads, smem, s>>>(a);
+  kernel<<<p.ctas, kWThreads, smem, s>>>(a, maps);
   count_launches(1);
   CB_CUDA(cudaGetLastError());
   if (p.merges > 0) {
@@ -415,10 +431,12 @@ extern "C" int cascade_attn_weights(const cascade_attn_plan_info_t *plan,
   a.width = args->width;
   a.fill = args->fill;
   a.c = args->scale * kLog2e;
+  TileMaps maps;
+  make_maps(*args, p, false, &maps);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = args->dtype == CASCADE_KV_BF16;
   if (p.head_dim == 128)
-    return bf ? run_weights<128, true>(a, p, s)
-              : run_weights<128, false>(a, p, s);
-  return bf ? run_weights<64, true>(a, p, s) : run_weights<64, false>(a, p, s);
+    return bf ? run_weights<128, true>(a, maps, p, s)
+              : run_weights<128, false>(a, maps, p, s);
+  return bf ? run_weights<64, true>(a, maps, p, s) : run_weights<64, false>(a, maps, p, s);
 }
