@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ct.empty[i]), kDual ? 1 : 2);
     }
     mbar_init(smem_u32(&ct.q_full), 128 + 4);
-    mbar_init(smem_u32(&ct.q_empty), 2);
-    mbar_init(smem_u32(&ct.done), 2);
+    mbar_init(smem_u32(&ct.q_empty), kDual ? 1 : 2);
+    mbar_init(smem_u32(&ct.done), kDual ? 1 : 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&ct.s_full[w]), 1);
       mbar_init(smem_u32(&ct.p_full[w]), 4);
@@ -778,15 +778,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     cp_async_wait_all();
   } else {
     // ------------------------------------------------------------ MMA
-    // One warp for each of the two chains S -> P -> O.  A tcgen05.mma holds
-    // its warp until the tensor pipe takes it, so whatever a warp does
-    // between two of them is time in which only the other warp's MMAs run.
-    // With two row tiles the warps take turns, a step's PV and next QK at a
-    // time: were their MMAs to interleave, both chains would fall into step,
-    // exponentials under exponentials and MMAs under MMAs (16384 tokens:
-    // 5.44 ms against 3.98).
+    // Two row tiles: one warp for each of the two chains S -> P -> O.  A
+    // tcgen05.mma holds its warp until the tensor pipe takes it, so whatever a
+    // warp does between two of them is time in which only the other warp's
+    // MMAs run.  The warps take turns, a step's PV and next QK at a time: MMAs
+    // that interleave slow each other down several times over, and both
+    // chains fall into step, exponentials under exponentials and MMAs under
+    // MMAs (16384 tokens: 5.44 ms against 3.98).
+    //
+    // Two key tiles, where HBM is the bound: one warp issues whatever is
+    // ready next of either chain.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp < 14) {
+    if (warp < (kDual ? 13 : 14)) {
       const int w = uniform(warp - 12);
       const uint32_t issue = lane == 0;
       const uint32_t tm_s = uniform(tmem) + w * 128, tm_o = tm_s + 256;
@@ -795,8 +798,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t ring = uniform(sm_ring);
       constexpr uint32_t id_qk = mma_idesc(kBf16, kTile, false);
       constexpr uint32_t id_pv = mma_idesc(kBf16, D, true);
-      constexpr int kStep = kDual ? 2 : 1;
       uint32_t base = 0, q_phase = 0, p_phase = 0;
+      uint32_t p_phases = 0;               // two key tiles: a bit a chain
+      auto ready = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu,
+                          mbar_test(bar, parity) || *give_up != 0);
+      };
       uint32_t turn_phase = w ^ 1;          // warp 0 has the first turn
       const int seg_last = uniform(seg_end);
       for (int si = uniform(seg_begin); si < seg_last; ++si) {
@@ -805,16 +812,64 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n0 = uniform(kDual ? sp->t1 : sp->n0);
         const int n1 = uniform(kDual ? sp->t1 : sp->n1);
         const int t_all = max(n0, n1), n_end = w ? n1 : n0;
-        const int t_first = kDual ? t0 + w : t0;
+        const int t_first = t0;
+        mbar_wait_warp(smem_u32(&ct.q_full), q_phase, give_up);
+        q_phase ^= 1;
         auto full = [&](uint32_t item) {
           return smem_u32(&ct.full[item % Sh::kSlots]);
         };
         auto phase = [&](uint32_t item) { return (item / Sh::kSlots) & 1; };
+        if constexpr (kDual) {
+          int tq = t0, tp = t0;            // next S and next O product
+          uint64_t since = 0;
+          while (tp < t_all) {
+            bool idle = true;
+            const uint32_t k_item = base + 2 * (tq - t0);
+            const uint32_t v_item = base + 2 * (tp - t0) + 1;
+            // S's buffer is free once the product with its last P is issued
+            if (tq < t_all && tq < tp + 2 &&
+                ready(full(k_item), phase(k_item))) {
+              const int h = (tq - t0) & 1;
+              const uint32_t slot = k_item % Sh::kSlots;
+              fence_async_proxy();
+              tc_fence_after();
+              mma_rows<0, D / 16>(tm_s + h * 128, q,
+                                  tile_desc(ring + slot * Sh::kTileBytes, 0),
+                                  id_qk, issue);
+              tc_commit(smem_u32(&ct.s_full[h]), issue);
+              tc_commit(smem_u32(&ct.empty[slot]), issue);
+              ++tq;
+              idle = false;
+            }
+            const int h = (tp - t0) & 1;
+            if (tp < tq &&
+                ready(smem_u32(&ct.p_full[h]), (p_phases >> h) & 1) &&
+                ready(full(v_item), phase(v_item))) {
+              const uint32_t slot = v_item % Sh::kSlots;
+              fence_async_proxy();
+              tc_fence_after();
+              mma_keys<0, kTile / 16>(
+                  tm_o + h * 128, tm_s + h * 128,
+                  tile_desc(ring + slot * Sh::kTileBytes, kTile * 128), id_pv,
+                  tp >= t0 + 2, issue);
+              tc_commit(smem_u32(&ct.empty[slot]), issue);
+              if (tp + 2 >= t_all) tc_commit(smem_u32(&ct.o_full[h]), issue);
+              p_phases ^= 1u << h;
+              ++tp;
+              idle = false;
+            }
+            if (idle)
+              give_up_after(&since, give_up);
+            else
+              since = 0;
+          }
+          tc_commit(smem_u32(&ct.q_empty), issue);
+          base += 2 * (t_all - t0);
+          continue;
+        }
         auto pass_turn = [&]() {
-          if (!kDual && issue) mbar_arrive(smem_u32(&ct.turn[w ^ 1]));
+          if (issue) mbar_arrive(smem_u32(&ct.turn[w ^ 1]));
         };
-        mbar_wait_warp(smem_u32(&ct.q_full), q_phase, give_up);
-        q_phase ^= 1;
         if (t_first < n_end) {
           const uint32_t item = base + 2 * (t_first - t0);
           const uint32_t slot = item % Sh::kSlots;
@@ -826,8 +881,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(smem_u32(&ct.s_full[w]), issue);
           tc_commit(smem_u32(&ct.empty[slot]), issue);
         }
-        for (int t = t_first; t < t_all; t += kStep) {
-          if (!kDual && t >= n_end) {
+        for (int t = t_first; t < t_all; ++t) {
+          if (t >= n_end) {
             // A tile that only the other row tile needs: give it back, pass
             // the turn on.
             for (int h = 0; h < 2; ++h) {
@@ -842,10 +897,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             continue;
           }
           const uint32_t v_item = base + 2 * (t - t0) + 1;
-          const uint32_t k_item = v_item + 2 * kStep - 1;
+          const uint32_t k_item = v_item + 1;
           const uint32_t slot = v_item % Sh::kSlots;
           const uint32_t k_slot = k_item % Sh::kSlots;
-          const bool more = t + kStep < n_end;
+          const bool more = t + 1 < n_end;
           mbar_wait_warp(full(v_item), phase(v_item), give_up);
           const uint32_t v =
               tile_desc(ring + slot * Sh::kTileBytes, kTile * 128);
@@ -856,10 +911,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_async_proxy();
           mbar_wait_warp(smem_u32(&ct.p_full[w]), p_phase, give_up);
           p_phase ^= 1;
-          if (!kDual) {
-            mbar_wait_warp(smem_u32(&ct.turn[w]), turn_phase, give_up);
-            turn_phase ^= 1;
-          }
+          mbar_wait_warp(smem_u32(&ct.turn[w]), turn_phase, give_up);
+          turn_phase ^= 1;
           tc_fence_after();
           mma_keys<0, kTile / 16>(tm_o, tm_s, v, id_pv, t != t_first, issue);
           if (!k_there) {

@@ -73,6 +73,19 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// The same without being put to sleep for a while: for polling several.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Waits of this source file's kernels that gave up, on this device.
 static __device__ unsigned int g_timeouts;
 
@@ -104,6 +117,20 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity,
                                           volatile int *give_up) {
   if (mbar_try(bar, parity)) return;
   mbar_wait_slow(bar, parity, give_up);
+}
+
+// For a loop that polls: gives up when it has had nothing to do for two
+// seconds (`since` starts at 0 and is set back to 0 by progress).
+__device__ __forceinline__ void give_up_after(uint64_t *since,
+                                              volatile int *give_up) {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  if (*since == 0) *since = t;
+  if (t - *since > 2000000000ull && *give_up == 0) {
+    *give_up = 1;
+    if ((threadIdx.x & 31) == 0) atomicAdd(&g_timeouts, 1u);
+  }
+  __syncwarp();
 }
 
 // The same for a whole warp, which stays converged.
