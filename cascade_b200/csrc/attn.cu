@@ -718,9 +718,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int total = sg.cached + sg.n_new;
       auto page_at = [&](int t) {        // the page of this lane's key
         const int key = t * kTile + lw * 32 + lane;
-        return key < sg.cached ? page_of(a.kv, sg.b, key) : -1;
+        return key < sg.cached ? table_entry(a.kv, sg.b, key) : -1;
       };
-      int page = page_at(sg.t0);
+      int entry = page_at(sg.t0);
       for (int t = sg.t0; t < t_all; ++t) {
         // Q goes behind a tile or two of its segment: it has to wait until
         // the segment before is through with its own, they do not.
@@ -728,6 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   : min(sg.t0 + Sh::kAhead, t_all - 1)))
           load_q(sg);
         const int key = t * kTile + lw * 32 + lane;
+        const int page = page_named(a.kv, entry);
         const char *kp = nullptr, *vp = nullptr;
         if (key < sg.cached) {
           if (page >= 0) {
@@ -742,8 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           kp = a.kv.k + n * a.kv.k_tok + sg.hk * a.kv.k_head;
           vp = a.kv.v + n * a.kv.v_tok + sg.hk * a.kv.v_head;
         }
-        const int this_page = page;
-        if (t + 1 < t_all) page = page_at(t + 1);
+        if (t + 1 < t_all) entry = page_at(t + 1);
         const uint32_t there = __ballot_sync(0xffffffffu, kp != nullptr);
         // Tiles of one kind that every row sees whole go by TMA.
         const bool by_page = maps.pages_ok && (t + 1) * kTile <= sg.cached;
@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (h == 0 && lane == 0) ct.valid[tile_no & 7][lw] = there;
           if (by_page) {
             fetch_pages<D>(dst + lw * 32 * 128, maps, h ? &maps.vp : &maps.kp,
-                           this_page, off, a.kv.pages, sg.hk, bar, 33);
+                           page, off, a.kv.pages, sg.hk, bar, 33);
           } else if (by_new) {
             fetch_new<D>(dst + lw * 32 * 128, h ? &maps.v : &maps.k, tok,
                          sg.hk, bar, 33);

@@ -311,6 +311,13 @@ __device__ __forceinline__ void tc_st16(uint32_t addr,
       CB_I8(x, 8), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tc_ld8(uint32_t (&x)[8], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : CB_R8(x, 0)
+      : "r"(addr));
+}
 __device__ __forceinline__ void tc_ld16(uint32_t (&x)[16], uint32_t addr) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -330,6 +337,9 @@ __device__ __forceinline__ void tc_hold(uint32_t (&x)[32]) {
   asm volatile("" : CB_K8(x, 0), CB_K8(x, 8), CB_K8(x, 16), CB_K8(x, 24));
 }
 
+__device__ __forceinline__ void tc_hold(uint32_t (&x)[8]) {
+  asm volatile("" : CB_K8(x, 0));
+}
 __device__ __forceinline__ void tc_hold(uint32_t (&x)[16]) {
   asm volatile("" : CB_K8(x, 0), CB_K8(x, 8));
 }
@@ -531,10 +541,18 @@ __device__ __forceinline__ void fetch_new(uint32_t dst, const CUtensorMap *map,
     tma_rows3(dst + lane * (kTile * 128), map, lane * 64, hk, tok, bar);
 }
 
-// Page of cached token `key` of sequence b, or -1 when the table names none.
-__device__ __forceinline__ int page_of(const KvSource &s, int b, int key) {
-  const int id = __ldg(s.table + (int64_t)b * s.table_row + key / s.page);
+// The table's entry for cached token `key` of sequence b, and the page that
+// it names (-1: none).  Apart, so that an entry can be on its way while other
+// work is done: it is waited for where it is first looked at.
+__device__ __forceinline__ int table_entry(const KvSource &s, int b,
+                                           int key) {
+  return __ldg(s.table + (int64_t)b * s.table_row + key / s.page);
+}
+__device__ __forceinline__ int page_named(const KvSource &s, int id) {
   return id >= 0 && id < s.pages ? id : -1;
+}
+__device__ __forceinline__ int page_of(const KvSource &s, int b, int key) {
+  return page_named(s, table_entry(s, b, key));
 }
 
 }  // namespace attn

@@ -115,8 +115,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
       float *out = a.out + sg.b * a.o_seq + hk * a.o_head;
       for (int pair = 0; pair < sg.n0; ++pair) {
         const int key = sg.key0 + pair * kKeys + kt;
-        bool there = key < total;
-        if (there && key < sg.cached) there = page_of(a.kv, sg.b, key) >= 0;
+        // on their way while the scores are waited for
+        const int entry =
+            key < sg.cached ? table_entry(a.kv, sg.b, key) : 0;
         float prev = 0.f;
         if (key < total && before != nullptr) prev = before[key];
         // rows from `from` on see this key
@@ -133,24 +134,45 @@ __global__ void __launch_bounds__(kWThreads, 1)
           const int64_t hidden = from - (int64_t)ch * kTile;
           const bool whole = __all_sync(0xffffffffu, hidden <= 0);
           float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+          const uint32_t src = tm + buf * 128;
+          if (whole && n == kTile) {
+            // kept short: its code and that of the other warps has to stay
+            // in the instruction cache
 #pragma unroll 1
-          for (int i = 0; i < n; i += 32) {
-            uint32_t x[32];
-            tc_ld32(x, tm + buf * 128 + i);
-            tc_wait_ld();
-            tc_hold(x);
-            if (!whole || i + 32 > n) {
+            for (int i = 0; i < kTile; i += 32) {
+              uint32_t x[32];
+              tc_ld32(x, src + i);
+              tc_wait_ld();
+              tc_hold(x);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;  // -inf
+              for (int e = 0; e < 8; ++e) {
+                const float4 l = l4[i / 4 + e];
+                s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
+                s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
+                s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
+                s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
+              }
             }
+          } else {
+            // few rows, or rows that do not see the key: -inf for those
+            // (the scores of rows that are not there may be anything)
+#pragma unroll 1
+            for (int i = 0; i < n; i += 8) {
+              uint32_t x[8];
+              tc_ld8(x, src + i);
+              tc_wait_ld();
+              tc_hold(x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 l = l4[i / 4 + e];
-              s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
-              s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
-              s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
-              s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
+              for (int e = 0; e < 8; ++e)
+                if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float4 l = l4[i / 4 + e];
+                s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
+                s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
+                s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
+                s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
+              }
             }
           }
           tc_fence_before();
@@ -161,7 +183,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
           }
           sum += (s0 + s1) + (s2 + s3);
         }
-        if (!there) sum = 0.f;
+        if (key >= total ||
+            (key < sg.cached && page_named(a.kv, entry) < 0))
+          sum = 0.f;
         if (sg.part >= 0)
           a.part[(int64_t)sg.part * kKeys + kt] = sum;
         else if (key < total)
@@ -228,29 +252,30 @@ __global__ void __launch_bounds__(kWThreads, 1)
       const int total = sg.cached + sg.n_new;
       auto page_at = [&](int tile) {
         const int key = sg.key0 + tile * kTile + lw * 32 + lane;
-        return key < sg.cached ? page_of(a.kv, sg.b, key) : -1;
+        return key < sg.cached ? table_entry(a.kv, sg.b, key) : -1;
       };
       const int tiles = 2 * sg.n0;
-      // pages of the next two tiles are looked up ahead
-      int page[2] = {page_at(0), page_at(1)};
+      // the table is read two tiles ahead
+      int entry[2] = {page_at(0), page_at(1)};
       for (int tile = 0; tile < tiles; ++tile) {
         const int key = sg.key0 + tile * kTile + lw * 32 + lane;
+        const int page = page_named(a.kv, entry[0]);
         const char *kp = nullptr;
         if (key < sg.cached) {
-          if (page[0] >= 0)
-            kp = a.kv.kp + page[0] * a.kv.kp_page + sg.hk * a.kv.kp_head +
+          if (page >= 0)
+            kp = a.kv.kp + page * a.kv.kp_page + sg.hk * a.kv.kp_head +
                  (key % a.kv.page) * a.kv.kp_tok;
         } else if (key < total) {
           kp = a.kv.k + (int64_t)(sg.tok0 + key - sg.cached) * a.kv.k_tok +
                sg.hk * a.kv.k_head;
         }
-        const int this_page = page[0], off = key % a.kv.page;
+        const int off = key % a.kv.page;
         const int key0 = sg.key0 + tile * kTile;
         const bool by_page = maps.pages_ok && key0 + kTile <= sg.cached;
         const bool by_new =
             maps.new_ok && key0 >= sg.cached && key0 + kTile <= total;
-        page[0] = page[1];
-        if (tile + 2 < tiles) page[1] = page_at(tile + 2);
+        entry[0] = entry[1];
+        if (tile + 2 < tiles) entry[1] = page_at(tile + 2);
         const uint32_t slot = k_no % kKSlots;
         mbar_wait(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1,
                   give_up);
@@ -258,7 +283,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         const uint32_t bar = smem_u32(&ct.k_full[slot]);
         const uint32_t dst = sm_k + slot * kTileBytes;
         if (by_page) {
-          fetch_pages<D>(dst + lw * 32 * 128, maps, &maps.kp, this_page, off,
+          fetch_pages<D>(dst + lw * 32 * 128, maps, &maps.kp, page, off,
                          a.kv.pages, sg.hk, bar, 32);
         } else if (by_new) {
           fetch_new<D>(dst + lw * 32 * 128, &maps.k,
