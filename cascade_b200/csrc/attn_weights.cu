@@ -6,7 +6,7 @@ namespace cb {
 namespace attn {
 namespace {
 
-constexpr int kWThreads = 416;     // 2 x 4 summing warps, 4 loaders, MMA
+constexpr int kWThreads = 672;     // 4 x 4 summing warps, 4 loaders, MMA
 constexpr int kKeys = 2 * kTile;   // keys of an item
 constexpr int kKSlots = 4, kQSlots = 3;   // tiles of 128 keys, of 128 rows
 
@@ -27,7 +27,9 @@ struct WeightArgs {
 };
 
 struct WControl {
-  alignas(16) float lse2[kQSlots][kTile];      // lse of a chunk's rows, in powers of two
+  // lse of a chunk's rows, in powers of two
+  alignas(16) float lse2[kQSlots][kTile];
+  float other[kKeys];              // sums of the odd chunks
   uint64_t k_full[kKSlots], k_empty[kKSlots];
   uint64_t q_full[kQSlots], q_empty[kQSlots];
   uint64_t s_full[2][2], s_empty[2][2];
@@ -47,7 +49,7 @@ static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
 // K Q^T, with 128 keys as the rows of a tcgen05 tile: a thread owns one key
 // and adds along its own row, so the sum over the rows of all heads of a
 // group needs no reduction across threads and no atomics, and its order is
-// fixed.  Two warpgroups take 128 keys each (a pair).  With many query rows
+// fixed.  A pair of tiles of 128 keys is worked on at a time.  With many query rows
 // a segment is one pair that stays resident while chunks of 128 rows stream
 // by; with up to 128 rows (a decode step, a short window) it is a run of
 // pairs that stream by one resident chunk of N = 32, 64, ... columns.  Key j
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
     }
     for (int i = 0; i < kQSlots; ++i) {
       mbar_init(smem_u32(&ct.q_full[i]), 128 + 4);
-      mbar_init(smem_u32(&ct.q_empty[i]), 9);   // the MMAs and 8 warps
+      mbar_init(smem_u32(&ct.q_empty[i]), 17);  // the MMAs and 16 warps
     }
     for (int w = 0; w < 2; ++w)
       for (int i = 0; i < 2; ++i) {
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
     ct.give_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) tc_alloc(smem_u32(&ct.tmem), 512);
+  if (warp == 20) tc_alloc(smem_u32(&ct.tmem), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -99,9 +101,11 @@ __global__ void __launch_bounds__(kWThreads, 1)
       reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
   const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ---------------------------------------------------------- sums
-    const int w = warp >> 2;
+    // Two warpgroups for each 128 keys take chunks (or pairs) in turn.
+    const int w = (warp >> 2) & 1;
+    const uint32_t buf = warp >> 3;
     const int kt = w * kTile + (warp & 3) * 32 + lane;   // key of the item
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
     uint32_t step = 0, q_no = 0;
@@ -114,6 +118,11 @@ __global__ void __launch_bounds__(kWThreads, 1)
                               : nullptr;
       float *out = a.out + sg.b * a.o_seq + hk * a.o_head;
       for (int pair = 0; pair < sg.n0; ++pair) {
+        // runs of pairs: each is one step, and one warpgroup's of two
+        if (sg.n0 > 1 && (sg.t1 > sg.t0 ? step & 1 : 0) != buf) {
+          step += sg.t1 - sg.t0;
+          continue;
+        }
         const int key = sg.key0 + pair * kKeys + kt;
         // on their way while the scores are waited for
         const int entry =
@@ -125,7 +134,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             (int64_t)(key - sg.cached - sg.row0) * a.group;
         float sum = 0.f;
         for (int ch = sg.t0; ch < sg.t1; ++ch, ++step) {
-          const uint32_t buf = step & 1;
+          if ((step & 1) != buf) continue;
           const uint32_t slot = (q_no + ch - sg.t0) % kQSlots;
           const int n = min(kTile, sg.rows - ch * kTile);
           mbar_wait(smem_u32(&ct.s_full[w][buf]), (step >> 1) & 1, give_up);
@@ -179,9 +188,21 @@ __global__ void __launch_bounds__(kWThreads, 1)
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(smem_u32(&ct.s_empty[w][buf]));
-            if (pair + 1 == sg.n0) mbar_arrive(smem_u32(&ct.q_empty[slot]));
+            // the chunk is done with after this warpgroup's last pair
+            if (sg.n0 == 1)
+              mbar_arrive_n(smem_u32(&ct.q_empty[slot]), 2);
+            else if (pair + 2 >= sg.n0)
+              mbar_arrive(smem_u32(&ct.q_empty[slot]));
           }
           sum += (s0 + s1) + (s2 + s3);
+        }
+        if (sg.n0 == 1) {
+          // one pair: its odd and even chunks are joined
+          if (buf) ct.other[kt] = sum;
+          asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory");
+          if (!buf) sum += ct.other[kt];
+          asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory");
+          if (buf) continue;
         }
         if (key >= total ||
             (key < sg.cached && page_named(a.kv, entry) < 0))
@@ -192,15 +213,15 @@ __global__ void __launch_bounds__(kWThreads, 1)
           out[key] = prev + sum;
       }
       q_no += sg.t1 - sg.t0;
-      if (sg.fill && a.fill)
+      if (sg.fill && a.fill && buf == 0)
         for (int k = total + kt; k < a.width; k += kKeys)
           out[k] = before != nullptr ? before[k] : 0.f;
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------- loaders
     constexpr int kChunks = D / 8;
     constexpr int kRowsPer = 32 / kChunks;
-    const int lw = warp - 8;
+    const int lw = warp - 16;
     const int chunk = lane % kChunks, sub_row = lane / kChunks;
     uint32_t k_no = 0, q_no = 0;
     auto place = [&](int row) {
@@ -352,7 +373,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     tc_dealloc(tmem, 512);
   }
