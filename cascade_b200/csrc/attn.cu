@@ -559,29 +559,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         char *orow = a.out + (int64_t)(sg.tok0 + tok) * a.o_tok +
                      (int64_t)head * a.o_head;
 #pragma unroll 1
-        for (int cb0 = 0; cb0 < kCols; cb0 += 32) {
-          const int col = c_base + cb0;
-          float o[32];
+        for (int col = c_base; col < c_base + kCols; col += 16) {
+          float o[16];
+          uint32_t u[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = fill;
-          uint32_t u[32];
+          for (int e = 0; e < 16; ++e) o[e] = fill;
           if (steps) {
-            tc_ld32(u, tm_o + col);
+            tc_ld16(u, tm_o + col);
             tc_wait_ld();
             tc_hold(u);
             if (f1 != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+              for (int e = 0; e < 16; ++e)
                 o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
             }
           }
           if (kDual && steps2) {
-            tc_ld32(u, lane_base + 256 + (w ^ 1) * 128 + col);
+            tc_ld16(u, lane_base + 256 + (w ^ 1) * 128 + col);
             tc_wait_ld();
             tc_hold(u);
             if (f2 != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+              for (int e = 0; e < 16; ++e)
                 o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
             }
           }
@@ -593,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (sg.part >= 0) {
               float *dst = a.part_o + prow * D + col;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
+              for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   v[e] = __float_as_uint(o[8 * i + e]);
@@ -601,13 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  v[e] = pack16<kBf16>(o[16 * i + 2 * e],
-                                       o[16 * i + 2 * e + 1]);
-                store32(orow + col * 2 + 32 * i, v, a.out32);
-              }
+              for (int e = 0; e < 8; ++e)
+                v[e] = pack16<kBf16>(o[2 * e], o[2 * e + 1]);
+              store32(orow + col * 2, v, a.out32);
             }
           }
         }

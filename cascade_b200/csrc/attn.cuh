@@ -91,26 +91,18 @@ static __device__ unsigned int g_timeouts;
 
 // A wait on another role of the same CTA.  Every role's loops are finite and
 // no address depends on data that a wait guards, so a wait that runs out
-// (two seconds) sets the CTA's flag, lets every later wait of the CTA
-// through, and the kernel ends by itself.
-__device__ __forceinline__ void mbar_wait_slow(uint32_t bar,
-                                                   uint32_t parity,
-                                                   volatile int *give_up) {
-  uint64_t t0 = 0;
-  for (uint32_t n = 1;; ++n) {
+// (four million tries, each of which may sleep; seconds in all) sets the
+// CTA's flag, lets every later wait of the CTA through, and the kernel ends
+// by itself.  Kept short: it is inlined at every wait.
+__device__ __forceinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity,
+                                               volatile int *give_up) {
+#pragma unroll 1
+  for (uint32_t n = 1; n < (1u << 22); ++n) {
     if (mbar_try(bar, parity)) return;
-    if ((n & 63) == 0) {
-      if (*give_up) return;
-      uint64_t t;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t0 == 0) t0 = t;
-      if (t - t0 > 2000000000ull) {
-        *give_up = 1;
-        atomicAdd(&g_timeouts, 1u);
-        return;
-      }
-    }
+    if ((n & 255) == 0 && *give_up) return;
   }
+  if (*give_up == 0) atomicAdd(&g_timeouts, 1u);
+  *give_up = 1;
 }
 
 __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity,

@@ -160,31 +160,66 @@ struct Costs {
 };
 
 constexpr double kBytesPerNs = 6200;       // HBM, all SMs together
+constexpr double kPartBytesPerNs = 35;     // partial results, one SM
 
-std::vector<std::vector<Segment>> whole_items(const std::vector<Item> &items,
-                                              int ctas, const Costs &c,
-                                              double *makespan) {
-  std::vector<int> order(items.size());
+Merge merge_of(const Segment &s, bool fwd, int part0, int parts) {
+  Merge m{};
+  m.tok0 = s.tok0;
+  m.hk = s.hk;
+  m.row0 = s.row0;
+  m.rows = fwd ? s.rows : s.n_new + s.cached;
+  m.part0 = part0;
+  m.parts = parts;
+  m.b = s.b;
+  m.key0 = s.key0;
+  return m;
+}
+
+// Items longer than `cap` units are cut into equal pieces; the pieces go, the
+// longest first, each to the CTA with the least to do.
+std::vector<std::vector<Segment>> cut_items(const std::vector<Item> &items,
+                                            int ctas, int cap, bool fwd,
+                                            const Costs &c,
+                                            std::vector<Merge> *merges,
+                                            int *parts, double *makespan) {
+  std::vector<Segment> pieces;
+  pieces.reserve(items.size());
+  for (const Item &it : items) {
+    const int n = std::max(1, (int)div_up(it.units(), cap));
+    if (n > 1) merges->push_back(merge_of(it.seg, fwd, *parts, n));
+    for (int k = 0; k < n; ++k) {
+      Segment s = it.seg;
+      s.t0 = it.seg.t0 + (int)((int64_t)it.units() * k / n);
+      s.t1 = it.seg.t0 + (int)((int64_t)it.units() * (k + 1) / n);
+      if (n > 1) s.part = (*parts)++;
+      pieces.push_back(s);
+    }
+  }
+  std::vector<int> order(pieces.size());
   for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
-    return items[x].units() > items[y].units();
+    return pieces[x].t1 - pieces[x].t0 > pieces[y].t1 - pieces[y].t0;
   });
-  ctas = (int)std::min<size_t>(ctas, items.size());
+  ctas = (int)std::min<size_t>(ctas, pieces.size());
   std::vector<std::vector<Segment>> out(ctas);
   using Load = std::pair<double, int>;
   std::priority_queue<Load, std::vector<Load>, std::greater<Load>> heap;
   for (int i = 0; i < ctas; ++i) heap.push({0.0, i});
-  const double unit =
-      std::max(c.unit, c.unit_bytes * ctas / kBytesPerNs);
-  *makespan = 0;
+  const double unit = std::max(c.unit, c.unit_bytes * ctas / kBytesPerNs);
+  double longest = 0;
   for (int i : order) {
     Load l = heap.top();
     heap.pop();
-    l.first += items[i].units() * unit + c.segment;
-    *makespan = std::max(*makespan, l.first);
-    out[l.second].push_back(items[i].seg);
+    const Segment &s = pieces[i];
+    l.first += (s.t1 - s.t0) * unit + c.segment +
+               (s.part >= 0 ? c.part_bytes / 2 / kPartBytesPerNs : 0);
+    longest = std::max(longest, l.first);
+    out[l.second].push_back(s);
     heap.push(l);
   }
+  *makespan = longest + (*parts ? c.merge + *parts * c.part_bytes / 2 /
+                                                4000.0
+                                : 0);
   return out;
 }
 
@@ -224,16 +259,7 @@ std::vector<std::vector<Segment>> equal_runs(const std::vector<Item> &items,
       if (done < units) ++cta;
     } while (done < units);
     if (pieces.size() > 1) {
-      Merge m{};
-      m.tok0 = it.seg.tok0;
-      m.hk = it.seg.hk;
-      m.row0 = it.seg.row0;
-      m.rows = fwd ? it.seg.rows : it.seg.n_new + it.seg.cached;
-      m.part0 = *parts;
-      m.parts = (int)pieces.size();
-      m.b = it.seg.b;
-      m.key0 = it.seg.key0;
-      merges->push_back(m);
+      merges->push_back(merge_of(it.seg, fwd, *parts, (int)pieces.size()));
       for (const auto &at : pieces) out[at.first][at.second].part = (*parts)++;
     }
     pos += units + ov;
@@ -358,9 +384,9 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
   Costs cost{};
   const double tile_bytes = 2.0 * kTile * p.head_dim;
   if (fwd) {
-    cost.unit = row_tile == kTile ? 600 : 1400;
+    cost.unit = row_tile == kTile ? 700 : 2200;
     cost.unit_bytes = row_tile == kTile ? 2 * tile_bytes : 0;
-    cost.segment = 1500;
+    cost.segment = row_tile == kTile ? 2500 : 5000;
     cost.part_bytes = 8.0 * (p.head_dim + 1) *
                       std::min<int64_t>(row_tile, (int64_t)max_new * group);
   } else {
@@ -376,16 +402,37 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
   std::vector<Merge> merges;
   int parts = 0;
   if (!items.empty()) {
-    double t_best;
-    best = whole_items(items, sms, cost, &t_best);
-    double units = 0;
+    int64_t units = 0;
     int most = 0;
     for (const Item &it : items) {
       units += it.units();
       most = std::max(most, it.units());
     }
-    // Runs of equal length over n CTAs; worth it where whole items leave
-    // SMs idle, and splitting needs something to split.
+    // Whole items, or items cut to a length between the longest's and an
+    // equal share's.
+    double t_best = 0;
+    const int share = (int)std::max<int64_t>(1, units / sms);
+    int caps[6] = {std::max(most, 1)}, n_caps = 1;
+    if (!by_keys)
+      for (int k = 1; k <= 4; ++k) {
+        const int cap = std::max(1, share * (k + 3) / 4);
+        if (cap < most) caps[n_caps++] = cap;
+      }
+    for (int k = 0; k < n_caps; ++k) {
+      std::vector<Merge> m;
+      int n_parts = 0;
+      double t;
+      auto plan = cut_items(items, sms, caps[k], fwd, cost, &m, &n_parts, &t);
+      if (k == 0 || t < t_best * 0.97) {
+        t_best = t;
+        best.swap(plan);
+        merges.swap(m);
+        parts = n_parts;
+      }
+      if (items.size() > 20000) break;      // many items balance by themselves
+    }
+    // Runs of equal length over n CTAs: where the items are many and HBM is
+    // the bound, each CTA then cuts two items at most.
     int n_best = 0;
     if (most > 1) {
       for (int n = sms; n >= 2; n = n * 3 / 4) {
@@ -394,14 +441,19 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
             std::max(cost.unit, cost.unit_bytes * n / kBytesPerNs);
         const double t = (units * unit + items.size() * cost.segment) / n +
                          cost.segment + cost.merge +
-                         2.0 * n * cost.part_bytes / 4000.0;
+                         cost.part_bytes / kPartBytesPerNs +
+                         n * cost.part_bytes / 4000.0;
         if (t < t_best * 0.97) {
           t_best = t;
           n_best = n;
         }
       }
     }
-    if (n_best) best = equal_runs(items, n_best, cost, fwd, &merges, &parts);
+    if (n_best) {
+      merges.clear();
+      parts = 0;
+      best = equal_runs(items, n_best, cost, fwd, &merges, &parts);
+    }
     if (by_keys) {
       merges.clear();
       parts = 0;
