@@ -833,7 +833,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   id_qk, issue);
               tc_commit(smem_u32(&ct.s_full[h]), issue);
               tc_commit(smem_u32(&ct.empty[slot]), issue);
-              ++tq;
+              // Q is free for the next segment's from here on
+              if (++tq == t_all) tc_commit(smem_u32(&ct.q_empty), issue);
               idle = false;
             }
             const int h = (tp - t0) & 1;
@@ -858,7 +859,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             else
               since = 0;
           }
-          tc_commit(smem_u32(&ct.q_empty), issue);
           base += 2 * (t_all - t0);
           continue;
         }
@@ -876,6 +876,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(smem_u32(&ct.s_full[w]), issue);
           tc_commit(smem_u32(&ct.empty[slot]), issue);
         }
+        // Q is free for the next segment's once the last product with it is
+        // done, long before this segment is
+        if (t_first + 1 >= n_end) tc_commit(smem_u32(&ct.q_empty), issue);
         for (int t = t_first; t < t_all; ++t) {
           if (t >= n_end) {
             // A tile that only the other row tile needs: give it back, pass
@@ -925,8 +928,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_commit(smem_u32(&ct.s_full[w]), issue);
           tc_commit(smem_u32(&ct.empty[k_slot]), issue);
+          if (t + 2 == n_end) tc_commit(smem_u32(&ct.q_empty), issue);
         }
-        tc_commit(smem_u32(&ct.q_empty), issue);
         base += 2 * (t_all - t0);
       }
       // TMEM is freed only when no MMA is in flight.
