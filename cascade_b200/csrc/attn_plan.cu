@@ -21,8 +21,9 @@ int check_args(const cascade_attn_plan_info_t &p,
                ((uintptr_t)a.workspace & 31) == 0,
            CASCADE_ERR_INVALID,
            "the plan must be 16-byte, the workspace 32-byte aligned");
-  CB_CHECK(std::isfinite(a.scale) && a.scale > 0.f, CASCADE_ERR_INVALID,
-           "scale must be finite and above 0");
+  // (the kernels work with scale log2(e) and 8 / that)
+  CB_CHECK(a.scale >= 0x1p-64f && a.scale <= 0x1p64f, CASCADE_ERR_INVALID,
+           "scale must be in [2^-64, 2^64]");
   uint64_t bits = (uintptr_t)a.q | (uintptr_t)a.k;
   int64_t strides = a.q_tok | a.q_head | a.k_tok | a.k_head;
   if (forward) {
@@ -316,7 +317,7 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
              (fwd ? (int64_t)div_up((uint64_t)n_new[b] * group, row_tile)
                   : std::max<int64_t>(1, (int64_t)div_up(keys, row_tile)));
   }
-  CB_CHECK(count <= (1 << 24), CASCADE_ERR_INVALID,
+  CB_CHECK(count <= (1 << 22), CASCADE_ERR_INVALID,
            "the batch is too large for one call");
   items.reserve(count);
   for (int b = 0; b < p.batch; ++b) {

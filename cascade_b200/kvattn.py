@@ -21,7 +21,8 @@ kv_heads).  Tensors are float16 or bfloat16, head_dim 64 or 128 and
 contiguous; other strides may be anything whose rows start on 16-byte
 boundaries (a slice of a fused projection, a [1, heads, seq, dim] cache
 permuted to [seq, heads, dim]).  Rows of `out` that belong to no sequence are
-left as they were.  There are no backward passes: tensors that require a
+left as they were.  A value of V that is not finite leaves the rows that see
+it not finite, and the rows that do not see it alone.  There are no backward passes: tensors that require a
 gradient are refused while gradients are enabled.
 
 Work is enqueued on the current stream of the tensors' device.  A plan may be
@@ -32,7 +33,6 @@ that overlap share nothing.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 
 from . import _lib, kvwire
@@ -221,9 +221,8 @@ def _writable(name, t):
 def _scale(scale, dim):
     if scale is None:
         return dim ** -0.5
-    if not (math.isfinite(scale) and scale > 0.0
-            and 0.0 < ctypes.c_float(scale).value < math.inf):
-        raise ValueError("scale must be finite and above 0")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        raise ValueError("scale must be in [2**-64, 2**64]")
     return scale
 
 

@@ -197,7 +197,7 @@ int cascade_attn_plan(cascade_attn_plan_info_t *info,
 typedef struct {
   int32_t dtype;       /* CASCADE_KV_FP16 or CASCADE_KV_BF16 */
   int32_t pages;       /* pages there are */
-  float scale;         /* of the scores, > 0 */
+  float scale;         /* of the scores, in [2^-64, 2^64] */
   int32_t add;         /* weights: add to `before` */
   const int32_t *plan; /* device copy of the plan buffer */
   const void *q, *k, *v;
@@ -228,7 +228,8 @@ typedef struct {
 /* softmax(scale q k^T) v per query head, over every cached token and, of
  * the new tokens of its own sequence, those up to itself (or, with a plan
  * for trees, those its mask row names).  A row that sees nothing is 0 with
- * lse -inf. */
+ * lse -inf.  A value of v that is not finite leaves the rows
+ * that see it not finite, and others alone. */
 int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
                          const cascade_attn_args_t *args, void *stream);
 

@@ -235,7 +235,7 @@ def test_launches_refuse_bad_arguments():
     assert call(L.cascade_attn_forward, info, args) == 1       # alignment
     assert b"16-byte" in L.cascade_last_error()
     args.q_tok = 8
-    for bad in (0.0, -1.0, float("inf"), float("nan")):
+    for bad in (0.0, -1.0, 1e-30, 1e30, float("inf"), float("nan")):
         args.scale = bad
         assert call(L.cascade_attn_forward, info, args) == 1
         assert b"scale" in L.cascade_last_error()

@@ -177,6 +177,34 @@ def test_forward(shape, dtype, tree):
     assert kvattn.wait_timeouts() == 0
 
 
+FORMS = [  # rows: up to 16, up to 128, more; each with parts and merges too
+    ([1, 1, 1], 4, 1), ([2, 1], 16, 2), ([3], 5, 1),
+    ([9, 4], 4, 1), ([16, 1], 8, 1), ([64, 20], 2, 1),
+    ([65, 300], 2, 1), ([40, 129], 8, 2)]
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 96, 128, 512])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_forms_and_page_sizes(form, dim, page):
+    # page sizes that whole tiles are fetched in, some pages gone, and pages
+    # laid out [page, token, head, dim]
+    new, H, G = FORMS[form]
+    cached = [1300, 127, 5000][:len(new)]
+    c = Case(new, cached, H, G, dim, "bf16", page, form % 2 == 1,
+             seed=form + page)
+    c.table[0, c.table.shape[1] // 3] = -1
+    check_forward(c, *c.run())
+    other = c.pool.transpose(2, 3).contiguous().transpose(2, 3)
+    assert other.stride() != c.pool.stride() or page == 1 or G == 1
+    before = c.run()
+    c.pool = other
+    after = c.run()
+    assert torch.equal(before[0], after[0])
+    assert torch.equal(before[1], after[1])
+    assert kvattn.wait_timeouts() == 0
+
+
 @pytest.mark.parametrize("scale", [0.01, 0.5])
 def test_scale(scale):
     c = Case([40, 3], [200, 90], 4, 2, 128, "fp16", scale=scale, seed=3)
@@ -272,9 +300,11 @@ def test_masked_infinities_of_a_tree():
     assert (out[3, :, ::3] == math.inf).all()
 
 
-def test_all_scores_minus_infinity_is_nan():
+@pytest.mark.parametrize("heads", [2, 32, 128])
+@pytest.mark.parametrize("cached", [40, 3000])
+def test_all_scores_minus_infinity_is_nan(heads, cached):
     # keys are seen, but no score is above -inf: 0 / 0, not an empty row
-    c = Case([2], [40], 2, 1, 64, "bf16", seed=10)
+    c = Case([2], [cached], heads, 1, 64, "bf16", seed=10)
     c.q = torch.full_like(c.q, 1.0)
     c.k = torch.full_like(c.k, -math.inf)
     c.pool[:, 0] = -math.inf
@@ -282,8 +312,9 @@ def test_all_scores_minus_infinity_is_nan():
     assert out.isnan().all()
 
 
-def test_scores_of_minus_infinity_weigh_nothing():
-    c = Case([1], [600], 2, 1, 64, "bf16", seed=10)
+@pytest.mark.parametrize("heads", [2, 32, 256])
+def test_scores_of_minus_infinity_weigh_nothing(heads):
+    c = Case([1], [600], heads, 1, 64, "bf16", seed=10)
     c.q = torch.full_like(c.q, 1.0)
     clean = c.run()
     ids = c.table[0].long()
@@ -317,6 +348,27 @@ def test_layouts_and_untouched_rows():
     assert torch.equal(o[:n], want) and torch.equal(l[:n], want_lse)
     assert (out[:, n:] == 7).all() and (out[:, :, 64:] == 7).all()
     assert (lse[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("heads", [2, 32, 256])
+def test_infinities_in_cached_values_stay_with_their_rows(heads):
+    c = Case([1, 1], [700, 300], heads, 1, 64, "fp16", seed=16)
+    clean = c.run()
+    page = int(c.table[0, 20])
+    c.pool[page, 1, 0, 3, ::5] = math.inf
+    out, lse = c.run()
+    assert torch.equal(lse, clean[1]) and torch.equal(out[1], clean[0][1])
+    assert not out[0, :, ::5].isfinite().any()
+    rest = torch.arange(64, device=DEV) % 5 != 0
+    assert torch.equal(out[0, :, rest], clean[0][0, :, rest])
+
+
+def test_one_vector_for_all_tokens():
+    # K and V expanded along the tokens (stride 0): no tensor map for those
+    c = Case([300], [0], 4, 2, 64, "bf16", seed=17)
+    c.k = c.k[:1].expand(300, 2, 64)
+    c.v = c.v[:1].expand(300, 2, 64)
+    check_forward(c, *c.run())
 
 
 def test_contiguous_cache_as_one_page_each():
@@ -406,7 +458,7 @@ def test_refusals():
                 dict(table=c.table.cpu()), dict(pages=(c.pages[0], None)),
                 dict(pages=(c.pages[0], c.pages[1][:, :, :8])),
                 dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
-                dict(scale=math.inf),
+                dict(scale=math.inf), dict(scale=1e-30), dict(scale=1e30),
                 dict(out=torch.empty(6, 4, 64, device=DEV)),
                 dict(out=torch.empty(1, 4, 64, dtype=c.dt, device=DEV)
                      .expand(6, 4, 64)),
