@@ -397,7 +397,9 @@ int make_plan(cascade_attn_plan_info_t *info, const int32_t *n_new,
     cost.segment = by_keys ? 500 : 1500;
     cost.part_bytes = by_keys ? 0 : 8.0 * row_tile;
   }
-  cost.merge = by_keys ? 0 : 3500;        // runs of keys need no merge
+  // a second launch, of which the host's share is the larger; runs of keys
+  // need no merge
+  cost.merge = by_keys ? 0 : 6000;
 
   std::vector<std::vector<Segment>> best;
   std::vector<Merge> merges;

@@ -56,13 +56,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512   ? 3
   __shared__ uint32_t cta_sum[2];
   __shared__ uint32_t cta_total[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t row = blockIdx.x / ranks;
-  const int i2 = (int)(row % a.dim2);
-  const int i1 = (int)(row / a.dim2 % a.dim1);
-  const int i0 = (int)(row / a.dim2 / a.dim1);
+  const uint32_t row = blockIdx.x / (uint32_t)ranks;
+  const uint32_t i01 = row / (uint32_t)a.dim2;
+  const uint32_t i2 = row - i01 * a.dim2, i0 = i01 / (uint32_t)a.dim1;
+  const uint32_t i1 = i01 - i0 * a.dim1;
   const float *w = a.w + i0 * a.stride[0] + i1 * a.stride[1] +
                    i2 * a.stride[2];
-  int32_t *keep = a.keep + row * a.budget;
+  int32_t *keep = a.keep + (int64_t)row * a.budget;
   int len = a.width;
   if (a.lengths != nullptr) len = min(max(a.lengths[i0], 0), a.width);
   const int kept = min(len, a.budget);
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512   ? 3
   if (need == 0) return;
 
   // this warp's candidates: per_warp consecutive ones, lane after lane
-  const int per_warp =
-      (int)div_up(div_up((uint64_t)n, 32), (uint64_t)ranks * kWarps) * 32;
+  const uint32_t warps = ranks * kWarps;
+  const int per_warp = ((n + 31u) / 32 + warps - 1) / warps * 32;
   const int64_t first = ((int64_t)rank * kWarps + warp) * per_warp;
   const int begin = (int)(first < n ? first : n);
   const int end = begin + per_warp < n ? begin + per_warp : n;

@@ -56,6 +56,7 @@ class _PlanInfo(ctypes.Structure):
                                       ("workspace_bytes", _u64)]
 
 
+_DIMS = struct.Struct("@3q")
 # cascade_attn_args_t, in the order of _pack_args' arguments
 _ARGS = struct.Struct("@iifi4P6q2P6qPqPqPqqPqqPqqPqqiiPQ")
 
@@ -127,7 +128,7 @@ class _Plan:
             # a blocking copy: the plan is ready for every stream
             self._buf = torch.from_numpy(buf[:info.ints].copy()).to(
                 self.device)
-        self._stream = torch.cuda.current_stream(self.device)
+        self._stream = _raw_stream(self.device.index)
         self._info = info
         self._ref = ctypes.byref(info)
         self.batch, self.tokens = info.batch, info.tokens
@@ -204,6 +205,33 @@ def _rows(name, t, shape, dtype, device):
     return p, st
 
 
+try:                               # the handle alone, without a Stream object
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:                # pragma: no cover - other torch versions
+    def _raw_stream(index):
+        import torch
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+class _on:
+    """Makes `device` the current one for a launch, where it is not."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        import torch
+        self.guard = None
+        if torch.cuda.current_device() != device.index:
+            self.guard = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def _no_grad(*tensors):
     import torch
     if torch.is_grad_enabled():
@@ -277,17 +305,11 @@ def _call(plan, kind, fn, q, k, v, k_pages, v_pages, page_table, scale, add,
             pvp, pvs = _rows("v_pages", v_pages, shape, dt, dev)
         tp, trow = _table(page_table, plan.batch, plan._info.table_cols, dev)
     scale = _scale(scale, D)
-    if torch.cuda.current_device() != dev.index:
-        guard = torch.cuda.device(dev)
-    else:
-        guard = None
-    if guard is not None:
-        guard.__enter__()
-    try:
-        stream = torch.cuda.current_stream(dev)
+    with _on(dev):
+        stream = _raw_stream(dev.index)
         if stream != plan._stream:
             # the plan's memory must not be handed out while this call reads
-            plan._buf.record_stream(stream)
+            plan._buf.record_stream(torch.cuda.current_stream(dev))
         size = plan._info.workspace_bytes
         # freed on return: the allocator hands it out again only to work
         # ordered behind this call on the same stream
@@ -299,10 +321,7 @@ def _call(plan, kind, fn, q, k, v, k_pages, v_pages, page_table, scale, add,
             out[1][1], lse[0], lse[1][0], lse[1][1], before[0], before[1][0],
             before[1][1], weights[0], weights[1][0], weights[1][1],
             weights[2], weights[3], ws.data_ptr() if size else 0, size)
-        check(fn(plan._ref, args, stream.cuda_stream))
-    finally:
-        if guard is not None:
-            guard.__exit__(None, None, None)
+        check(fn(plan._ref, args, stream))
 
 
 _NONE = (0, (0, 0))
@@ -468,13 +487,12 @@ def select_kept(weights, budget, recent=0, sink=0, lengths=None):
         raise ValueError(f"lengths must be int32 [{lead[0]}] on {dev}")
     keep = torch.empty(lead + [budget], dtype=torch.int32, device=dev)
     pad = 3 - len(lead)
-    dims = (_i64 * 3)(*(lead + [1] * pad))
-    strides = (_i64 * 3)(*(st[:-1] + (0,) * pad))
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(_lib.load().cascade_kv_evict_select(
-            weights.data_ptr(), dims, strides, weights.shape[-1],
+            weights.data_ptr(), _DIMS.pack(*lead, *(1,) * pad),
+            _DIMS.pack(*st[:-1], *(0,) * pad), weights.shape[-1],
             lengths.data_ptr() if lengths is not None else None, budget,
-            recent, sink, keep.data_ptr(), kvwire._stream(dev)))
+            recent, sink, keep.data_ptr(), _raw_stream(dev.index)))
     return keep
 
 
@@ -514,18 +532,17 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     kept = min(budget, S)
     keep = keep[..., :kept]
     kv = torch.empty((n, L, 2, H, kept, D), dtype=dt, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(_lib.load().cascade_kv_evict_gather(
-            desc.ctypes.data, n * L, L if weights.dim() == 3 else 1, H, S, D,
+            desc, n * L, L if weights.dim() == 3 else 1, H, S, D,
             dt.itemsize, keep.data_ptr(), kept, None, 0, 0, 0, 0, 0,
-            kv.data_ptr(), kvwire._stream(dev)))
+            kv.data_ptr(), _raw_stream(dev.index)))
     return kv, keep
 
 
 def _descriptors(tensors):
     """Host cascade_kv_tensor_t rows of [1, heads, seq, dim] or [heads, seq,
     dim] tensors of one shape, dtype and device, and those."""
-    import numpy as np
     t0 = tensors[0]
     shape, dt, dev = t0.shape, t0.dtype, t0.device
     if dev.type != "cuda" or dt.itemsize not in (2, 4):
@@ -535,27 +552,18 @@ def _descriptors(tensors):
                          f"{tuple(shape)}")
     H, S, D = shape[-3:]
     other = (1, H, S, D) if len(shape) == 3 else (H, S, D)
-    rows = np.empty((len(tensors), 3), dtype=np.int64)
-    strides = []
+    rows = []
     for t in tensors:
         if (t.shape != shape and t.shape != other) or t.dtype is not dt \
                 or t.device != dev:
             raise ValueError("every K and V must have one shape, dtype and "
                              "device")
-        strides.append(t.stride()[-3:])
-    rows[:, 0] = [t.data_ptr() for t in tensors]
-    if strides.count(strides[0]) == len(strides):
-        rows[:, 1:] = strides[0][:2]
-        strides = strides[:1]
-    else:
-        rows[:, 1:] = [s[:2] for s in strides]
-    if D > 1 and any(s[2] != 1 for s in strides):
-        raise ValueError("head_dim must be contiguous (stride 1)")
-    if H == 1:
-        rows[:, 1] = 0
-    if S == 1:
-        rows[:, 2] = 0
-    return rows, (H, S, D, dev, dt)
+        st = t.stride()
+        if st[-1] != 1 and D > 1:
+            raise ValueError("head_dim must be contiguous (stride 1)")
+        rows += (t.data_ptr(), st[-3] if H > 1 else 0,
+                 st[-2] if S > 1 else 0)
+    return struct.pack(f"@{len(rows)}q", *rows), (H, S, D, dev, dt)
 
 
 def cache_views(kv):
@@ -574,7 +582,6 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
     Returns (k, v, keep): [sequences, kv heads, budget, dim] each and the
     positions, int32 [sequences, kv heads, budget].  A sequence of fewer
     tokens keeps them all; its rows behind them are zeros and -1."""
-    import numpy as np
     import torch
     dev, dt = k_pages.device, k_pages.dtype
     if not k_pages.is_cuda or dt.itemsize not in (2, 4):
@@ -590,26 +597,25 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
         raise ValueError(f"weights must be [{B}, {H}, tokens] on {dev}")
     if page < 1:
         raise ValueError("pages hold at least one token")
-    desc = np.empty((2, 3), np.int64)
+    desc = []
     st = _strides(k_pages)
     if _strides(v_pages)[0] != st[0]:
         raise ValueError("k_pages and v_pages must have one page stride")
-    for i, t in enumerate((k_pages, v_pages)):
+    for t in (k_pages, v_pages):
         s = _strides(t)
         if D > 1 and s[3] != 1:
             raise ValueError("head_dim must be contiguous (stride 1)")
-        desc[i] = (t.data_ptr(), s[1], s[2])
+        desc += (t.data_ptr(), s[1], s[2])
     table, table_row = _table(page_table, B, 0, dev)
     keep = select_kept(weights, budget, recent, sink, lengths)
     kv = torch.empty((B, 2, H, budget, D), dtype=dt, device=dev)
     if kv.numel():
-        src = np.tile(desc, (B, 1))
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(_lib.load().cascade_kv_evict_gather(
-                src.ctypes.data, B, 1, H, 0, D,
-                dt.itemsize, keep.data_ptr(), budget, table, table_row,
+                struct.pack("@6q", *desc) * B, B, 1, H, 0, D, dt.itemsize,
+                keep.data_ptr(), budget, table, table_row,
                 page_table.shape[1], st[0], page, P, kv.data_ptr(),
-                kvwire._stream(dev)))
+                _raw_stream(dev.index)))
     return kv[:, 0], kv[:, 1], keep
 
 
