@@ -278,18 +278,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             raise_maximum<D>(m, l, fmaxf(m, top), first, a.c, tm_o);
           first = false;
           const float mc = m == -INFINITY ? 0.f : m * a.c;
-          float s0 = 0.f, s1 = 0.f;
+          const uint64_t c2 = pair_of(a.c, a.c), m2 = pair_of(-mc, -mc);
+          uint64_t sum[2] = {0, 0};
           uint32_t p[16], none[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float y0 = ex2(fmaf(__uint_as_float(x[2 * e]), a.c, -mc));
-            const float y1 =
-                ex2(fmaf(__uint_as_float(x[2 * e + 1]), a.c, -mc));
-            s0 += y0;
-            s1 += y1;
-            p[e] = pack16<kBf16>(y0, y1);
+            p[e] = weigh2<kBf16>(x[2 * e], x[2 * e + 1], c2, m2, sum[e & 1]);
             none[e] = 0;
           }
+          float s0, s1;
+          unpair(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -359,22 +357,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             raise_maximum<D>(m, l, fmaxf(m, top), first, a.c, tm_o);
           first = false;
           const float mc = m == -INFINITY ? 0.f : m * a.c;
-          float s0 = 0.f, s1 = 0.f;
+          const uint64_t c2 = pair_of(a.c, a.c), m2 = pair_of(-mc, -mc);
+          uint64_t sum[2] = {0, 0};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float y0 =
-                  ex2(fmaf(__uint_as_float(x[i][2 * e]), a.c, -mc));
-              const float y1 =
-                  ex2(fmaf(__uint_as_float(x[i][2 * e + 1]), a.c, -mc));
-              s0 += y0;
-              s1 += y1;
-              p[e] = pack16<kBf16>(y0, y1);
-            }
+            for (int e = 0; e < 16; ++e)
+              p[e] = weigh2<kBf16>(x[i][2 * e], x[i][2 * e + 1], c2, m2,
+                                   sum[e & 1]);
             tc_st16(tm_s + i * 16, p);
           }
+          float s0, s1;
+          unpair(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
           tc_wait_st();
           tc_fence_before();

@@ -369,6 +369,40 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return r;
 }
 
+// Pairs of floats in one register pair: one instruction works on both (and
+// takes half the room in the instruction cache, which is what it is for).
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^(x c + d) of a pair, joined to `sum`; returns the two rounded to 16 bits.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t weigh2(uint32_t x0, uint32_t x1,
+                                           uint64_t c, uint64_t d,
+                                           uint64_t &sum) {
+  float y0, y1;
+  unpair(fma2(pair_of(__uint_as_float(x0), __uint_as_float(x1)), c, d), y0,
+         y1);
+  y0 = ex2(y0);
+  y1 = ex2(y1);
+  sum = add2(sum, pair_of(y0, y1));
+  return pack16<kBf16>(y0, y1);
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------- where a key's row is

@@ -27,7 +27,7 @@ struct WeightArgs {
 };
 
 struct WControl {
-  // lse of a chunk's rows, in powers of two
+  // minus the lse of a chunk's rows, in powers of two
   alignas(16) float lse2[kQSlots][kTile];
   float other[kKeys];              // sums of the odd chunks
   uint64_t k_full[kKSlots], k_empty[kKSlots];
@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
     const uint32_t buf = warp >> 3;
     const int kt = w * kTile + (warp & 3) * 32 + lane;   // key of the item
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
+    const uint64_t c2 = pair_of(a.c, a.c);
     uint32_t step = 0, q_no = 0;
     for (int si = seg_begin; si < seg_end; ++si) {
       const Segment sg = segs[si];
@@ -139,10 +140,15 @@ __global__ void __launch_bounds__(kWThreads, 1)
           const int n = min(kTile, sg.rows - ch * kTile);
           mbar_wait(smem_u32(&ct.s_full[w][buf]), (step >> 1) & 1, give_up);
           tc_fence_after();
-          const float4 *l4 = reinterpret_cast<const float4 *>(ct.lse2[slot]);
+          const ulonglong2 *l4 =
+              reinterpret_cast<const ulonglong2 *>(ct.lse2[slot]);
           const int64_t hidden = from - (int64_t)ch * kTile;
           const bool whole = __all_sync(0xffffffffu, hidden <= 0);
-          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+          uint64_t s0 = 0, s1 = 0;
+          auto add4 = [&](const uint32_t *x, const ulonglong2 &l) {
+            weigh2<false>(x[0], x[1], c2, l.x, s0);
+            weigh2<false>(x[2], x[3], c2, l.y, s1);
+          };
           const uint32_t src = tm + buf * 128;
           if (whole && n == kTile) {
             // kept short: its code and that of the other warps has to stay
@@ -154,13 +160,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
               tc_wait_ld();
               tc_hold(x);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float4 l = l4[i / 4 + e];
-                s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
-                s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
-                s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
-                s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
-              }
+              for (int e = 0; e < 8; ++e) add4(&x[4 * e], l4[i / 4 + e]);
             }
           } else {
             // few rows, or rows that do not see the key: -inf for those
@@ -175,13 +175,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
               for (int e = 0; e < 8; ++e)
                 if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float4 l = l4[i / 4 + e];
-                s0 += ex2(fmaf(__uint_as_float(x[4 * e]), a.c, -l.x));
-                s1 += ex2(fmaf(__uint_as_float(x[4 * e + 1]), a.c, -l.y));
-                s2 += ex2(fmaf(__uint_as_float(x[4 * e + 2]), a.c, -l.z));
-                s3 += ex2(fmaf(__uint_as_float(x[4 * e + 3]), a.c, -l.w));
-              }
+              for (int e = 0; e < 2; ++e) add4(&x[4 * e], l4[i / 4 + e]);
             }
           }
           tc_fence_before();
@@ -194,7 +188,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
             else if (pair + 2 >= sg.n0)
               mbar_arrive(smem_u32(&ct.q_empty[slot]));
           }
-          sum += (s0 + s1) + (s2 + s3);
+          float y0, y1;
+          unpair(add2(s0, s1), y0, y1);
+          sum += y0 + y1;
         }
         if (sg.n0 == 1) {
           // one pair: its odd and even chunks are joined
@@ -242,13 +238,13 @@ __global__ void __launch_bounds__(kWThreads, 1)
     auto row_at = [&](const Segment &sg, int ch, const char **src) {
       const int r = lw * 32 + lane, row = ch * kTile + r;
       *src = nullptr;
-      if (row >= sg.rows) return INFINITY;    // a row that counts for nothing
+      if (row >= sg.rows) return -INFINITY;   // a row that counts for nothing
       const int tok = row / a.group;
       const int64_t head = sg.hk * a.group + row - tok * a.group;
       const int64_t at = (int64_t)sg.tok0 + sg.row0 + tok;
       *src = a.q + at * a.q_tok + head * a.q_head;
       const float l = a.lse[at * a.l_tok + head * a.l_head];
-      return l == -INFINITY ? INFINITY : l * kLog2e;
+      return l == -INFINITY ? -INFINITY : l * -kLog2e;
     };
     auto load_chunk = [&](const Segment &sg, int ch) {
       const uint32_t slot = q_no % kQSlots;
