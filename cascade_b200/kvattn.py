@@ -519,7 +519,11 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
             tensors += kv
     if not tensors:
         raise ValueError("a KV cache needs at least one layer")
-    desc, (H, S, D, dev, dt) = _descriptors(tensors)
+    t0 = tensors[0]
+    if t0.dim() not in (3, 4):
+        raise ValueError("KV tensors are [1, heads, seq, dim]; got "
+                         f"{tuple(t0.shape)}")
+    (H, S, D), dev, dt = t0.shape[-3:], t0.device, t0.dtype
     lead = (n, L, H) if weights.dim() == 4 else (n, H)
     if tuple(weights.shape) != lead + (S,) or weights.device != dev:
         raise ValueError(f"weights must be {lead + (S,)} on {dev}; got "
@@ -528,7 +532,9 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
             recent + sink <= budget:
         recent, sink = min(recent, S), 0         # everything is kept
         budget = max(S, 1)
+    # the choice is made while the host looks the tensors over
     keep = select_kept(weights, budget, recent, sink)
+    desc = _descriptors(tensors, (H, S, D), dev, dt)
     kept = min(budget, S)
     keep = keep[..., :kept]
     kv = torch.empty((n, L, 2, H, kept, D), dtype=dt, device=dev)
@@ -540,30 +546,25 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     return kv, keep
 
 
-def _descriptors(tensors):
+def _descriptors(tensors, shape, dev, dt):
     """Host cascade_kv_tensor_t rows of [1, heads, seq, dim] or [heads, seq,
-    dim] tensors of one shape, dtype and device, and those."""
-    t0 = tensors[0]
-    shape, dt, dev = t0.shape, t0.dtype, t0.device
+    dim] tensors, all of `shape` on `dev`."""
     if dev.type != "cuda" or dt.itemsize not in (2, 4):
         raise ValueError("KV tensors are CUDA tensors of 2- or 4-byte values")
-    if len(shape) not in (3, 4) or (len(shape) == 4 and shape[0] != 1):
-        raise ValueError("KV tensors are [1, heads, seq, dim]; got "
-                         f"{tuple(shape)}")
-    H, S, D = shape[-3:]
-    other = (1, H, S, D) if len(shape) == 3 else (H, S, D)
+    H, S, D = shape
+    one = (1, H, S, D)
     rows = []
     for t in tensors:
-        if (t.shape != shape and t.shape != other) or t.dtype is not dt \
+        if (t.shape != one and t.shape != shape) or t.dtype is not dt \
                 or t.device != dev:
-            raise ValueError("every K and V must have one shape, dtype and "
-                             "device")
+            raise ValueError("every K and V must have one shape ([1,] heads, "
+                             "seq, dim), dtype and device")
         st = t.stride()
         if st[-1] != 1 and D > 1:
             raise ValueError("head_dim must be contiguous (stride 1)")
         rows += (t.data_ptr(), st[-3] if H > 1 else 0,
                  st[-2] if S > 1 else 0)
-    return struct.pack(f"@{len(rows)}q", *rows), (H, S, D, dev, dt)
+    return struct.pack(f"@{len(rows)}q", *rows)
 
 
 def cache_views(kv):
