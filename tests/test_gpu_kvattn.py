@@ -609,3 +609,107 @@ def test_weights_refusals():
             call(**bad)
     with pytest.raises(ValueError):
         c.plan(kvattn.WeightsPlan, window=0)
+
+
+# ------------------------------------------------------ calls of all sorts
+def test_many_short_sequences():
+    n = 3001
+    c = Case([1] * n, [(i * 7) % 40 for i in range(n)], 4, 2, 64, "fp16",
+             seed=70)
+    out, lse = c.run()
+    tok = torch.arange(40, device=DEV)
+    rows = c.pool[c.table.long()[:, tok // 16].clamp(min=0), :, :, tok % 16]
+    k = torch.cat([rows[:, :, 0], c.k[:, None]], 1).double()
+    v = torch.cat([rows[:, :, 1], c.v[:, None]], 1).double()
+    see = torch.ones(n, 41, dtype=torch.bool, device=DEV)
+    see[:, :40] = tok[None] < torch.tensor(c.cached, device=DEV)[:, None]
+    s = torch.einsum("nghd,nkgd->nghk", c.q.double().view(n, 2, 2, 64), k) / 8
+    s = s.masked_fill(~see[:, None, None], -math.inf)
+    want = torch.einsum("nghk,nkgd->nghd", s.softmax(-1), v).view(n, 4, 64)
+    # |v| <= 5.5, the weights and the output are rounded once
+    assert (out.double() - want).abs().max() < 2 * 2.0 ** -11 * 5.5
+    assert (lse.double() - torch.logsumexp(s, -1).view(n, 4)).abs().max() \
+        < 1e-4
+    w = kvattn.attention_weights(c.plan(kvattn.WeightsPlan), c.q, c.k, lse,
+                                 c.pages[0], c.table)
+    assert (w.sum(-1) - 2).abs().max() < 1e-3
+
+
+def test_one_table_row_for_all_sequences():
+    # sequences that share a prefix: an expanded table row
+    c = Case([3, 1, 2], [200, 200, 200], 8, 2, 128, "bf16", seed=71)
+    c.table = c.table[:1].expand(3, -1)
+    check_forward(c, *c.run())
+
+
+def test_mask_of_bytes_and_wider_rows():
+    c = Case([5, 9], [30, 4], 4, 2, 64, "fp16", tree=True, seed=72)
+    want = c.run()
+    wide = torch.zeros(14, 40, dtype=torch.uint8, device=DEV)
+    wide[:, 3:12] = c.mask[:, :9].to(torch.uint8) * 7
+    c.mask = wide[:, 3:20]
+    got = c.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_calls_from_several_threads():
+    import threading
+    cases = [Case([2, 40], [900, 10], 8, 2, 64, "bf16", seed=80 + i)
+             for i in range(4)]
+    want = [c.run() for c in cases]
+    plans = [c.plan() for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                out, lse = cases[i].run(plans[i])
+                s.synchronize()
+                if not torch.equal(out, want[i][0]):
+                    bad.append(i)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from cascade_b200 import kvattn
+plans = [(n, kvattn.AttentionPlan([n], [3000], q_heads=4, kv_heads=1,
+                                  head_dim=64, page_size=16))
+         for n in (1, 20, 200)]
+w = kvattn.WeightsPlan([200], [3000], q_heads=4, kv_heads=1, head_dim=64,
+                       page_size=16)
+t = torch.arange(188, dtype=torch.int32, device="cuda")[None]
+kv = torch.randn(188, 2, 1, 16, 64, device="cuda").half()
+ins = [[torch.randn(n, h, 64, device="cuda").half() for h in (4, 1, 1)]
+       for n, _ in plans]
+def calls():
+    r = [kvattn.prompt_attention(p, *x, (kv[:, 0], kv[:, 1]), t)
+         for (_, p), x in zip(plans, ins)]
+    weights = kvattn.attention_weights(w, ins[2][0], ins[2][1], r[2][1],
+                                       kv[:, 0], t)
+    keep = kvattn.evict_pages(kv[:, 0], kv[:, 1], t, torch.full(
+        (1,), 3000, dtype=torch.int32, device="cuda"), weights, 100)
+    return [o for o, _ in r] + [weights, *keep]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = calls()
+g.replay()
+torch.cuda.synchronize()
+a = [x.clone() for x in a]
+b = calls()
+assert all(torch.equal(x, y) for x, y in zip(a, b))
+print("captured first")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, text=True,
+                       capture_output=True, timeout=120)
+    assert "captured first" in r.stdout, r.stderr[-2000:]

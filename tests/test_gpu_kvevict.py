@@ -334,3 +334,25 @@ def test_store_attend_weigh_evict_store_attend():
     with pytest.raises(ValueError):
         kvwire.store_kv_caches(store, ["x"], [cache], weights=weights)
     store.close()
+
+
+def test_evict_captured_and_on_another_stream():
+    src = caches(2, 3, 2, 500, 64, torch.bfloat16, 1)
+    w = weights("heavy", (2, 3, 2, 500), 2)
+    want, keep = kvattn.evict_kv_caches(src, w, 77, 5, 3)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        kv, k = kvattn.evict_kv_caches(src, w, 77, 5, 3)
+    s.synchronize()
+    assert torch.equal(kv, want) and torch.equal(k, keep)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv, k = kvattn.evict_kv_caches(src, w, 77, 5, 3)
+    kv.zero_()
+    w.mul_(-1.0)                       # other weights, the same graph
+    g.replay()
+    torch.cuda.synchronize()
+    assert not torch.equal(k, keep)
+    check_keep(w, k, 77, 5, 3)
+    check_kv(src, kv, k)
