@@ -509,16 +509,13 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     n = len(caches)
     if n == 0:
         raise ValueError("no caches to evict from")
-    tensors, L = [], 0
-    for c in caches:
-        pairs = kvwire.extract_kv_pairs(c)
-        if L not in (0, len(pairs)):
-            raise ValueError("every cache must have the same layers")
-        L = len(pairs)
-        for kv in pairs:
-            tensors += kv
-    if not tensors:
+    per = [kvwire.extract_kv_pairs(c) for c in caches]
+    L = len(per[0])
+    if any(len(pairs) != L for pairs in per):
+        raise ValueError("every cache must have the same layers")
+    if L == 0:
         raise ValueError("a KV cache needs at least one layer")
+    tensors = [t for pairs in per for kv in pairs for t in kv]
     t0 = tensors[0]
     if t0.dim() not in (3, 4):
         raise ValueError("KV tensors are [1, heads, seq, dim]; got "

@@ -6,6 +6,7 @@ import random
 
 import numpy as np
 import pytest
+import torch
 
 from cascade_b200 import _lib, kvattn
 
@@ -277,3 +278,11 @@ def test_evict_refuses_bad_arguments():
     assert gather(out=None) == 1 and gather(ptr=0) == 1
     assert gather(table=4096, cols=1, page=0) == 1
     assert gather(items=0) == 0 and gather(kept=0) == 0
+
+
+@pytest.mark.parametrize("layers", [(0, 1), (0, 0, 2), (1, 0), (2, 1)])
+def test_evict_refuses_caches_of_different_layers(layers):
+    kv = torch.zeros(1, 2, 9, 8, dtype=torch.float16)
+    caches = [[(kv, kv)] * n for n in layers]
+    with pytest.raises(ValueError, match="same layers"):
+        kvattn.evict_kv_caches(caches, torch.zeros(len(layers), 2, 9), 4)
