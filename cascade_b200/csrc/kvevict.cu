@@ -323,6 +323,9 @@ extern "C" int cascade_kv_evict_select(
                (int64_t)recent + sink <= budget,
            CASCADE_ERR_INVALID,
            "budget must be above 0 and at least recent + sink");
+  // positions are stepped along in 32 bits
+  CB_CHECK(width <= 1 << 30 && budget <= 1 << 30, CASCADE_ERR_INVALID,
+           "rows have at most 2^30 tokens");
   const int64_t big = (int64_t)1 << 27;
   CB_CHECK(dims[0] <= big && dims[1] <= big && dims[2] <= big &&
                dims[0] * dims[1] <= big && dims[0] * dims[1] * dims[2] <= big,

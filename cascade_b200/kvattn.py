@@ -477,8 +477,8 @@ def select_kept(weights, budget, recent=0, sink=0, lengths=None):
     if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
         raise ValueError("budget must be above 0 and at least recent + sink "
                          f"(got {budget}, {recent}, {sink})")
-    if max(budget, weights.shape[-1]) >= 1 << 31:
-        raise ValueError("rows have fewer than 2**31 tokens")
+    if max(budget, weights.shape[-1]) > 1 << 30:
+        raise ValueError("rows have at most 2**30 tokens")
     dev, lead = weights.device, list(weights.shape[:-1])
     if lengths is not None and (
             lengths.dtype != torch.int32 or lengths.device != dev

@@ -248,7 +248,7 @@ void cascade_attn_struct_sizes(size_t *plan_info, size_t *args);
  * to the lowest position; NaN ranks with -inf.  d_lengths (per index of the
  * first dimension, or NULL: all `width`) is clamped to [0, width].  d_keep
  * receives `budget` positions per row, ascending; a row of fewer tokens
- * keeps them all and ends in -1. */
+ * keeps them all and ends in -1.  Rows and budgets have at most 2^30 tokens. */
 int cascade_kv_evict_select(const float *d_weights, const int64_t dims[3],
                             const int64_t strides[3], int32_t width,
                             const int32_t *d_lengths, int32_t budget,

@@ -280,6 +280,16 @@ def test_evict_refuses_bad_arguments():
     assert gather(items=0) == 0 and gather(kept=0) == 0
 
 
+def test_evict_refuses_rows_that_32_bit_steps_would_pass():
+    L = _lib.load()
+    dims, st = (ctypes.c_int64 * 3)(2, 1, 1), (ctypes.c_int64 * 3)(9, 0, 0)
+    for width, budget in ((2 ** 31 - 1, 9), ((1 << 30) + 1, 9),
+                          (9, 2 ** 31 - 1), (9, (1 << 30) + 1)):
+        assert L.cascade_kv_evict_select(4096, dims, st, width, None, budget,
+                                         1, 1, 4096, None) == 1
+        assert b"2^30" in L.cascade_last_error()
+
+
 @pytest.mark.parametrize("layers", [(0, 1), (0, 0, 2), (1, 0), (2, 1)])
 def test_evict_refuses_caches_of_different_layers(layers):
     kv = torch.zeros(1, 2, 9, 8, dtype=torch.float16)
