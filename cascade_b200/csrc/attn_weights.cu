@@ -26,6 +26,16 @@ struct WeightArgs {
   float c;                         // scale * log2(e)
 };
 
+// 2^(x c + d) of a pair, 0 where it is not on.
+__device__ __forceinline__ uint64_t exp2_where(uint32_t x0, uint32_t x1,
+                                               uint64_t c, uint64_t d,
+                                               bool on0, bool on1) {
+  float y0, y1;
+  unpair(fma2(pair_of(__uint_as_float(x0), __uint_as_float(x1)), c, d), y0,
+         y1);
+  return pair_of(on0 ? ex2(y0) : 0.f, on1 ? ex2(y1) : 0.f);
+}
+
 struct WControl {
   // minus the lse of a chunk's rows, in powers of two
   alignas(16) float lse2[kQSlots][kTile];
@@ -163,8 +173,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
               for (int e = 0; e < 8; ++e) add4(&x[4 * e], l4[i / 4 + e]);
             }
           } else {
-            // few rows, or rows that do not see the key: -inf for those
-            // (the scores of rows that are not there may be anything)
+            // few rows, or rows that do not see the key: nothing of those is
+            // added, whatever their scores and lse are (NaN included)
 #pragma unroll 1
             for (int i = 0; i < n; i += 8) {
               uint32_t x[8];
@@ -172,10 +182,14 @@ __global__ void __launch_bounds__(kWThreads, 1)
               tc_wait_ld();
               tc_hold(x);
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (i + e < hidden || i + e >= n) x[e] = 0xff800000u;
-#pragma unroll
-              for (int e = 0; e < 2; ++e) add4(&x[4 * e], l4[i / 4 + e]);
+              for (int e = 0; e < 4; ++e) {
+                const ulonglong2 l = l4[i / 4 + e / 2];
+                const bool on0 = i + 2 * e >= hidden && i + 2 * e < n;
+                const bool on1 = i + 2 * e + 1 >= hidden && i + 2 * e + 1 < n;
+                uint64_t &to = e & 1 ? s1 : s0;
+                to = add2(to, exp2_where(x[2 * e], x[2 * e + 1], c2,
+                                         e & 1 ? l.y : l.x, on0, on1));
+              }
             }
           }
           tc_fence_before();

@@ -590,6 +590,34 @@ def test_weights_of_gone_pages_and_captured():
     assert torch.equal(w, w2)
 
 
+@pytest.mark.parametrize("heads", [2, 8, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_weights_of_keys_that_a_broken_row_does_not_see(value, heads):
+    # tokens 9 and 150 of a prompt ask with inf or NaN, so their lse is NaN:
+    # the keys behind them were not seen by them
+    c = Case([200, 12], [40, 0], heads, 2, 64, "bf16", seed=63)
+    plan = c.plan(kvattn.WeightsPlan)
+
+    def weigh(q, lse, plan=plan):
+        return kvattn.attention_weights(plan, q, c.k, lse, c.pages[0],
+                                        c.table)
+    out, lse = c.run()
+    clean = weigh(c.q, lse)
+    for token, after in ((9, c.plan(kvattn.WeightsPlan)),
+                         (150, c.plan(kvattn.WeightsPlan, window=60))):
+        q = c.q.clone()
+        q[token, :, ::5] = value
+        bad = lse.clone()
+        bad[token] = math.nan
+        want = weigh(c.q, lse, after)
+        got = weigh(q, bad, after)
+        assert got[0, :, :40 + token + 1].isnan().all()
+        assert torch.equal(got[0, :, 40 + token + 1:],
+                           want[0, :, 40 + token + 1:])
+        assert torch.equal(got[1], want[1])
+    assert not clean.isnan().any()
+
+
 def test_weights_refusals():
     c = Case([4, 2], [30, 5], 4, 2, 64, "fp16", seed=62)
     out, lse = c.run()
