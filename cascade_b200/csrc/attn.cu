@@ -503,12 +503,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<float4 *>(
                 a.part_o + ((int64_t)sg.part * kTile + row) * D + col) =
                 make_float4(o[0], o[1], o[2], o[3]);
-          else
+          else {
+            keep_finite<kBf16>(o);
             *reinterpret_cast<uint2 *>(
                 a.out + (int64_t)(sg.tok0 + tk) * a.o_tok +
                 (int64_t)hd * a.o_head + col * 2) =
                 make_uint2(pack16<kBf16>(o[0], o[1]),
                            pack16<kBf16>(o[2], o[3]));
+          }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         continue;
@@ -605,6 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 store32(dst + 8 * i, v, true);
               }
             } else {
+              keep_finite<kBf16>(o);
 #pragma unroll
               for (int e = 0; e < 8; ++e)
                 v[e] = pack16<kBf16>(o[2 * e], o[2 * e + 1]);
@@ -992,9 +995,12 @@ __global__ void __launch_bounds__(256)
   char *dst = a.out + (int64_t)(mg.tok0 + tok) * a.o_tok +
               (int64_t)head * a.o_head + lane * kPer * 2;
 #pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] *= inv;
+  keep_finite<kBf16>(acc);
+#pragma unroll
   for (int e = 0; e < kPer; e += 2)
     *reinterpret_cast<uint32_t *>(dst + e * 2) =
-        pack16<kBf16>(acc[e] * inv, acc[e + 1] * inv);
+        pack16<kBf16>(acc[e], acc[e + 1]);
   if (lane == 0)
     a.lse[(int64_t)(mg.tok0 + tok) * a.l_tok + (int64_t)head * a.l_head] =
         top == -INFINITY ? (total != total ? NAN : -INFINITY)

@@ -369,6 +369,21 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return r;
 }
 
+// FP16 outputs: a mean of values lies within the type's range, but P's
+// rounding can take it 2^-11 beyond the largest value, which would round to
+// infinity.  Infinities themselves stay.
+template <bool kBf16, int kN>
+__device__ __forceinline__ void keep_finite(float (&o)[kN]) {
+  if (kBf16) return;
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < kN; ++e) top = fmaxf(top, fabsf(o[e]));
+  if (top <= 65504.f) return;
+#pragma unroll
+  for (int e = 0; e < kN; ++e)
+    if (fabsf(o[e]) < INFINITY) o[e] = fminf(fmaxf(o[e], -65504.f), 65504.f);
+}
+
 // Pairs of floats in one register pair: one instruction works on both (and
 // takes half the room in the instruction cache, which is what it is for).
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {

@@ -326,6 +326,35 @@ def test_scores_of_minus_infinity_weigh_nothing(heads):
     assert not torch.equal(clean[0], want[0])
 
 
+@pytest.mark.parametrize("heads,new", [(2, 1), (64, 1), (8, 64), (8, 300)])
+@pytest.mark.parametrize("cached", [400, 9000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_means_of_the_largest_values_stay_finite(heads, new, cached, sign):
+    # Every value is the largest of FP16 and 31 of 32 weights round up by
+    # nearly half a step, 2^-11: the sum of the products would round to
+    # infinity, the mean of such values is that value.
+    c = Case([new], [cached], heads, 2, 64, "fp16", seed=11, scale=1.0)
+    top = torch.finfo(torch.float16).max
+    # p = (1 + 1.1 * 2^-11) / 2, its score as a sum of two halves
+    x = math.log(0.5 * (1 + 1.1 * 2.0 ** -11))
+    coarse = torch.tensor(x).half()
+    fine = torch.tensor(x - float(coarse)).half()
+    c.q, c.k, c.v = c.q.clone(), c.k.clone(), c.v.clone()
+    c.q.zero_()
+    c.q[..., :2] = 1.0
+    c.pool[:, 0] = 0.0
+    c.pool[:, 0, ..., 0], c.pool[:, 0, ..., 1] = coarse, fine
+    c.pool[c.table[0, ::2].long(), 0, :, 0] = 0.0  # p = 1, each 32nd token
+    c.pool[:, 1] = sign * top
+    c.k.zero_()
+    c.k[..., 0], c.k[..., 1] = coarse, fine
+    c.v.fill_(sign * top)
+    out, lse = c.run()
+    # P's roundings 2^-11, the output's 2^-11, sums of n values n 2^-24
+    low = top * (1 - 2.0 ** -10 - (cached + new) * 2.0 ** -23)
+    assert (out.float() * sign >= low).all() and out.isfinite().all()
+
+
 def test_layouts_and_untouched_rows():
     # q, out and lse as slices of larger tensors, K and V as a permuted
     # [heads, tokens, dim] cache, more packed rows than the plan has
