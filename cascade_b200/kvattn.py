@@ -237,7 +237,7 @@ def _no_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                raise RuntimeError("the attention operators have no backward "
+                raise RuntimeError("operators over KV caches have no backward "
                                    "pass: call them under torch.no_grad()")
 
 
@@ -466,6 +466,7 @@ def select_kept(weights, budget, recent=0, sink=0, lengths=None):
     sequence early.  Returns int32 [sequences, ..., budget], ascending; a row
     of fewer tokens than budget keeps all and ends in -1."""
     import torch
+    _no_grad(weights)
     if weights.dtype != torch.float32 or not weights.is_cuda:
         raise ValueError("weights must be a float32 CUDA tensor")
     if not 2 <= weights.dim() <= 4:
@@ -516,6 +517,7 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     if L == 0:
         raise ValueError("a KV cache needs at least one layer")
     tensors = [t for pairs in per for kv in pairs for t in kv]
+    _no_grad(*tensors)
     t0 = tensors[0]
     if t0.dim() not in (3, 4):
         raise ValueError("KV tensors are [1, heads, seq, dim]; got "
@@ -581,6 +583,7 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
     positions, int32 [sequences, kv heads, budget].  A sequence of fewer
     tokens keeps them all; its rows behind them are zeros and -1."""
     import torch
+    _no_grad(k_pages, v_pages)
     dev, dt = k_pages.device, k_pages.dtype
     if not k_pages.is_cuda or dt.itemsize not in (2, 4):
         raise ValueError("pages must be CUDA tensors of 2- or 4-byte values")

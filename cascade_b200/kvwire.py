@@ -281,9 +281,11 @@ def store_kv_caches(store, block_ids: Sequence, caches: Sequence,
     if n == 0:
         return []
     if weights is not None:
+        import torch
         from . import kvattn
-        caches = kvattn.cache_views(kvattn.evict_kv_caches(
-            caches, weights, budget, recent, sink)[0])
+        with torch.no_grad():          # blocks hold values, no gradients
+            caches = kvattn.cache_views(kvattn.evict_kv_caches(
+                caches, weights, budget, recent, sink)[0])
     L, H, S, D, dev, dt, src = _sources(caches)
     keys = np.frombuffer(b"".join(store._key(b) for b in block_ids),
                          dtype=np.uint8).copy()

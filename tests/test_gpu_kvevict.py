@@ -238,6 +238,39 @@ def test_evict_refusals():
             kvattn.evict_pages(*a, 4)
 
 
+def test_evict_refuses_what_needs_a_gradient():
+    src = caches(2, 2, 2, 30, 64, torch.float16, 0)
+    w = torch.rand(2, 2, 2, 30, device=DEV)
+    grad = [[(k.clone().requires_grad_(), v) for k, v in c] for c in src]
+    kp = torch.zeros(3, 2, 16, 64, device=DEV).half()
+    t = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    n = torch.full((2,), 20, dtype=torch.int32, device=DEV)
+    pw = torch.rand(2, 2, 30, device=DEV)
+    for f in (lambda: kvattn.evict_kv_caches(grad, w, 10),
+              lambda: kvattn.evict_kv_caches(src, w.clone().requires_grad_(),
+                                             10),
+              lambda: kvattn.select_kept(w.clone().requires_grad_(), 10),
+              lambda: kvattn.evict_pages(kp.clone().requires_grad_(), kp, t,
+                                         n, pw, 4),
+              lambda: kvattn.evict_pages(kp, kp.clone().requires_grad_(), t,
+                                         n, pw, 4)):
+        with pytest.raises(RuntimeError, match="backward"):
+            f()
+        with torch.no_grad():
+            f()
+    # what is stored has no gradient to lose
+    store = _store()
+    st = kvwire.store_kv_caches(store, ["a", "b"], grad, weights=w, budget=10)
+    assert (np.asarray(st) == 0).all()
+    got = kvwire.load_kv_caches(store, ["a", "b"], 2, 2, 10, 64)
+    kv, _ = kvattn.evict_kv_caches(src, w, 10)
+    for i, cache in enumerate(got):
+        for l, (k, v) in enumerate(cache):
+            assert torch.equal(k[0], kv[i, l, 0])
+            assert torch.equal(v[0], kv[i, l, 1])
+    store.close()
+
+
 # ------------------------------------------------------- a run of them all
 def _store(gib=1):
     cfg = cc.CascadeConfig()
