@@ -4,7 +4,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
-#include <new>
+#include <exception>
 #include <queue>
 #include <vector>
 
@@ -534,7 +534,7 @@ extern "C" int cascade_attn_plan(cascade_attn_plan_info_t *info,
   try {
     return cb::attn::make_plan(info, new_lengths, cached_lengths, out,
                                capacity);
-  } catch (const std::bad_alloc &) {
+  } catch (const std::exception &) {     // an allocation's, there are no others
     cb::set_error("out of host memory for the plan");
     return CASCADE_ERR_NOMEM;
   }

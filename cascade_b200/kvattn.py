@@ -20,10 +20,11 @@ count as unseen.  Query head h uses key/value head h // (q_heads //
 kv_heads).  Tensors are float16 or bfloat16, head_dim 64 or 128 and
 contiguous; other strides may be anything whose rows start on 16-byte
 boundaries (a slice of a fused projection, a [1, heads, seq, dim] cache
-permuted to [seq, heads, dim]).  Rows of `out` that belong to no sequence are
-left as they were.  A value of V that is not finite leaves the rows that see
-it not finite, and the rows that do not see it alone.  There are no backward passes: tensors that require a
-gradient are refused while gradients are enabled.
+permuted to [seq, heads, dim]).  Outputs share no memory with inputs, except
+where a call says so.  Rows of `out` that belong to no sequence are left as
+they were.  A value of V that is not finite leaves the rows that see it not
+finite, and the rows that do not see it alone.  There are no backward passes:
+tensors that require a gradient are refused while gradients are enabled.
 
 Work is enqueued on the current stream of the tensors' device.  A plan may be
 used on any stream, and in captured graphs for as long as it is kept alive;
@@ -237,8 +238,9 @@ def _no_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                raise RuntimeError("operators over KV caches have no backward "
-                                   "pass: call them under torch.no_grad()")
+                raise RuntimeError("operators over KV caches have no "
+                                   "backward pass: call them under "
+                                   "torch.no_grad()")
 
 
 def _writable(name, t):
@@ -577,7 +579,8 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
                 recent=0, sink=0):
     """The same for one layer of a batch in pages: sequence b's tokens are
     the first lengths[b] (int32 CUDA [sequences]) of the pages that its row
-    of page_table names; weights is float32 [sequences, kv heads, tokens].
+    of page_table names, and no more than weights, float32 [sequences, kv
+    heads, tokens], has.
 
     Returns (k, v, keep): [sequences, kv heads, budget, dim] each and the
     positions, int32 [sequences, kv heads, budget].  A sequence of fewer
