@@ -33,6 +33,7 @@ that overlap share nothing.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import struct
 
@@ -206,31 +207,27 @@ def _rows(name, t, shape, dtype, device):
     return p, st
 
 
-try:                               # the handle alone, without a Stream object
+try:                               # the plain calls, without Python objects
     from torch._C import _cuda_getCurrentRawStream as _raw_stream
+    from torch._C import _cuda_getDevice as _current_device
 except ImportError:                # pragma: no cover - other torch versions
     def _raw_stream(index):
         import torch
         return torch.cuda.current_stream(index).cuda_stream
 
-
-class _on:
-    """Makes `device` the current one for a launch, where it is not."""
-    __slots__ = ("guard",)
-
-    def __init__(self, device):
+    def _current_device():
         import torch
-        self.guard = None
-        if torch.cuda.current_device() != device.index:
-            self.guard = torch.cuda.device(device)
+        return torch.cuda.current_device()
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(device, fn, *args):
+    """fn(*args, current stream of `device`), with that device current."""
+    if _current_device() == device.index:
+        check(fn(*args, _raw_stream(device.index)))
+        return
+    import torch
+    with torch.cuda.device(device):
+        check(fn(*args, _raw_stream(device.index)))
 
 
 def _no_grad(*tensors):
@@ -307,23 +304,21 @@ def _call(plan, kind, fn, q, k, v, k_pages, v_pages, page_table, scale, add,
             pvp, pvs = _rows("v_pages", v_pages, shape, dt, dev)
         tp, trow = _table(page_table, plan.batch, plan._info.table_cols, dev)
     scale = _scale(scale, D)
-    with _on(dev):
-        stream = _raw_stream(dev.index)
-        if stream != plan._stream:
-            # the plan's memory must not be handed out while this call reads
-            plan._buf.record_stream(torch.cuda.current_stream(dev))
-        size = plan._info.workspace_bytes
-        # freed on return: the allocator hands it out again only to work
-        # ordered behind this call on the same stream
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        args = _ARGS.pack(
-            code, P, scale, add, plan._ptr, qp, kp, vp, qs[0], qs[1], ks[0],
-            ks[1], vs[0], vs[1], pkp, pvp, pks[0], pks[1], pks[2], pvs[0],
-            pvs[1], pvs[2], tp, trow, mask[0], mask[1], out[0], out[1][0],
-            out[1][1], lse[0], lse[1][0], lse[1][1], before[0], before[1][0],
-            before[1][1], weights[0], weights[1][0], weights[1][1],
-            weights[2], weights[3], ws.data_ptr() if size else 0, size)
-        check(fn(plan._ref, args, stream))
+    if _raw_stream(dev.index) != plan._stream:
+        # the plan's memory must not be handed out while this call reads
+        plan._buf.record_stream(torch.cuda.current_stream(dev))
+    size = plan._info.workspace_bytes
+    # freed on return: the allocator hands it out again only to work
+    # ordered behind this call on the same stream
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    args = _ARGS.pack(
+        code, P, scale, add, plan._ptr, qp, kp, vp, qs[0], qs[1], ks[0],
+        ks[1], vs[0], vs[1], pkp, pvp, pks[0], pks[1], pks[2], pvs[0],
+        pvs[1], pvs[2], tp, trow, mask[0], mask[1], out[0], out[1][0],
+        out[1][1], lse[0], lse[1][0], lse[1][1], before[0], before[1][0],
+        before[1][1], weights[0], weights[1][0], weights[1][1],
+        weights[2], weights[3], ws.data_ptr() if size else 0, size)
+    _launch(dev, fn, plan._ref, args)
 
 
 _NONE = (0, (0, 0))
@@ -474,28 +469,35 @@ def select_kept(weights, budget, recent=0, sink=0, lengths=None):
     if not 2 <= weights.dim() <= 4:
         raise ValueError("weights has 1 to 3 dimensions before the tokens; "
                          f"got shape {tuple(weights.shape)}")
-    st = _strides(weights)
-    if weights.shape[-1] > 1 and st[-1] != 1:
+    lead = tuple(weights.shape[:-1])
+    if lengths is not None and (
+            lengths.dtype != torch.int32 or lengths.device != weights.device
+            or tuple(lengths.shape) != (lead[0],)
+            or not lengths.is_contiguous()):
+        raise ValueError(f"lengths must be int32 [{lead[0]}] on "
+                         f"{weights.device}")
+    return _select(weights, lead, weights.shape[-1], weights.device, budget,
+                   recent, sink, lengths)
+
+
+def _select(weights, lead, width, dev, budget, recent, sink, lengths=None):
+    """select_kept for float32 weights of shape (*lead, width) on dev."""
+    import torch
+    st = weights.stride()
+    if width > 1 and st[-1] != 1:
         raise ValueError("weights: rows must be contiguous")
     if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
         raise ValueError("budget must be above 0 and at least recent + sink "
                          f"(got {budget}, {recent}, {sink})")
-    if max(budget, weights.shape[-1]) > 1 << 30:
+    if max(budget, width) > 1 << 30:
         raise ValueError("rows have at most 2**30 tokens")
-    dev, lead = weights.device, list(weights.shape[:-1])
-    if lengths is not None and (
-            lengths.dtype != torch.int32 or lengths.device != dev
-            or tuple(lengths.shape) != (lead[0],)
-            or not lengths.is_contiguous()):
-        raise ValueError(f"lengths must be int32 [{lead[0]}] on {dev}")
-    keep = torch.empty(lead + [budget], dtype=torch.int32, device=dev)
+    keep = torch.empty(lead + (budget,), dtype=torch.int32, device=dev)
     pad = 3 - len(lead)
-    with _on(dev):
-        check(_lib.load().cascade_kv_evict_select(
-            weights.data_ptr(), _DIMS.pack(*lead, *(1,) * pad),
-            _DIMS.pack(*st[:-1], *(0,) * pad), weights.shape[-1],
+    _launch(dev, _lib.load().cascade_kv_evict_select, weights.data_ptr(),
+            _DIMS.pack(*lead, *(1,) * pad),
+            _DIMS.pack(*st[:-1], *(0,) * pad), width,
             lengths.data_ptr() if lengths is not None else None, budget,
-            recent, sink, keep.data_ptr(), _raw_stream(dev.index)))
+            recent, sink, keep.data_ptr())
     return keep
 
 
@@ -519,7 +521,7 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     if L == 0:
         raise ValueError("a KV cache needs at least one layer")
     tensors = [t for pairs in per for kv in pairs for t in kv]
-    _no_grad(*tensors)
+    _no_grad(weights, *tensors)
     t0 = tensors[0]
     if t0.dim() not in (3, 4):
         raise ValueError("KV tensors are [1, heads, seq, dim]; got "
@@ -533,39 +535,42 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
             recent + sink <= budget:
         recent, sink = min(recent, S), 0         # everything is kept
         budget = max(S, 1)
+    if weights.dtype is not torch.float32 or dev.type != "cuda":
+        raise ValueError("weights must be a float32 CUDA tensor")
     # the choice is made while the host looks the tensors over
-    keep = select_kept(weights, budget, recent, sink)
+    keep = _select(weights, lead, S, dev, budget, recent, sink)
     desc = _descriptors(tensors, (H, S, D), dev, dt)
     kept = min(budget, S)
-    keep = keep[..., :kept]
+    if kept < budget:
+        keep = keep[..., :kept]
     kv = torch.empty((n, L, 2, H, kept, D), dtype=dt, device=dev)
-    with _on(dev):
-        check(_lib.load().cascade_kv_evict_gather(
-            desc, n * L, L if weights.dim() == 3 else 1, H, S, D,
-            dt.itemsize, keep.data_ptr(), kept, None, 0, 0, 0, 0, 0,
-            kv.data_ptr(), _raw_stream(dev.index)))
+    _launch(dev, _lib.load().cascade_kv_evict_gather, desc.buffer_info()[0],
+            n * L, L if len(lead) == 2 else 1, H, S, D, dt.itemsize,
+            keep.data_ptr(), kept, None, 0, 0, 0, 0, 0, kv.data_ptr())
     return kv, keep
 
 
 def _descriptors(tensors, shape, dev, dt):
-    """Host cascade_kv_tensor_t rows of [1, heads, seq, dim] or [heads, seq,
-    dim] tensors, all of `shape` on `dev`."""
-    if dev.type != "cuda" or dt.itemsize not in (2, 4):
+    """Host cascade_kv_tensor_t rows, as an array, of [1, heads, seq, dim] or
+    [heads, seq, dim] tensors, all of `shape` on `dev`."""
+    if dt.itemsize not in (2, 4):
         raise ValueError("KV tensors are CUDA tensors of 2- or 4-byte values")
     H, S, D = shape
     one = (1, H, S, D)
-    rows = []
+    rows = array.array("q")
     for t in tensors:
-        if (t.shape != one and t.shape != shape) or t.dtype is not dt \
+        size = t.shape
+        if (size != one and size != shape) or t.dtype is not dt \
                 or t.device != dev:
             raise ValueError("every K and V must have one shape ([1,] heads, "
                              "seq, dim), dtype and device")
         st = t.stride()
         if st[-1] != 1 and D > 1:
             raise ValueError("head_dim must be contiguous (stride 1)")
-        rows += (t.data_ptr(), st[-3] if H > 1 else 0,
-                 st[-2] if S > 1 else 0)
-    return struct.pack(f"@{len(rows)}q", *rows)
+        rows.append(t.data_ptr())
+        rows.append(st[-3] if H > 1 else 0)
+        rows.append(st[-2] if S > 1 else 0)
+    return rows
 
 
 def cache_views(kv):
@@ -614,12 +619,10 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
     keep = select_kept(weights, budget, recent, sink, lengths)
     kv = torch.empty((B, 2, H, budget, D), dtype=dt, device=dev)
     if kv.numel():
-        with _on(dev):
-            check(_lib.load().cascade_kv_evict_gather(
+        _launch(dev, _lib.load().cascade_kv_evict_gather,
                 struct.pack("@6q", *desc) * B, B, 1, H, 0, D, dt.itemsize,
                 keep.data_ptr(), budget, table, table_row,
-                page_table.shape[1], st[0], page, P, kv.data_ptr(),
-                _raw_stream(dev.index)))
+                page_table.shape[1], st[0], page, P, kv.data_ptr())
     return kv[:, 0], kv[:, 1], keep
 
 
