@@ -140,8 +140,9 @@ __device__ __forceinline__ void give_back(float (&o)[kN], const KvSource &kv,
 // O stay in TMEM, P (rounded to the inputs' 16 bits, as an MMA operand must
 // be; its sum l is taken in FP32 before the rounding) overwrites its own S,
 // and a thread owns one row, so no reduction crosses threads.  O is rescaled
-// only when a row's maximum grew by more than 2^8 (P and l then exceed 1 by
-// at most that, far inside both types' ranges).
+// only when a row's maximum grew by more than 2^8, so weights reach 2^8; in
+// FP16 they are scaled by 2^7 besides, to 2^15 at most (its largest is 2^16),
+// so that weights down to 2^-21 of the largest keep all their bits.
 //
 // Roles.  Two softmax warpgroups, four loader warps that keep a ring of K and
 // V tiles full (TMA for whole tiles, cp.async for ragged ones), and one or two
@@ -164,6 +165,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ TileMaps maps) {
   using Sh = Shape<D, kForm>;
   constexpr bool kDual = Sh::kDual, kFew = kForm == kFewRows;
+  // P and l are 2^kShift times the weights, so that fewer of them fall below
+  // 2^-14, where FP16 has fewer bits
+  constexpr float kShift = kBf16 ? 0.f : 7.f;
+  constexpr float kUnshift = kBf16 ? 1.f : 0x1p-7f;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sm_q = smem_u32(smem);
   const uint32_t sm_ring = sm_q + Sh::kQTiles * Sh::kTileBytes;
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (__any_sync(0xffffffffu, top > m + grow))
             raise_maximum<D>(m, l, fmaxf(m, top), first, a.c, tm_o);
           first = false;
-          const float mc = m == -INFINITY ? 0.f : m * a.c;
+          const float mc = m == -INFINITY ? 0.f : fmaf(m, a.c, -kShift);
           const uint64_t c2 = pair_of(a.c, a.c), m2 = pair_of(-mc, -mc);
           uint64_t sum[2] = {0, 0};
           uint32_t p[16], none[16];
@@ -356,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (__any_sync(0xffffffffu, top > m + grow))
             raise_maximum<D>(m, l, fmaxf(m, top), first, a.c, tm_o);
           first = false;
-          const float mc = m == -INFINITY ? 0.f : m * a.c;
+          const float mc = m == -INFINITY ? 0.f : fmaf(m, a.c, -kShift);
           const uint64_t c2 = pair_of(a.c, a.c), m2 = pair_of(-mc, -mc);
           uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -468,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (row_on && part == 0 && w == 0) {
           const float lse =
-              empty ? -INFINITY : mm * a.scale + logf(lsum);
+              empty ? -INFINITY : mm * a.scale + logf(lsum * kUnshift);
           if (sg.part >= 0)
             a.part_lse[(int64_t)sg.part * kTile + lane] = lse;
           else
@@ -553,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float inv = empty ? 0.f : 1.f / lsum;
         const float fill = empty && seen ? NAN : 0.f;
         const float lse =
-            empty ? -INFINITY : mm * a.scale + logf(lsum);
+            empty ? -INFINITY : mm * a.scale + logf(lsum * kUnshift);
         f1 *= inv;
         f2 *= inv;
         if (!steps || empty) f1 = 0.f;

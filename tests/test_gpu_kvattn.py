@@ -355,6 +355,32 @@ def test_means_of_the_largest_values_stay_finite(heads, new, cached, sign):
     assert (out.float() * sign >= low).all() and out.isfinite().all()
 
 
+@pytest.mark.parametrize("heads,new", [(2, 1), (64, 1), (8, 64), (8, 300)])
+@pytest.mark.parametrize("cached", [400, 9000])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_small_weights_beside_a_large_one_of_no_value(heads, new, cached,
+                                                      dtype):
+    # Each 32nd token takes nearly all weight and has the value 0; the others
+    # weigh 11.6 * 2^-24, which has four bits as an FP16 number.
+    c = Case([new], [cached], heads, 2, 64, dtype, seed=12, scale=1.0)
+    x = math.log(11.6 * 2.0 ** -24)
+    coarse = torch.tensor(x).to(c.dt)
+    fine = torch.tensor(x - float(coarse)).to(c.dt)
+    c.q, c.k, c.v = c.q.clone(), c.k.clone(), c.v.clone()
+    c.q.zero_()
+    c.q[..., :2] = 1.0
+    c.k.zero_()
+    c.k[..., 0], c.k[..., 1] = coarse, fine
+    c.v.fill_(1000.0)
+    c.pool[:, 0] = 0.0
+    c.pool[:, 0, ..., 0], c.pool[:, 0, ..., 1] = coarse, fine
+    c.pool[:, 1] = 1000.0
+    ids = c.table[0, ::2].long()
+    c.pool[ids, :, :, 0] = 0.0
+    out, lse = c.run()
+    check_forward(c, out, lse)
+
+
 def test_layouts_and_untouched_rows():
     # q, out and lse as slices of larger tensors, K and V as a permuted
     # [heads, tokens, dim] cache, more packed rows than the plan has
