@@ -130,6 +130,9 @@ class _Plan:
             # a blocking copy: the plan is ready for every stream
             self._buf = torch.from_numpy(buf[:info.ints].copy()).to(
                 self.device)
+            # new_empty of a tensor takes less time than torch.empty
+            self._f32 = torch.empty(0, device=self.device,
+                                    dtype=torch.float32)
         self._stream = _raw_stream(self.device.index)
         self._info = info
         self._ref = ctypes.byref(info)
@@ -347,13 +350,14 @@ def _forward(plan, q, k, v, mask, pages, page_table, scale, out, lse):
             raise ValueError("mask: rows must be contiguous")
         mp = mask.data_ptr(), mask.stride(0)
     if out is None:
-        out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
+        # (_call refuses a q of another shape or device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         op = out.data_ptr(), (H * D, D)
     else:
         _writable("out", out)
         op = _rows("out", out, (rows, H, D), q.dtype, dev)
     if lse is None:
-        lse = torch.empty((rows, H), dtype=torch.float32, device=dev)
+        lse = plan._f32.new_empty((rows, H))
         lp = lse.data_ptr(), (H, 1)
     else:
         _writable("lse", lse)
@@ -439,8 +443,7 @@ def attention_weights(plan, q, k, lse, k_pages=None, page_table=None, *,
         bp, add = _weight_rows("add_to", add_to, plan), 1
     if out is None:
         width = plan.max_keys if add_to is None else add_to.shape[2]
-        out = torch.empty((plan.batch, plan.kv_heads, width),
-                          dtype=torch.float32, device=dev)
+        out = plan._f32.new_empty((plan.batch, plan.kv_heads, width))
         wp, fill = (out.data_ptr(), out.stride()), 1
     else:
         _writable("out", out)
@@ -491,7 +494,7 @@ def _select(weights, lead, width, dev, budget, recent, sink, lengths=None):
                          f"(got {budget}, {recent}, {sink})")
     if max(budget, width) > 1 << 30:
         raise ValueError("rows have at most 2**30 tokens")
-    keep = torch.empty(lead + (budget,), dtype=torch.int32, device=dev)
+    keep = weights.new_empty(lead + (budget,), dtype=torch.int32)
     pad = 3 - len(lead)
     _launch(dev, _lib.load().cascade_kv_evict_select, weights.data_ptr(),
             _DIMS.pack(*lead, *(1,) * pad),
@@ -543,7 +546,7 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
     kept = min(budget, S)
     if kept < budget:
         keep = keep[..., :kept]
-    kv = torch.empty((n, L, 2, H, kept, D), dtype=dt, device=dev)
+    kv = t0.new_empty((n, L, 2, H, kept, D))
     _launch(dev, _lib.load().cascade_kv_evict_gather, desc.buffer_info()[0],
             n * L, L if len(lead) == 2 else 1, H, S, D, dt.itemsize,
             keep.data_ptr(), kept, None, 0, 0, 0, 0, 0, kv.data_ptr())
