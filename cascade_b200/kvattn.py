@@ -556,23 +556,31 @@ def evict_kv_caches(caches, weights, budget, recent=0, sink=0):
 def _descriptors(tensors, shape, dev, dt):
     """Host cascade_kv_tensor_t rows, as an array, of [1, heads, seq, dim] or
     [heads, seq, dim] tensors, all of `shape` on `dev`."""
+    import torch
     if dt.itemsize not in (2, 4):
         raise ValueError("KV tensors are CUDA tensors of 2- or 4-byte values")
     H, S, D = shape
-    one = (1, H, S, D)
-    rows = array.array("q")
-    for t in tensors:
-        size = t.shape
-        if (size != one and size != shape) or t.dtype is not dt \
-                or t.device != dev:
-            raise ValueError("every K and V must have one shape ([1,] heads, "
-                             "seq, dim), dtype and device")
-        st = t.stride()
+    n, one, T = len(tensors), (1, H, S, D), torch.Tensor
+    # whole lists at a time: 0.4 us a tensor, one by one 0.65
+    sizes = [t.shape for t in tensors]
+    if (sizes.count(one) + sizes.count(shape) != n
+            or [t.dtype for t in tensors].count(dt) != n
+            or list(map(T.get_device, tensors)).count(dev.index) != n):
+        raise ValueError("every K and V must have one shape ([1,] heads, "
+                         "seq, dim), dtype and device")
+    rows = array.array("q", bytes(24 * n))
+    rows[0::3] = array.array("q", map(T.data_ptr, tensors))
+    strides = list(map(T.stride, tensors))
+    if strides.count(strides[0]) == n:          # the usual case
+        strides = strides[:1]
+    for i, st in enumerate(strides):
         if st[-1] != 1 and D > 1:
             raise ValueError("head_dim must be contiguous (stride 1)")
-        rows.append(t.data_ptr())
-        rows.append(st[-3] if H > 1 else 0)
-        rows.append(st[-2] if S > 1 else 0)
+        rows[3 * i + 1] = st[-3] if H > 1 else 0
+        rows[3 * i + 2] = st[-2] if S > 1 else 0
+    if len(strides) < n:
+        rows[1::3] = rows[1:2] * n
+        rows[2::3] = rows[2:3] * n
     return rows
 
 
