@@ -617,24 +617,21 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
         raise ValueError(f"weights must be [{B}, {H}, tokens] on {dev}")
     if page < 1:
         raise ValueError("pages hold at least one token")
-    desc = []
-    st = _strides(k_pages)
-    if _strides(v_pages)[0] != st[0]:
+    ks, vs = _strides(k_pages), _strides(v_pages)
+    if ks[0] != vs[0]:
         raise ValueError("k_pages and v_pages must have one page stride")
-    for t in (k_pages, v_pages):
-        s = _strides(t)
-        if D > 1 and s[3] != 1:
-            raise ValueError("head_dim must be contiguous (stride 1)")
-        desc += (t.data_ptr(), s[1], s[2])
+    if D > 1 and not ks[3] == vs[3] == 1:
+        raise ValueError("head_dim must be contiguous (stride 1)")
     table, table_row = _table(page_table, B, 0, dev)
     keep = select_kept(weights, budget, recent, sink, lengths)
-    kv = torch.empty((B, 2, H, budget, D), dtype=dt, device=dev)
+    kv = k_pages.new_empty((B, 2, H, budget, D))
     if kv.numel():
-        _launch(dev, _lib.load().cascade_kv_evict_gather,
-                struct.pack("@6q", *desc) * B, B, 1, H, 0, D, dt.itemsize,
-                keep.data_ptr(), budget, table, table_row,
-                page_table.shape[1], st[0], page, P, kv.data_ptr())
-    return kv[:, 0], kv[:, 1], keep
+        desc = struct.pack("@6q", k_pages.data_ptr(), ks[1], ks[2],
+                           v_pages.data_ptr(), vs[1], vs[2])
+        _launch(dev, _lib.load().cascade_kv_evict_gather, desc * B, B, 1, H,
+                0, D, dt.itemsize, keep.data_ptr(), budget, table, table_row,
+                page_table.shape[1], ks[0], page, P, kv.data_ptr())
+    return (*kv.unbind(1), keep)
 
 
 def wait_timeouts() -> int:
