@@ -78,7 +78,6 @@ __global__ void __launch_bounds__(kWThreads, 1)
   volatile int *give_up = &ct.give_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  let_next_start();
   if (sm_k & 1023) {
     if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1u);
     return;
@@ -107,9 +106,13 @@ __global__ void __launch_bounds__(kWThreads, 1)
   tc_fence_after();
   const uint32_t tmem = ct.tmem;
 
+  // The launch may be early: only the plan is sure to be there, all else may
+  // be what the kernel before this one writes.
   const Segment *segs =
       reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
   const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
+  wait_for_previous();
+  let_next_start();
 
   if (warp < 16) {
     // ---------------------------------------------------------- sums
@@ -418,9 +421,9 @@ int run_weights(const WeightArgs &a, const TileMaps &maps,
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     once.set();
   }
-  kernel<<<p.ctas, kWThreads, smem, s>>>(a, maps);
+  CB_CUDA(launch_early(kernel, dim3(p.ctas), dim3(kWThreads), smem, s, a,
+                       maps));
   count_launches(1);
-  CB_CUDA(cudaGetLastError());
   if (p.merges > 0) {
     const Segment *segs =
         reinterpret_cast<const Segment *>(a.plan + seg_offset(p.ctas));

@@ -796,3 +796,48 @@ print("captured first")
     r = subprocess.run([sys.executable, "-c", code], cwd=root, text=True,
                        capture_output=True, timeout=120)
     assert "captured first" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("new,cached,heads", [
+    ([1, 1, 1], [700, 30, 5000], 8), ([64, 9], [2000, 0], 16),
+    ([900, 300], [0, 100], 4)])
+def test_calls_that_feed_each_other_without_a_wait(new, cached, heads):
+    # launches may start before the one in front has ended: each call reads
+    # what the one before it wrote, into the same buffers, with no other
+    # kernel between
+    c = Case(new, cached, heads, 2, 64, "bf16", seed=64)
+    plan, wplan = c.plan(), c.plan(kvattn.WeightsPlan)
+    a, b = c.q.contiguous().clone(), torch.empty_like(c.q.contiguous())
+    lse = torch.empty(sum(new), heads, device=DEV)
+    acc = torch.zeros(len(new), 2, wplan.max_keys, device=DEV)
+
+    def steps(wait):
+        for x, y in ((a, b), (b, a)) * 4:
+            kvattn.prompt_attention(plan, x, c.k, c.v, c.pages, c.table,
+                                    out=y, lse=lse)
+            wait()
+            kvattn.attention_weights(wplan, x, c.k, lse, c.pages[0], c.table,
+                                     add_to=acc, out=acc)
+            wait()
+            keep = kvattn.select_kept(acc, 3)
+            wait()
+        return [t.clone() for t in (a, b, lse, acc, keep)]
+
+    def reset():
+        a.copy_(c.q)
+        b.zero_()
+        acc.zero_()
+    reset()
+    want = steps(torch.cuda.synchronize)
+    for _ in range(5):
+        reset()
+        assert all(map(torch.equal, steps(lambda: None), want))
+    reset()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = steps(lambda: None)
+    for _ in range(3):
+        reset()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, got, want))
