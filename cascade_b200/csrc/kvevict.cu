@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512   ? 3
                                                          : 8)
     evict_select_kernel(const __grid_constant__ SelectArgs a) {
   constexpr int kWarps = kThreads / 32;
+  wait_for_previous();
   let_next_start();
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks();
@@ -370,13 +371,15 @@ extern "C" int cascade_kv_evict_select(
   cfg.gridDim = dim3((unsigned)(rows * ranks));
   cfg.blockDim = dim3(threads);
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   count_launches(1);
   return CASCADE_OK;
