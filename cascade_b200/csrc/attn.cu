@@ -157,8 +157,9 @@ __device__ __forceinline__ void give_back(float (&o)[kN], const KvSource &kv,
 // What bounds it (B200, D = 128).  Prompts: the chain of a row tile, softmax
 // (about 2100 cycles a tile, of which 1024 on the special-function unit) then
 // PV and QK (1040 cycles of MMA and 300 of hand-over), two chains at a time:
-// 16384 tokens of 64 heads take 3.8 to 4.0 ms, 1100 to 1150 TFLOP/s.  Decode:
-// HBM; 64 sequences of 4200 tokens read 1.12 GB in 197 us, 5.7 TB/s.
+// 16384 tokens of 64 heads take 3.7 to 4.0 ms, 1100 to 1190 TFLOP/s (4.4 ms in
+// a long run, under the power cap).  Decode: HBM; 64 sequences of 4200 tokens
+// read 1.12 GB in 183 to 193 us, 5.8 to 6.1 TB/s.
 template <int D, bool kBf16, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ FwdArgs a,
@@ -965,7 +966,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the partial results of items that several CTAs worked on: one warp
-// per row, weights exp(lse_p - max lse), in the order of the parts.
+// per row, weights exp(lse_p - max lse), in the order of the parts.  A few
+// megabytes, mostly in L2: about 4 us, bound by its launch and one round trip.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256)
     attn_merge_kernel(const __grid_constant__ FwdArgs a, const Merge *merges,
