@@ -966,8 +966,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the partial results of items that several CTAs worked on: one warp
-// per row, weights exp(lse_p - max lse), in the order of the parts.  A few
-// megabytes, mostly in L2: about 4 us, bound by its launch and one round trip.
+// per row, weights exp(lse_p - max lse), in the order of the parts.  It reads a
+// few megabytes, mostly from L2; launched early, it is there when the parts
+// are, so that what it costs is one round trip.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256)
     attn_merge_kernel(const __grid_constant__ FwdArgs a, const Merge *merges,
