@@ -1,5 +1,6 @@
 // Attention over KV caches: causal prompts and trees of drafted tokens, with
 // grouped heads, over cached tokens in pages followed by new packed tokens.
+#include <cfloat>
 #include <type_traits>
 
 #include "attn.cuh"
@@ -65,6 +66,9 @@ struct Shape {
   static_assert(kSlots <= kMaxSlots, "ring");
   static_assert(kSmem <= 232448, "shared memory of one SM");
 };
+
+// The lse of a part whose row saw keys, all of scores of -inf.
+constexpr float kNoWeight = -FLT_MAX;
 
 // First key tile of an item in which some row does not see every key.
 __device__ __forceinline__ int first_masked_tile(const Segment &s, int group,
@@ -429,11 +433,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const bool empty = lsum == 0.f;
         const float inv = empty ? 0.f : 1.f / lsum;
-        const float fill = part == 0 && empty && seen ? NAN : 0.f;
+        const float fill =
+            part == 0 && empty && seen && sg.part < 0 ? NAN : 0.f;
         f1 *= inv;
         f2 *= inv;
         if (!steps || empty) f1 = 0.f;
         if (!steps2 || empty) f2 = 0.f;
+        // A part of no weight is multiplied like the others: 0 * inf shows.
         // Each warpgroup joins half of the columns: [part][row][column],
         // 16-byte pieces permuted by the row so that lanes hit all banks.
         constexpr int kCols = D / 2, kPieces = kCols / 4;
@@ -450,21 +456,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_ld32(u, tm_o + w * kCols + col);
             tc_wait_ld();
             tc_hold(u);
-            if (f1 != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
-            }
+            for (int e = 0; e < 32; ++e)
+              o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
           }
           if (steps2) {
             tc_ld32(u, lane_base + 256 + (w ^ 1) * 128 + w * kCols + col);
             tc_wait_ld();
             tc_hold(u);
-            if (f2 != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
-            }
+            for (int e = 0; e < 32; ++e)
+              o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
           }
           if (row_on) {
 #pragma unroll
@@ -477,7 +479,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (row_on && part == 0 && w == 0) {
           const float lse =
-              empty ? -INFINITY : mm * a.scale + logf(lsum * kUnshift);
+              empty ? seen && sg.part >= 0 ? kNoWeight : -INFINITY
+                    : mm * a.scale + logf(lsum * kUnshift);
           if (sg.part >= 0)
             a.part_lse[(int64_t)sg.part * kTile + lane] = lse;
           else
@@ -560,9 +563,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const bool empty = lsum == 0.f;
         float inv = empty ? 0.f : 1.f / lsum;
-        const float fill = empty && seen ? NAN : 0.f;
+        const float fill = empty && seen && sg.part < 0 ? NAN : 0.f;
         const float lse =
-            empty ? -INFINITY : mm * a.scale + logf(lsum * kUnshift);
+            empty ? seen && sg.part >= 0 ? kNoWeight : -INFINITY
+                  : mm * a.scale + logf(lsum * kUnshift);
         f1 *= inv;
         f2 *= inv;
         if (!steps || empty) f1 = 0.f;
@@ -585,21 +589,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_ld16(u, tm_o + col);
             tc_wait_ld();
             tc_hold(u);
-            if (f1 != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
-            }
+            for (int e = 0; e < 16; ++e)
+              o[e] = fmaf(__uint_as_float(u[e]), f1, o[e]);
           }
           if (kDual && steps2) {
             tc_ld16(u, lane_base + 256 + (w ^ 1) * 128 + col);
             tc_wait_ld();
             tc_hold(u);
-            if (f2 != 0.f) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
-            }
+            for (int e = 0; e < 16; ++e)
+              o[e] = fmaf(__uint_as_float(u[e]), f2, o[e]);
           }
           if (row_on) {
             if (fix)
@@ -990,23 +990,24 @@ __global__ void __launch_bounds__(256)
   for (int p = 0; p < mg.parts; ++p) {
     const int64_t row = row0 + (int64_t)p * slot_rows;
     const float lse = a.part_lse[row];
-    // a part without weight counts only when no part has any (its value is
-    // then 0, or NaN where keys were seen but none had weight)
-    const float wgt = top == -INFINITY ? (lse == -INFINITY ? 1.f : lse)
-                                       : __expf(lse - top);
-    if (lse == -INFINITY && top != -INFINITY) continue;
-    if (top != -INFINITY || lse != lse) total += wgt;
+    // a part without weight is 0, or NaN where it saw values that are not
+    // finite, which stays
+    const float wgt = lse <= kNoWeight ? 0.f : __expf(lse - top);
+    total += wgt;
     const float *src = a.part_o + row * D + lane * kPer;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] = fmaf(src[e], wgt, acc[e]);
   }
-  const float inv = top == -INFINITY ? 1.f : 1.f / total;
+  // no part has any weight (a NaN is one): 0, or NaN where keys were seen
+  const bool none = total == 0.f;
+  const float inv = none ? 0.f : 1.f / total;
+  const float fill = none && top == kNoWeight ? NAN : 0.f;
   const int tok = (mg.row0 + r) / a.group;
   const int head = mg.hk * a.group + (mg.row0 + r) - tok * a.group;
   char *dst = a.out + (int64_t)(mg.tok0 + tok) * a.o_tok +
               (int64_t)head * a.o_head + lane * kPer * 2;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) acc[e] *= inv;
+  for (int e = 0; e < kPer; ++e) acc[e] = fmaf(acc[e], inv, fill);
   keep_finite<kBf16>(acc);
 #pragma unroll
   for (int e = 0; e < kPer; e += 2)
@@ -1014,8 +1015,7 @@ __global__ void __launch_bounds__(256)
         pack16<kBf16>(acc[e], acc[e + 1]);
   if (lane == 0)
     a.lse[(int64_t)(mg.tok0 + tok) * a.l_tok + (int64_t)head * a.l_head] =
-        top == -INFINITY ? (total != total ? NAN : -INFINITY)
-                         : top + logf(total);
+        none ? -INFINITY : top + logf(total);
 }
 
 template <int D, bool kBf16, int kForm>

@@ -1,0 +1,48 @@
+"""The attention operators over KV caches where their documentation makes a
+promise that ordinary inputs do not try: values that are not finite under
+weights of nothing, empty batches, captured and threaded calls."""
+import math
+
+import pytest
+import torch
+
+from cascade_b200 import kvattn
+from test_gpu_kvattn import Case
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def far_apart(heads, cached, low_key, low_score):
+    """One token, alike for all heads, whose cached keys score `low_score` or
+    100: low in every other tile of 128 keys, the poisoned key's among them.
+    The weight of a low key is exp(-200) or less, which is 0 in 32 bits."""
+    c = Case([1], [cached], heads, 1, 64, "fp16", seed=90)
+    c.q[:] = 0
+    c.q[..., 0] = 40.0                        # score = 40 k[0] / 8
+    for t in range(cached):
+        low = (t // 128) % 2 == (low_key // 128) % 2
+        c.pool[c.table[0, t // 16], 0, 0, t % 16, 0] = \
+            (low_score if low else 100.0) / 5.0
+    c.k[..., 0] = 20.0
+    return c
+
+
+@pytest.mark.parametrize("heads", [2, 32, 256])
+@pytest.mark.parametrize("cached", [700, 6000])
+@pytest.mark.parametrize("low_score", [-100.0, -math.inf])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("key", [5, 250])
+def test_bad_values_show_whatever_their_weight(heads, cached, low_score,
+                                               value, key):
+    # 0 * inf is NaN: a row that sees a value that is not finite is not
+    # finite, whichever part of the kernel the key falls to
+    c = far_apart(heads, cached, key, low_score)
+    clean, lse = c.run()
+    assert clean.isfinite().all()
+    c.pool[c.table[0, key // 16], 1, 0, key % 16, ::5] = value
+    out, lse2 = c.run()
+    assert torch.equal(lse, lse2)
+    assert not out[0, :, ::5].isfinite().any()
+    rest = torch.arange(64, device=DEV) % 5 != 0
+    assert torch.equal(out[0, :, rest], clean[0, :, rest])
