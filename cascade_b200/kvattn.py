@@ -202,9 +202,9 @@ def _rows(name, t, shape, dtype, device):
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be {dtype} on {device}; got {t.dtype} "
                          f"on {t.device}")
-    st = _strides(t)
-    if st[-1] not in (0, 1):
+    if st[-1] != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
+    st = _strides(t)
     if p % 16 or any(s % 8 for s in st[:-1]):
         raise ValueError(f"{name}: rows must start on 16-byte boundaries")
     return p, st

@@ -1,0 +1,29 @@
+"""What the operators over KV caches refuse before anything is launched, on a
+machine without a GPU."""
+import pytest
+import torch
+
+from cascade_b200 import kvattn
+
+CPU = torch.device("cpu")
+
+
+@pytest.mark.parametrize("t", [
+    torch.ones(1, dtype=torch.float16).expand(6, 4, 64),
+    torch.ones(6, 4, 8, dtype=torch.float16)[..., :1].expand(6, 4, 64),
+    torch.ones(64, 4, 6, dtype=torch.float16).permute(2, 1, 0),
+    torch.ones(6, 4, 128, dtype=torch.float16)[..., ::2]])
+def test_rows_must_be_contiguous(t):
+    # a row is read as 64 values in a row: an expanded one has only one
+    with pytest.raises(ValueError, match="contiguous"):
+        kvattn._rows("q", t, (6, 4, 64), torch.float16, CPU)
+
+
+@pytest.mark.parametrize("t,strides", [
+    (torch.ones(6, 4, 64, dtype=torch.float16), (256, 64, 1)),
+    (torch.ones(1, 1, 64, dtype=torch.float16).expand(6, 4, 64), (0, 0, 1)),
+    (torch.ones(6, 4, 72, dtype=torch.float16)[..., :64], (288, 72, 1)),
+    (torch.ones(0, 4, 64, dtype=torch.float16), (256, 64, 1))])
+def test_other_strides_are_taken(t, strides):
+    got = kvattn._rows("q", t, tuple(t.shape), torch.float16, CPU)
+    assert got == (t.data_ptr(), strides)
