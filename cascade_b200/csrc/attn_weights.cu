@@ -466,6 +466,8 @@ extern "C" int cascade_attn_weights(const cascade_attn_plan_info_t *plan,
            CASCADE_ERR_INVALID, "dtype must be FP16 or BF16");
   int rc = check_args(p, *args, false);
   if (rc != CASCADE_OK || p.segments == 0) return rc;
+  // no keys, and no positions behind them that are to be written
+  if (p.max_keys == 0 && (args->width == 0 || !args->fill)) return rc;
   CB_CHECK(args->weights && (p.tokens == 0 || args->lse),
            CASCADE_ERR_INVALID, "null pointer argument");
   CB_CHECK(args->width >= p.max_keys, CASCADE_ERR_INVALID,

@@ -46,3 +46,20 @@ def test_bad_values_show_whatever_their_weight(heads, cached, low_score,
     assert not out[0, :, ::5].isfinite().any()
     rest = torch.arange(64, device=DEV) % 5 != 0
     assert torch.equal(out[0, :, rest], clean[0, :, rest])
+
+
+@pytest.mark.parametrize("new", [[0], [0, 0, 0]])
+def test_weights_of_batches_without_tokens(new):
+    plan = kvattn.WeightsPlan(new, q_heads=4, kv_heads=2, head_dim=64,
+                              device=DEV)
+    q = torch.zeros(0, 4, 64, dtype=torch.float16, device=DEV)
+    k = torch.zeros(0, 2, 64, dtype=torch.float16, device=DEV)
+    lse = torch.zeros(0, 4, device=DEV)
+    assert kvattn.attention_weights(plan, q, k, lse).shape == (len(new), 2, 0)
+    # positions behind the sequences are there all the same
+    before = torch.rand(len(new), 2, 7, device=DEV)
+    got = kvattn.attention_weights(plan, q, k, lse, add_to=before)
+    assert torch.equal(got, before)
+    out = torch.full_like(before, 3.0)
+    kvattn.attention_weights(plan, q, k, lse, add_to=before, out=out)
+    assert (out == 3).all()

@@ -1,9 +1,12 @@
 """What the operators over KV caches refuse before anything is launched, on a
 machine without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
-from cascade_b200 import kvattn
+from cascade_b200 import _lib, kvattn
+from test_attn_plan import Args, make
 
 CPU = torch.device("cpu")
 
@@ -27,3 +30,13 @@ def test_rows_must_be_contiguous(t):
 def test_other_strides_are_taken(t, strides):
     got = kvattn._rows("q", t, tuple(t.shape), torch.float16, CPU)
     assert got == (t.data_ptr(), strides)
+
+
+@pytest.mark.parametrize("width,fill", [(0, 0), (0, 1), (9, 0)])
+def test_weights_without_keys_write_nothing(width, fill):
+    # an empty tensor has no address
+    info, _ = make(kvattn.WEIGHTS, [0, 0], [0, 0])
+    args = Args(scale=1.0, plan=4096, width=width, fill=fill,
+                weights=4096 if width else 0)
+    assert _lib.load().cascade_attn_weights(
+        ctypes.byref(info), args.pack(), None) == 0
