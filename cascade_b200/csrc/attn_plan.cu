@@ -33,7 +33,9 @@ int check_args(const cascade_attn_plan_info_t &p,
   CB_CHECK(p.tokens == 0 || (a.q && a.k && (a.v || !forward)),
            CASCADE_ERR_INVALID, "null pointer argument");
   if (p.max_cached > 0) {
-    CB_CHECK(a.k_pages && a.table && (a.v_pages || !forward) && a.pages >= 0,
+    // (no pages at all have no address)
+    CB_CHECK(a.table && a.pages >= 0 &&
+                 (a.pages == 0 || (a.k_pages && (a.v_pages || !forward))),
              CASCADE_ERR_INVALID, "cached tokens need pages and a table");
     bits |= (uintptr_t)a.k_pages;
     strides |= a.kp_page | a.kp_head | a.kp_tok;

@@ -63,3 +63,20 @@ def test_weights_of_batches_without_tokens(new):
     out = torch.full_like(before, 3.0)
     kvattn.attention_weights(plan, q, k, lse, add_to=before, out=out)
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("heads", [2, 32, 256])
+def test_no_pages_at_all(heads):
+    # a prefix of which the store held nothing: its tokens count as unseen
+    c = Case([3, 1], [300, 40], heads, 1, 64, "bf16", seed=91)
+    c.table[:] = 0
+    empty = c.pool[:0]
+    got, lse = kvattn.prompt_attention(
+        c.plan(), c.q, c.k, c.v, (empty[:, 0], empty[:, 1]), c.table)
+    c.table[:] = -1
+    want = c.run()
+    assert torch.equal(got, want[0]) and torch.equal(lse, want[1])
+    wplan = c.plan(kvattn.WeightsPlan)
+    assert torch.equal(
+        kvattn.attention_weights(wplan, c.q, c.k, lse, empty[:, 0], c.table),
+        kvattn.attention_weights(wplan, c.q, c.k, lse, c.pages[0], c.table))

@@ -40,3 +40,18 @@ def test_weights_without_keys_write_nothing(width, fill):
                 weights=4096 if width else 0)
     assert _lib.load().cascade_attn_weights(
         ctypes.byref(info), args.pack(), None) == 0
+
+
+@pytest.mark.parametrize("kind", [kvattn.FORWARD, kvattn.WEIGHTS])
+def test_no_pages_at_all_are_taken(kind):
+    # every table entry is then outside [0, 0); the call goes on to what it
+    # looks at next
+    info, _ = make(kind, [4], [10])
+    args = Args(scale=1.0, plan=4096, q=4096, k=4096, v=4096, table=4096)
+    call = (_lib.load().cascade_attn_forward if kind == kvattn.FORWARD
+            else _lib.load().cascade_attn_weights)
+    assert call(ctypes.byref(info), args.pack(), None) == 1
+    assert b"pages" not in _lib.load().cascade_last_error()
+    args.pages = 1
+    assert call(ctypes.byref(info), args.pack(), None) == 1
+    assert b"pages" in _lib.load().cascade_last_error()
