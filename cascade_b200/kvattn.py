@@ -113,10 +113,15 @@ class _Plan:
         if cached.size != new.size:
             raise ValueError("one cached length per sequence: "
                              f"{cached.size} for {new.size}")
+        page_size = page_size or 0
+        for name, n in (("q_heads", q_heads), ("kv_heads", kv_heads),
+                        ("head_dim", head_dim), ("page_size", page_size)):
+            if not 0 <= n < 1 << 31:
+                raise ValueError(f"{name} must be in [0, 2**31); got {n}")
         self.device = _cuda_device(device)
         info = _PlanInfo(
             kind=kind, batch=new.size, q_heads=q_heads, kv_heads=kv_heads,
-            head_dim=head_dim, page_size=page_size or 0, tree=int(tree),
+            head_dim=head_dim, page_size=page_size, tree=int(tree),
             window=window)
         with torch.cuda.device(self.device):
             buf = np.empty(4096, np.int32)

@@ -55,3 +55,17 @@ def test_no_pages_at_all_are_taken(kind):
     args.pages = 1
     assert call(ctypes.byref(info), args.pack(), None) == 1
     assert b"pages" in _lib.load().cascade_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(page_size=2 ** 32 + 16), dict(page_size=-16),
+    dict(q_heads=2 ** 32 + 4), dict(kv_heads=2 ** 32 + 2),
+    dict(head_dim=2 ** 32 + 64)])
+@pytest.mark.parametrize("cls", [kvattn.AttentionPlan, kvattn.WeightsPlan])
+def test_plan_sizes_beyond_32_bits(cls, kw):
+    # the C fields have 32 bits: 2^32 + 16 must not become 16
+    a = dict(q_heads=4, kv_heads=2, head_dim=64, page_size=16,
+             device="cuda:0")
+    a.update(kw)
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        cls([1], [1], **a)
