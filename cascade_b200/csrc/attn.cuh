@@ -526,10 +526,12 @@ __device__ __forceinline__ void fetch_new(uint32_t dst, const CUtensorMap *map,
 
 // The table's entry for cached token `key` of sequence b, and the page that
 // it names (-1: none).  Apart, so that an entry can be on its way while other
-// work is done: it is waited for where it is first looked at.
+// work is done: it is waited for where it is first looked at.  A plain load:
+// the non-coherent path is for memory that nothing writes during the kernel's
+// life, and an early launch may live beside the kernel that writes the table.
 __device__ __forceinline__ int table_entry(const KvSource &s, int b,
                                            int key) {
-  return __ldg(s.table + (int64_t)b * s.table_row + key / s.page);
+  return s.table[(int64_t)b * s.table_row + key / s.page];
 }
 __device__ __forceinline__ int page_named(const KvSource &s, int id) {
   return id >= 0 && id < s.pages ? id : -1;

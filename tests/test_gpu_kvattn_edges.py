@@ -80,3 +80,41 @@ def test_no_pages_at_all(heads):
     assert torch.equal(
         kvattn.attention_weights(wplan, c.q, c.k, lse, empty[:, 0], c.table),
         kvattn.attention_weights(wplan, c.q, c.k, lse, c.pages[0], c.table))
+
+
+@pytest.mark.parametrize("new,heads", [([1, 1, 1], 4), ([90, 3, 40], 4)])
+def test_a_page_table_that_the_call_before_writes(new, heads):
+    # the heaviest pages of each sequence, chosen on the device into the same
+    # tensor as the step before: the attention call may be launched while
+    # the choice still runs
+    pages, kept = 400, 60
+    c = Case(new, [kept * 16] * 3, heads, 2, 64, "bf16", seed=92)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    c.pool = torch.randn(pages, 2, 2, 16, 64, generator=g,
+                         device=DEV).bfloat16()
+    scores = torch.rand(6, 3, pages, generator=g, device=DEV)
+    plan, wplan = c.plan(), c.plan(kvattn.WeightsPlan)
+
+    def steps(wait):
+        outs = []
+        for s in scores:
+            table = kvattn.select_kept(s, kept)
+            wait()
+            out, lse = kvattn.prompt_attention(plan, c.q, c.k, c.v, c.pages,
+                                               table)
+            wait()
+            outs += [out, lse, kvattn.attention_weights(
+                wplan, c.q, c.k, lse, c.pages[0], table)]
+            wait()
+            del table             # the next choice is written to its memory
+        return outs
+    want = steps(torch.cuda.synchronize)
+    for _ in range(5):
+        assert all(map(torch.equal, steps(lambda: None), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = steps(lambda: None)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, got, want))
