@@ -210,13 +210,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = ct.tmem;
 
-  // The launch may be early: only the plan is sure to be there, all else may
-  // be what the kernel before this one writes.
+  // The launch may be early: what is in memory may be what the kernel before
+  // this one writes, the plan included.
+  wait_for_previous();
+  let_next_start();
   const Segment *segs =
       reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
   const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
-  wait_for_previous();
-  let_next_start();
 
   if (warp < 8) {
     // ------------------------------------------------------ softmax
@@ -973,8 +973,8 @@ template <int D, bool kBf16>
 __global__ void __launch_bounds__(256)
     attn_merge_kernel(const __grid_constant__ FwdArgs a, const Merge *merges,
                       int slot_rows) {
-  const Merge mg = merges[blockIdx.y];   // the plan is not the kernel's
   wait_for_previous();
+  const Merge mg = merges[blockIdx.y];
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (r >= mg.rows) return;
@@ -1037,7 +1037,7 @@ int run_fwd(const FwdArgs &a, const TileMaps &maps,
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
     once.set();
   }
-  // early: barriers, TMEM and the plan are set up while the kernel before ends
+  // early: barriers and TMEM are set up while the kernel before ends
   // (8 prompts up to 1500 tokens: 135 us a pass against 139)
   CB_CUDA(launch_early(kernel, dim3(p.ctas), dim3(kThreads), Sh::kSmem, s, a,
                        maps));

@@ -112,13 +112,13 @@ __global__ void __launch_bounds__(kWThreads, 1)
   tc_fence_after();
   const uint32_t tmem = ct.tmem;
 
-  // The launch may be early: only the plan is sure to be there, all else may
-  // be what the kernel before this one writes.
+  // The launch may be early: what is in memory may be what the kernel before
+  // this one writes, the plan included.
+  wait_for_previous();
+  let_next_start();
   const Segment *segs =
       reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
   const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
-  wait_for_previous();
-  let_next_start();
 
   if (warp < 16) {
     // ---------------------------------------------------------- sums
@@ -402,8 +402,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
 __global__ void __launch_bounds__(kKeys)
     weights_merge_kernel(const __grid_constant__ WeightArgs a,
                          const Merge *merges) {
-  const Merge mg = merges[blockIdx.x];   // the plan is not the kernel's
   wait_for_previous();
+  const Merge mg = merges[blockIdx.x];
   const int key = mg.key0 + threadIdx.x;
   if (key >= mg.rows) return;
   float sum = 0.f;

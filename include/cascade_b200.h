@@ -199,7 +199,8 @@ typedef struct {
   int32_t pages;       /* pages there are */
   float scale;         /* of the scores, in [2^-64, 2^64] */
   int32_t add;         /* weights: add to `before` */
-  const int32_t *plan; /* device copy of the plan buffer */
+  const int32_t *plan; /* device copy of the plan buffer, read in the
+                          stream's order */
   const void *q, *k, *v;
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
   const void *k_pages, *v_pages;

@@ -118,3 +118,37 @@ def test_a_page_table_that_the_call_before_writes(new, heads):
         graph.replay()
         torch.cuda.synchronize()
         assert all(map(torch.equal, got, want))
+
+
+def test_a_plan_that_the_stream_writes_before_the_call():
+    # a caller of the C ABI may keep one device buffer for its plans and
+    # fill it by a kernel of the same stream right before the call
+    shapes = [([1, 1, 1], [700, 30, 5000]), ([64, 9, 1], [2000, 0, 3]),
+              ([300, 2, 17], [100, 9, 1000])]
+    cases = [Case(*s, 8, 2, 64, "bf16", seed=93) for s in shapes]
+    plans = [(c.plan(), c.plan(kvattn.WeightsPlan)) for c in cases]
+    assert any(p._info.merges for ps in plans for p in ps)
+    want = []
+    for c, (p, w) in zip(cases, plans):
+        out, lse = c.run(p)
+        want.append((out, lse, kvattn.attention_weights(
+            w, c.q, c.k, lse, c.pages[0], c.table)))
+    bufs = [[p._buf for p in ps] for ps in plans]
+    shared = torch.zeros(max(b.numel() for bs in bufs for b in bs),
+                         dtype=torch.int32, device=DEV)
+    for ps in plans:
+        for p in ps:
+            p._ptr = shared.data_ptr()
+
+    def write(b):
+        torch.bitwise_or(b, 0, out=shared[:b.numel()])
+    for _ in range(10):
+        for c, (p, w), (pb, wb), (o0, l0, w0) in zip(cases, plans, bufs,
+                                                     want):
+            write(pb)
+            out, lse = c.run(p)
+            write(wb)
+            got = kvattn.attention_weights(w, c.q, c.k, lse, c.pages[0],
+                                           c.table)
+            assert torch.equal(out, o0) and torch.equal(lse, l0)
+            assert torch.equal(got, w0)
