@@ -204,16 +204,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     ct.bad_v = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // The launch may be early: what is in memory may be what the kernel before
+  // this one writes, the plan included.  TMEM too is taken behind the wait:
+  // a block of that kernel that shares the SM may still have to get its own,
+  // and each would wait for the other.  The next kernel may start once it is
+  // taken.
+  wait_for_previous();
   if (warp == 12) tc_alloc(smem_u32(&ct.tmem), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ct.tmem;
-
-  // The launch may be early: what is in memory may be what the kernel before
-  // this one writes, the plan included.
-  wait_for_previous();
   let_next_start();
+  const uint32_t tmem = ct.tmem;
   const Segment *segs =
       reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
   const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];
@@ -1037,7 +1039,7 @@ int run_fwd(const FwdArgs &a, const TileMaps &maps,
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
     once.set();
   }
-  // early: barriers and TMEM are set up while the kernel before ends
+  // early: the blocks are there, barriers set, when the kernel before ends
   // (8 prompts up to 1500 tokens: 135 us a pass against 139)
   CB_CUDA(launch_early(kernel, dim3(p.ctas), dim3(kThreads), Sh::kSmem, s, a,
                        maps));

@@ -106,16 +106,18 @@ __global__ void __launch_bounds__(kWThreads, 1)
     ct.give_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // The launch may be early: what is in memory may be what the kernel before
+  // this one writes, the plan included.  TMEM too is taken behind the wait:
+  // a block of that kernel that shares the SM may still have to get its own,
+  // and each would wait for the other.  The next kernel may start once it is
+  // taken.
+  wait_for_previous();
   if (warp == 20) tc_alloc(smem_u32(&ct.tmem), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ct.tmem;
-
-  // The launch may be early: what is in memory may be what the kernel before
-  // this one writes, the plan included.
-  wait_for_previous();
   let_next_start();
+  const uint32_t tmem = ct.tmem;
   const Segment *segs =
       reinterpret_cast<const Segment *>(a.plan + seg_offset(a.ctas));
   const int seg_begin = a.plan[blockIdx.x], seg_end = a.plan[blockIdx.x + 1];

@@ -1,6 +1,7 @@
 """What the operators over KV caches refuse before anything is launched, on a
 machine without a GPU."""
 import ctypes
+import os
 
 import pytest
 import torch
@@ -69,3 +70,20 @@ def test_plan_sizes_beyond_32_bits(cls, kw):
     a.update(kw)
     with pytest.raises(ValueError, match=next(iter(kw))):
         cls([1], [1], **a)
+
+
+@pytest.mark.parametrize("name", ["attn.cu", "attn_weights.cu"])
+def test_tensor_memory_is_taken_behind_the_wait(name):
+    # A block launched early that holds all of an SM's tensor memory while it
+    # waits for the kernel before, and a block of that kernel which has yet
+    # to get some, would wait for each other.  No test can run that, so the
+    # order is read from the source: wait, take, let the next start.
+    path = os.path.join(os.path.dirname(kvattn.__file__), "csrc", name)
+    with open(path) as f:
+        text = f.read()
+    assert text.count("tc_alloc(") == 1
+    at = text.index("tc_alloc(")
+    start = text.rindex("__global__", 0, at)
+    wait = text.index("wait_for_previous();", start)
+    sync = text.index("__syncthreads();", at)
+    assert wait < at < sync < text.index("let_next_start();", start)
