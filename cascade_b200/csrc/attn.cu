@@ -25,7 +25,7 @@ struct FwdArgs {
   int64_t mask_row;
   const int32_t *plan;
   float *part_o, *part_lse;        // [slot][row tile rows][D], [slot][rows]
-  int ctas, group, tree;
+  int ctas, group, tree, give_up;
   int out32;                       // rows of out are 32-byte aligned
   float scale, c;                  // c = scale * log2(e)
 };
@@ -39,7 +39,7 @@ struct Control {
   uint64_t done;
   alignas(16) uint32_t valid[8][4];  // which keys of a tile there are
   float2 ml[2][kTile];             // two key tiles: each chain's (max, sum)
-  uint32_t tmem;
+  uint32_t tmem, sent[4];          // the latter: items of each loader warp
   int give_up;
   int bad_v;                       // a masked tile held inf or NaN
 };
@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ct.o_full[w]), 1);
       mbar_init(smem_u32(&ct.turn[w]), 1);
     }
-    ct.give_up = 0;
+    ct.give_up = a.give_up;
+    if (a.give_up) atomicAdd(&g_timeouts, 1u);
     ct.bad_v = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float grow = 8.f / a.c;                  // allowed growth of m
     uint32_t s_phase = 0, o_phase = 0, o_phase2 = 0;
     int tiles_done = 0;
+    bool on = true;                      // no wait was let through
     for (int si = seg_begin; si < seg_end; ++si) {
       const Segment sg = segs[si];
       const int n_end = kDual ? sg.t1 : (w ? sg.n1 : sg.n0);
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       bool seen = false, first = true;
       for (int t = t_first; t < n_end; t += kDual ? 2 : 1) {
-        mbar_wait(smem_u32(&ct.s_full[w]), s_phase, give_up);
+        on = mbar_wait(smem_u32(&ct.s_full[w]), s_phase, give_up) && on;
         s_phase ^= 1;
         if constexpr (kFew) {
           // This warp's 32 of the tile's 128 keys.  Its rows of P are zero
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ct.p_full[w]));
+        if (lane == 0 && on) mbar_arrive(smem_u32(&ct.p_full[w]));
       }
       tiles_done += t_all - sg.t0;
 
@@ -706,8 +708,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     auto load_q = [&](const Segment &sg) {
-      mbar_wait(smem_u32(&ct.q_empty), q_phase, give_up);
-      __syncwarp();
+      if (!mbar_wait_warp(smem_u32(&ct.q_empty), q_phase, give_up))
+        return false;
       q_phase ^= 1;
       for (int qt = 0; qt < Sh::kQTiles; ++qt) {
         const int r = kFew ? lane : qt * kTile + lw * 32 + lane;
@@ -722,10 +724,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         copy_rows(sm_q + qt * Sh::kTileBytes, src);
       }
       publish(smem_u32(&ct.q_full));
+      return true;
     };
 
     uint32_t tile_no = 0;
-    for (int si = seg_begin; si < seg_end; ++si) {
+    bool on = true;                      // no wait was let through
+    for (int si = seg_begin; si < seg_end && on; ++si) {
       const Segment sg = segs[si];
       const int t_all = kDual ? sg.t1 : max(sg.n0, sg.n1);
       const int masked_from = first_masked_tile(sg, a.group, a.tree);
@@ -741,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the segment before is through with its own, they do not.
         if (t == (si == seg_begin ? sg.t0
                                   : min(sg.t0 + Sh::kAhead, t_all - 1)))
-          load_q(sg);
+          on = load_q(sg);
         const int key = t * kTile + lw * 32 + lane;
         const int page = page_named(a.kv, entry);
         const char *kp = nullptr, *vp = nullptr;
@@ -767,13 +771,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int tok = sg.tok0 + t * kTile - sg.cached + lw * 32;
         const int off = key % a.kv.page;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h, ++item) {        // K, V
+        for (int h = 0; h < 2 && on; ++h) {          // K, V
           const uint32_t slot = item % Sh::kSlots;
           const uint32_t ph = (item / Sh::kSlots) & 1;
           const uint32_t bar = smem_u32(&ct.full[slot]);
           const uint32_t dst = sm_ring + slot * Sh::kTileBytes;
-          mbar_wait(smem_u32(&ct.empty[slot]), ph ^ 1, give_up);
-          __syncwarp();
+          on = mbar_wait_warp(smem_u32(&ct.empty[slot]), ph ^ 1, give_up);
+          if (!on) break;
           if (h == 0 && lane == 0) ct.valid[tile_no & 7][lw] = there;
           if (by_page) {
             fetch_pages<D>(dst + lw * 32 * 128, maps, h ? &maps.vp : &maps.kp,
@@ -786,11 +790,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (h == 1 && t >= masked_from) check_finite(dst);
             publish(bar);
           }
+          ++item;
         }
+        if (!on) break;
         ++tile_no;
       }
     }
     cp_async_wait_all();
+    end_copies<Sh::kSlots>(ct.full, ct.sent, lw, item, 33);
   } else {
     // ------------------------------------------------------------ MMA
     // Two row tiles: one warp for each of the two chains S -> P -> O.  A
@@ -806,7 +813,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < (kDual ? 13 : 14)) {
       const int w = uniform(warp - 12);
-      const uint32_t issue = lane == 0;
+      // one lane issues, none once a wait was let through
+      uint32_t issue = lane == 0;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!mbar_wait_warp(bar, parity, give_up)) issue = 0;
+      };
       const uint32_t tm_s = uniform(tmem) + w * 128, tm_o = tm_s + 256;
       const uint32_t q = tile_desc(
           uniform(sm_q) + (kDual ? 0 : w * Sh::kTileBytes), 0);
@@ -816,8 +827,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t base = 0, q_phase = 0, p_phase = 0;
       uint32_t p_phases = 0;               // two key tiles: a bit a chain
       auto ready = [&](uint32_t bar, uint32_t parity) {
-        return __all_sync(0xffffffffu,
-                          mbar_test(bar, parity) || *give_up != 0);
+        if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+        if (!__any_sync(0xffffffffu, *give_up != 0)) return false;
+        issue = 0;
+        return true;
       };
       uint32_t turn_phase = w ^ 1;          // warp 0 has the first turn
       const int seg_last = uniform(seg_end);
@@ -828,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n1 = uniform(kDual ? sp->t1 : sp->n1);
         const int t_all = max(n0, n1), n_end = w ? n1 : n0;
         const int t_first = t0;
-        mbar_wait_warp(smem_u32(&ct.q_full), q_phase, give_up);
+        wait(smem_u32(&ct.q_full), q_phase);
         q_phase ^= 1;
         auto full = [&](uint32_t item) {
           return smem_u32(&ct.full[item % Sh::kSlots]);
@@ -888,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t_first < n_end) {
           const uint32_t item = base + 2 * (t_first - t0);
           const uint32_t slot = item % Sh::kSlots;
-          mbar_wait_warp(full(item), phase(item), give_up);
+          wait(full(item), phase(item));
           fence_async_proxy();
           mma_rows<0, D / 16>(tm_s, q,
                               tile_desc(ring + slot * Sh::kTileBytes, 0),
@@ -905,11 +918,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the turn on.
             for (int h = 0; h < 2; ++h) {
               const uint32_t item = base + 2 * (t - t0) + h;
-              mbar_wait_warp(full(item), phase(item), give_up);
+              wait(full(item), phase(item));
               if (issue)
                 mbar_arrive(smem_u32(&ct.empty[item % Sh::kSlots]));
             }
-            mbar_wait_warp(smem_u32(&ct.turn[w]), turn_phase, give_up);
+            wait(smem_u32(&ct.turn[w]), turn_phase);
             turn_phase ^= 1;
             pass_turn();
             continue;
@@ -919,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t slot = v_item % Sh::kSlots;
           const uint32_t k_slot = k_item % Sh::kSlots;
           const bool more = t + 1 < n_end;
-          mbar_wait_warp(full(v_item), phase(v_item), give_up);
+          wait(full(v_item), phase(v_item));
           const uint32_t v =
               tile_desc(ring + slot * Sh::kTileBytes, kTile * 128);
           const uint32_t k = tile_desc(ring + k_slot * Sh::kTileBytes, 0);
@@ -927,9 +940,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               more && __all_sync(0xffffffffu,
                                  mbar_try(full(k_item), phase(k_item)));
           fence_async_proxy();
-          mbar_wait_warp(smem_u32(&ct.p_full[w]), p_phase, give_up);
+          wait(smem_u32(&ct.p_full[w]), p_phase);
           p_phase ^= 1;
-          mbar_wait_warp(smem_u32(&ct.turn[w]), turn_phase, give_up);
+          wait(smem_u32(&ct.turn[w]), turn_phase);
           turn_phase ^= 1;
           tc_fence_after();
           mma_keys<0, kTile / 16>(tm_o, tm_s, v, id_pv, t != t_first, issue);
@@ -938,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!more) tc_commit(smem_u32(&ct.o_full[w]), issue);
             tc_commit(smem_u32(&ct.empty[slot]), issue);
             if (!more) continue;
-            mbar_wait_warp(full(k_item), phase(k_item), give_up);
+            wait(full(k_item), phase(k_item));
             fence_async_proxy();
           }
           mma_rows<0, D / 16>(tm_s, q, k, id_qk, issue);
@@ -953,9 +966,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         base += 2 * (t_all - t0);
       }
       // TMEM is freed only when no MMA is in flight.
-      tc_commit(smem_u32(&ct.done), issue);
-      int gave_up = 0;
-      mbar_wait_warp(smem_u32(&ct.done), 0, &gave_up);
+      tc_commit(smem_u32(&ct.done), lane == 0);
+      int ran_out = 0;
+      mbar_wait_warp(smem_u32(&ct.done), 0, &ran_out);
     }
     __syncwarp();
   }
@@ -1103,6 +1116,7 @@ extern "C" int cascade_attn_forward(const cascade_attn_plan_info_t *plan,
   a.ctas = p.ctas;
   a.group = p.q_heads / p.kv_heads;
   a.tree = p.tree;
+  a.give_up = diag_give_up();
   a.out32 = (((uintptr_t)args->out | (uint64_t)a.o_tok |
               (uint64_t)a.o_head) &
              31) == 0;

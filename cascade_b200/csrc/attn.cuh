@@ -91,24 +91,28 @@ static __device__ unsigned int g_timeouts;
 
 // A wait on another role of the same CTA.  Every role's loops are finite and
 // no address depends on data that a wait guards, so a wait that runs out
-// (four million tries, each of which may sleep; seconds in all) sets the
-// CTA's flag, lets every later wait of the CTA through, and the kernel ends
-// by itself.  Kept short: it is inlined at every wait.
-__device__ __forceinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity,
+// (four million tries, each of which sleeps up to 1.3 us; 5.6 s in all) sets
+// the CTA's flag and lets every later wait of the CTA through that is not over
+// by itself.  False where it let through: from its own first such wait on a
+// warp issues, sends, commits and arrives at nothing more, so that what still
+// passes between warps has truly been waited for.  (An arrival that a barrier
+// does not expect faults: 2 where 1 is pending.)  The kernel ends by itself,
+// its copies waited for (end_copies).  Kept short: it is inlined at every wait.
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity,
                                                volatile int *give_up) {
 #pragma unroll 1
   for (uint32_t n = 1; n < (1u << 22); ++n) {
-    if (mbar_try(bar, parity)) return;
-    if ((n & 255) == 0 && *give_up) return;
+    if (mbar_try(bar, parity)) return true;
+    if (*give_up) return false;
   }
   if (*give_up == 0) atomicAdd(&g_timeouts, 1u);
   *give_up = 1;
+  return false;
 }
 
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity,
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity,
                                           volatile int *give_up) {
-  if (mbar_try(bar, parity)) return;
-  mbar_wait_slow(bar, parity, give_up);
+  return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, give_up);
 }
 
 // For a loop that polls: gives up when it has had nothing to do for two
@@ -126,11 +130,38 @@ __device__ __forceinline__ void give_up_after(uint64_t *since,
 }
 
 // The same for a whole warp, which stays converged.
-__device__ __forceinline__ void mbar_wait_warp(uint32_t bar, uint32_t parity,
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity,
                                                volatile int *give_up) {
-  if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
-  mbar_wait_slow(bar, parity, give_up);
-  __syncwarp();
+  if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_slow(bar, parity, give_up));
+}
+
+// The end of the four loader warps, whatever happened: no copy may land in a
+// CTA that is gone.  Item i goes to slot i % slots and each warp makes
+// `arrivals` of the slot's barrier's for it; a warp that gave up has made
+// fewer items than the others.  It makes its arrivals for the rest without
+// copies, so that the last phase of every slot completes once all copies have
+// landed, and waits for that.  (At most one item a slot is missing: for a
+// second, the others would have had to see the first consumed.)
+template <int kSlots>
+__device__ __forceinline__ void end_copies(const uint64_t *full,
+                                           volatile uint32_t *sent, int lw,
+                                           uint32_t item, uint32_t arrivals) {
+  if ((threadIdx.x & 31) == 0) sent[lw] = item;
+  asm volatile("bar.sync 4, 128;" ::: "memory");
+  const uint32_t top =
+      max(max(sent[0], sent[1]), max(sent[2], sent[3]));
+#pragma unroll 1
+  for (uint32_t i = item; i < top; ++i)
+    if ((threadIdx.x & 31) == 0)
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(
+                       smem_u32(&full[i % kSlots])),
+                   "r"(arrivals)
+                   : "memory");
+  int ran_out = 0;
+#pragma unroll 1
+  for (uint32_t i = top > kSlots ? top - kSlots : 0; i < top; ++i)
+    mbar_wait_warp(smem_u32(&full[i % kSlots]), (i / kSlots) & 1, &ran_out);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src,
@@ -438,6 +469,10 @@ void fill_source(const cascade_attn_args_t &a,
                  const cascade_attn_plan_info_t &p, KvSource *s);
 
 unsigned int *weights_timeouts_symbol();
+
+// Set by cascade_diag_attn_give_up: 1 when this thread's calls are to start
+// with their CTAs' flag up.
+int diag_give_up();
 
 // Tensor maps for tiles that TMA can fetch: 64 columns of up to 32 rows of
 // one head, in the 128-byte swizzle.  A warp fetches its 32 rows of a tile

@@ -73,6 +73,14 @@ void fill_source(const cascade_attn_args_t &a,
 
 namespace {
 
+thread_local int give_up = 0;
+
+}  // namespace
+
+int diag_give_up() { return give_up; }
+
+namespace {
+
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
 
 EncodeTiled encode_tiled() {
@@ -540,6 +548,10 @@ extern "C" int cascade_attn_plan(cascade_attn_plan_info_t *info,
     cb::set_error("out of host memory for the plan");
     return CASCADE_ERR_NOMEM;
   }
+}
+
+extern "C" void cascade_diag_attn_give_up(int32_t on) {
+  cb::attn::give_up = on != 0;
 }
 
 extern "C" void cascade_attn_struct_sizes(size_t *plan_info, size_t *args) {

@@ -22,7 +22,7 @@ struct WeightArgs {
   int64_t o_seq, o_head;
   const int32_t *plan;
   float *part;                     // [slot][256]
-  int ctas, group, width, fill;
+  int ctas, group, width, fill, give_up;
   float c;                         // scale * log2(e)
 };
 
@@ -44,7 +44,7 @@ struct WControl {
   uint64_t q_full[kQSlots], q_empty[kQSlots];
   uint64_t s_full[2][2], s_empty[2][2];
   uint64_t done;
-  uint32_t tmem;
+  uint32_t tmem, sent[4];          // the latter: key tiles of each loader
   int give_up;
 };
 
@@ -103,7 +103,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
         mbar_init(smem_u32(&ct.s_empty[w][i]), 4);
       }
     mbar_init(smem_u32(&ct.done), 1);
-    ct.give_up = 0;
+    ct.give_up = a.give_up;
+    if (a.give_up) atomicAdd(&g_timeouts, 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // The launch may be early: what is in memory may be what the kernel before
@@ -131,6 +132,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
     const uint64_t c2 = pair_of(a.c, a.c);
     uint32_t step = 0, q_no = 0;
+    bool on = true;                      // no wait was let through
     for (int si = seg_begin; si < seg_end; ++si) {
       const Segment sg = segs[si];
       const int total = sg.cached + sg.n_new;
@@ -159,7 +161,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
           if ((step & 1) != buf) continue;
           const uint32_t slot = (q_no + ch - sg.t0) % kQSlots;
           const int n = min(kTile, sg.rows - ch * kTile);
-          mbar_wait(smem_u32(&ct.s_full[w][buf]), (step >> 1) & 1, give_up);
+          on = mbar_wait(smem_u32(&ct.s_full[w][buf]), (step >> 1) & 1,
+                         give_up) &&
+               on;
           tc_fence_after();
           const ulonglong2 *l4 =
               reinterpret_cast<const ulonglong2 *>(ct.lse2[slot]);
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
+          if (lane == 0 && on) {
             mbar_arrive(smem_u32(&ct.s_empty[w][buf]));
             // the chunk is done with after this warpgroup's last pair
             if (sg.n0 == 1)
@@ -275,9 +279,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
       const uint32_t slot = q_no % kQSlots;
       const char *src;
       const float l2 = row_at(sg, ch, &src);
-      mbar_wait(smem_u32(&ct.q_empty[slot]), ((q_no / kQSlots) & 1) ^ 1,
-                give_up);
-      __syncwarp();
+      if (!mbar_wait_warp(smem_u32(&ct.q_empty[slot]),
+                          ((q_no / kQSlots) & 1) ^ 1, give_up))
+        return false;
       ct.lse2[slot][lw * 32 + lane] = l2;
       // the MMA reads the rows up to the next multiple of 32
       if (ch * kTile + lw * 32 < sg.rows)
@@ -287,8 +291,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ct.q_full[slot]));
       ++q_no;
+      return true;
     };
-    for (int si = seg_begin; si < seg_end; ++si) {
+    bool on = true;                      // no wait was let through
+    for (int si = seg_begin; si < seg_end && on; ++si) {
       const Segment sg = segs[si];
       if (sg.t0 >= sg.t1) continue;
       const int total = sg.cached + sg.n_new;
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
       const int tiles = 2 * sg.n0;
       // the table is read two tiles ahead
       int entry[2] = {page_at(0), page_at(1)};
-      for (int tile = 0; tile < tiles; ++tile) {
+      for (int tile = 0; tile < tiles && on; ++tile) {
         const int key = sg.key0 + tile * kTile + lw * 32 + lane;
         const int page = page_named(a.kv, entry[0]);
         const char *kp = nullptr;
@@ -319,9 +325,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
         entry[0] = entry[1];
         if (tile + 2 < tiles) entry[1] = page_at(tile + 2);
         const uint32_t slot = k_no % kKSlots;
-        mbar_wait(smem_u32(&ct.k_empty[slot]), ((k_no / kKSlots) & 1) ^ 1,
-                  give_up);
-        __syncwarp();
+        on = mbar_wait_warp(smem_u32(&ct.k_empty[slot]),
+                            ((k_no / kKSlots) & 1) ^ 1, give_up);
+        if (!on) break;
         const uint32_t bar = smem_u32(&ct.k_full[slot]);
         const uint32_t dst = sm_k + slot * kTileBytes;
         if (by_page) {
@@ -337,15 +343,20 @@ __global__ void __launch_bounds__(kWThreads, 1)
         ++k_no;
         // the first chunk goes behind the first pair: its slot may still
         // have to be freed, theirs are free already
-        if (tile == 1) load_chunk(sg, sg.t0);
+        if (tile == 1) on = load_chunk(sg, sg.t0);
       }
-      for (int ch = sg.t0 + 1; ch < sg.t1; ++ch) load_chunk(sg, ch);
+      for (int ch = sg.t0 + 1; ch < sg.t1 && on; ++ch) on = load_chunk(sg, ch);
     }
     cp_async_wait_all();
+    end_copies<kKSlots>(ct.k_full, ct.sent, lw, k_no, 32);
   } else {
     // ------------------------------------------------------------ MMA
     {
-      const uint32_t issue = lane == 0;
+      // one lane issues, none once a wait was let through
+      uint32_t issue = lane == 0;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!mbar_wait_warp(bar, parity, give_up)) issue = 0;
+      };
       const uint32_t tm = uniform(tmem), sk = uniform(sm_k);
       const uint32_t sq = uniform(sm_q);
       uint32_t k_no = 0, step = 0, q_no = 0;
@@ -362,17 +373,14 @@ __global__ void __launch_bounds__(kWThreads, 1)
             const uint32_t idesc = mma_idesc(kBf16, n, false);
             const uint32_t q = tile_desc(sq + slot * kTileBytes, 0);
             if (pair == 0)
-              mbar_wait_warp(smem_u32(&ct.q_full[slot]), (qi / kQSlots) & 1,
-                             give_up);
+              wait(smem_u32(&ct.q_full[slot]), (qi / kQSlots) & 1);
 #pragma unroll 1
             for (int w = 0; w < 2; ++w) {
               const uint32_t ks = (k_no + w) % kKSlots;
               if (ch == t0)
-                mbar_wait_warp(smem_u32(&ct.k_full[ks]),
-                               ((k_no + w) / kKSlots) & 1, give_up);
+                wait(smem_u32(&ct.k_full[ks]), ((k_no + w) / kKSlots) & 1);
               fence_async_proxy();
-              mbar_wait_warp(smem_u32(&ct.s_empty[w][buf]),
-                             ((step >> 1) & 1) ^ 1, give_up);
+              wait(smem_u32(&ct.s_empty[w][buf]), ((step >> 1) & 1) ^ 1);
               tc_fence_after();
               mma_rows<0, D / 16>(tm + w * 256 + buf * 128,
                                   tile_desc(sk + ks * kTileBytes, 0), q,
@@ -386,9 +394,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
         }
         q_no += t1 - t0;
       }
-      tc_commit(smem_u32(&ct.done), issue);
-      int gave_up = 0;
-      mbar_wait_warp(smem_u32(&ct.done), 0, &gave_up);
+      tc_commit(smem_u32(&ct.done), lane == 0);
+      int ran_out = 0;
+      mbar_wait_warp(smem_u32(&ct.done), 0, &ran_out);
     }
     __syncwarp();
   }
@@ -499,6 +507,7 @@ extern "C" int cascade_attn_weights(const cascade_attn_plan_info_t *plan,
   a.group = p.q_heads / p.kv_heads;
   a.width = args->width;
   a.fill = args->fill;
+  a.give_up = diag_give_up();
   a.c = args->scale * kLog2e;
   TileMaps maps;
   make_maps(*args, p, false, &maps);

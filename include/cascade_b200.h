@@ -279,6 +279,11 @@ int cascade_kv_evict_gather(const cascade_kv_tensor_t *src, uint32_t items,
  * library is broken).  Synchronous. */
 int cascade_diag_attn_timeouts(uint64_t *count);
 
+/* For tests: with `on`, the attention calls that this thread makes from now on
+ * behave as if a wait had run out in every block as it starts: any other that
+ * is not over at once is let through. */
+void cascade_diag_attn_give_up(int32_t on);
+
 /* n device-to-device block copies in one launch (the pool copy that
  * GPUBackend::put/get do with cudaMemcpyAsync, gpu_backend.cu:298-308,
  * 362-377). */

@@ -152,3 +152,58 @@ def test_a_plan_that_the_stream_writes_before_the_call():
                                            c.table)
             assert torch.equal(out, o0) and torch.equal(lse, l0)
             assert torch.equal(got, w0)
+
+
+GIVES_UP = """
+import ctypes, itertools, math, sys, torch
+sys.path.insert(0, "tests")
+from cascade_b200 import _lib, kvattn
+from test_gpu_kvattn import Case
+give_up = _lib.load().cascade_diag_attn_give_up
+give_up.argtypes, give_up.restype = [ctypes.c_int32], None
+
+def calls(c):
+    out, lse = c.run()
+    return out, lse, None if c.tree else kvattn.attention_weights(
+        c.plan(kvattn.WeightsPlan), c.q, c.k, c.run()[1], c.pages[0], c.table)
+
+def same(a, b):
+    return all(x is y or torch.equal(x, y) for x, y in zip(a, b))
+
+def run(new, cached, heads, dim, page, tree):
+    c = Case(new, cached, heads, 2, dim, "bf16", page=page, tree=tree, seed=94)
+    want = calls(c)
+    torch.cuda.synchronize()
+    for i in range(4):
+        before = kvattn.wait_timeouts()
+        give_up(1)
+        got = calls(c)
+        torch.cuda.synchronize()
+        assert kvattn.wait_timeouts() > before
+        give_up(0)
+        assert same(calls(c), want)
+        CHECK
+
+for form in (([1], [3000], 4), ([1, 1], [9000, 300], 64), ([130], [900], 4),
+             ([300, 20], [0, 4000], 16), ([5] * 90, [30] * 90, 4),
+             ([1] * 300, [70] * 300, 8)):
+    for dim, page, tree in itertools.product((64, 128), (16, 37), (False, True)):
+        run(*form, dim, page, tree)
+print("gave up and went on")
+"""
+
+
+def gives_up(check):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", GIVES_UP.replace(
+        "CHECK", check)], cwd=root, text=True, capture_output=True,
+        timeout=240)
+    assert "gave up and went on" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_after_one_that_gave_up():
+    # in a process of its own, since the others expect no wait to run out
+    gives_up("pass")
