@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto phase = [&](uint32_t item) { return (item / Sh::kSlots) & 1; };
         if constexpr (kDual) {
           int tq = t0, tp = t0;            // next S and next O product
-          uint64_t since = 0;
+          uint32_t rounds = 0;
           while (tp < t_all) {
             bool idle = true;
             const uint32_t k_item = base + 2 * (tq - t0);
@@ -888,9 +888,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               idle = false;
             }
             if (idle)
-              give_up_after(&since, give_up);
+              give_up_after(&rounds, give_up);
             else
-              since = 0;
+              rounds = 0;
           }
           base += 2 * (t_all - t0);
           continue;

@@ -115,14 +115,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity,
   return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, give_up);
 }
 
-// For a loop that polls: gives up when it has had nothing to do for two
-// seconds (`since` starts at 0 and is set back to 0 by progress).
-__device__ __forceinline__ void give_up_after(uint64_t *since,
+// For a loop that polls: gives up when it has had nothing to do for 2^25 rounds
+// (over a second; `rounds` starts at 0 and is set back to 0 by progress).  Counted,
+// as the waits are, and not timed: a process that does not get the GPU for a
+// while has waited for nothing.
+__device__ __forceinline__ void give_up_after(uint32_t *rounds,
                                               volatile int *give_up) {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  if (*since == 0) *since = t;
-  if (t - *since > 2000000000ull && *give_up == 0) {
+  if (++*rounds > (1u << 25) && *give_up == 0) {
     *give_up = 1;
     if ((threadIdx.x & 31) == 0) atomicAdd(&g_timeouts, 1u);
   }

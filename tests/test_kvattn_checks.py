@@ -87,3 +87,13 @@ def test_tensor_memory_is_taken_behind_the_wait(name):
     wait = text.index("wait_for_previous();", start)
     sync = text.index("__syncthreads();", at)
     assert wait < at < sync < text.index("let_next_start();", start)
+
+
+@pytest.mark.parametrize("name", ["attn.cu", "attn.cuh", "attn_weights.cu"])
+def test_waits_are_counted_not_timed(name):
+    # a process that another one keeps from the GPU for seconds has waited
+    # for nothing: no wait may give up by the clock
+    path = os.path.join(os.path.dirname(kvattn.__file__), "csrc", name)
+    with open(path) as f:
+        text = f.read()
+    assert not any(x in text for x in ("globaltimer", "clock64", "clock("))
