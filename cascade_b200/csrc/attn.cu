@@ -435,10 +435,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           o_phase2 ^= 1;
         }
         tc_fence_after();
+        // what a CTA that gave up computed is no result
+        if (*give_up) lsum = NAN;
         const bool empty = lsum == 0.f;
         const float inv = empty ? 0.f : 1.f / lsum;
         const float fill =
-            part == 0 && empty && seen && sg.part < 0 ? NAN : 0.f;
+            part == 0 && ((empty && seen && sg.part < 0) || lsum != lsum)
+                ? NAN : 0.f;
         f1 *= inv;
         f2 *= inv;
         if (!steps || empty) f1 = 0.f;
@@ -565,9 +568,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           f2 = m2 == -INFINITY ? (l2 == 0.f ? 0.f : l2) : ex2(m2 * a.c - mc);
           lsum = l * f1 + l2 * f2;
         }
+        // what a CTA that gave up computed is no result
+        if (*give_up) lsum = NAN;
         const bool empty = lsum == 0.f;
         float inv = empty ? 0.f : 1.f / lsum;
-        const float fill = empty && seen && sg.part < 0 ? NAN : 0.f;
+        const float fill =
+            (empty && seen && sg.part < 0) || lsum != lsum ? NAN : 0.f;
         const float lse =
             empty ? seen && sg.part >= 0 ? kNoWeight : -INFINITY
                   : mm * a.scale + logf(lsum * kUnshift);

@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         if (key >= total ||
             (key < sg.cached && page_named(a.kv, entry) < 0))
           sum = 0.f;
+        if (*give_up) sum = NAN;         // no result
         if (sg.part >= 0)
           a.part[(int64_t)sg.part * kKeys + kt] = sum;
         else if (key < total)

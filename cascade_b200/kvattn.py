@@ -29,7 +29,9 @@ tensors that require a gradient are refused while gradients are enabled.
 Work is enqueued on the current stream of the tensors' device.  A plan may be
 used on any stream, and in captured graphs for as long as it is kept alive;
 workspaces are allocated per call, so calls on several streams and graphs
-that overlap share nothing.
+that overlap share nothing.  Waits inside the attention kernels are bounded:
+results of a block whose wait ran out (which takes a broken device or library)
+are NaN, and wait_timeouts() counts them.
 """
 from __future__ import annotations
 
@@ -641,7 +643,8 @@ def evict_pages(k_pages, v_pages, page_table, lengths, weights, budget,
 
 def wait_timeouts() -> int:
     """Waits inside attention kernels that gave up on the current device
-    (0 unless something is broken).  Synchronises."""
+    (0 unless something is broken); the results of their blocks are NaN.
+    Synchronises."""
     n = _u64(0)
     check(_lib.load().cascade_diag_attn_timeouts(ctypes.byref(n)))
     return n.value

@@ -276,7 +276,7 @@ int cascade_kv_evict_gather(const cascade_kv_tensor_t *src, uint32_t items,
                             void *stream);
 
 /* Waits inside attention kernels that gave up (0 unless the hardware or the
- * library is broken).  Synchronous. */
+ * library is broken); the results of their blocks are NaN.  Synchronous. */
 int cascade_diag_attn_timeouts(uint64_t *count);
 
 /* For tests: with `on`, the attention calls that this thread makes from now on

@@ -207,3 +207,25 @@ def gives_up(check):
 def test_calls_after_one_that_gave_up():
     # in a process of its own, since the others expect no wait to run out
     gives_up("pass")
+
+
+def test_results_of_calls_that_gave_up_are_nan():
+    gives_up("""out, lse, w = got
+        assert out.isnan().all() and lse.isnan().all()
+        for b, n in enumerate(a + b for a, b in zip(new, cached)):
+            assert w is None or w[b, :, :n].isnan().all()
+            assert w is None or (w[b, :, n:] == 0).all()
+        rows = sum(new)          # nothing else is written
+        q, k, v = (torch.cat([t, t[:1]]) for t in (c.q, c.k, c.v))
+        o, l = torch.full_like(q, 7.0), torch.full((rows + 1, heads), 7.0,
+                                                   device=q.device)
+        give_up(1)
+        if tree:
+            kvattn.tree_attention(c.plan(), q, k, v, torch.cat(
+                [c.mask, c.mask[:1]]), c.pages, c.table, out=o, lse=l)
+        else:
+            kvattn.prompt_attention(c.plan(), q, k, v, c.pages, c.table,
+                                    out=o, lse=l)
+        give_up(0)
+        assert (o[rows:] == 7).all() and (l[rows:] == 7).all()
+        assert o[:rows].isnan().all() and l[:rows].isnan().all()""")
