@@ -1,6 +1,6 @@
-"""The attention operators over KV caches where their documentation makes a
-promise that ordinary inputs do not try: values that are not finite under
-weights of nothing, empty batches, captured and threaded calls."""
+"""The operators over KV caches where their documentation makes a promise that
+ordinary inputs do not try: values that are not finite under weights of
+nothing, empty batches, captured and threaded calls, blocks that give up."""
 import math
 
 import pytest
@@ -229,3 +229,68 @@ def test_results_of_calls_that_gave_up_are_nan():
         give_up(0)
         assert (o[rows:] == 7).all() and (l[rows:] == 7).all()
         assert o[:rows].isnan().all() and l[:rows].isnan().all()""")
+
+
+@pytest.mark.parametrize("new,cached,heads,kv_heads,page,tree", [
+    ([70, 30, 5], [0, 0, 0], 16, 4, 16, False),
+    ([1500, 700], [0, 0], 32, 8, 16, False),
+    ([400, 90], [9000, 40], 32, 8, 16, False),
+    ([1], [1000], 32, 8, 16, True), ([1] * 20, [3000] * 20, 32, 8, 37, True),
+    ([64, 64], [4096, 100], 64, 8, 16, True)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_equal_calls_have_equal_results(new, cached, heads, kv_heads, page,
+                                        tree, dtype):
+    # sums are taken in a fixed order, whatever the blocks' timing
+    c = Case(new, cached, heads, kv_heads, 128, dtype, page=page, tree=tree,
+             seed=95)
+    plan, wplan = c.plan(), c.plan(kvattn.WeightsPlan)
+
+    def calls():
+        out, lse = c.run(plan)
+        return out, lse, kvattn.attention_weights(
+            wplan, c.q, c.k, lse, c.pages[0], c.table)
+    want = calls()
+    for _ in range(10):
+        assert all(map(torch.equal, calls(), want))
+
+
+def test_every_thread_gets_its_results():
+    # errors of a thread are raised by result()
+    from concurrent.futures import ThreadPoolExecutor
+    cases = [Case([2, 40], [900, 10], 8, 2, 64, "bf16", seed=96 + i)
+             for i in range(4)]
+    plans = [(c.plan(), c.plan(kvattn.WeightsPlan)) for c in cases]
+
+    def calls(c, plan, wplan):
+        out, lse = c.run(plan)
+        w = kvattn.attention_weights(wplan, c.q, c.k, lse, c.pages[0],
+                                     c.table)
+        return out, lse, w, kvattn.select_kept(w, 9, 2, 1)
+    want = [calls(c, *p) for c, p in zip(cases, plans)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        done, s = 0, torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = calls(cases[i], *plans[i])
+                s.synchronize()
+                done += all(map(torch.equal, got, want[i]))
+        return done
+    with ThreadPoolExecutor(4) as pool:
+        assert [f.result() for f in
+                [pool.submit(work, i) for i in range(4)]] == [20] * 4
+
+
+@pytest.mark.parametrize("width", [8193, 20000, 32768])
+def test_select_many_rows_beyond_one_block_of_512(width):
+    # more rows than clusters for them: one block of 1024 a row, ties in it
+    g = torch.Generator(device=DEV).manual_seed(width)
+    w = torch.randn(400, width, generator=g, device=DEV).mul(50).round()
+    w[7] = 1.0
+    keep = kvattn.select_kept(w, 3001, 100, 4)
+    w[:, :4] = math.inf
+    w[:, width - 100:] = math.inf
+    want = w.sort(dim=1, descending=True, stable=True).indices[
+        :, :3001].sort(1).values
+    assert torch.equal(keep.long(), want)
