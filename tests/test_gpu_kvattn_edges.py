@@ -294,3 +294,43 @@ def test_select_many_rows_beyond_one_block_of_512(width):
     want = w.sort(dim=1, descending=True, stable=True).indices[
         :, :3001].sort(1).values
     assert torch.equal(keep.long(), want)
+
+
+@pytest.mark.parametrize("window", [None, 1])
+@pytest.mark.parametrize("heads", [2, 64])
+def test_weights_of_cached_tokens_alone(window, heads):
+    # sequences without new tokens keep what they had
+    for new, cached in (([0, 0], [300, 1]), ([0, 3], [1000, 40])):
+        c = Case(new, cached, heads, 2, 64, "fp16", seed=97)
+        plan = c.plan(kvattn.WeightsPlan, window=window)
+        lse = c.run()[1]
+        before = torch.rand(2, 2, plan.max_keys + 5, device=DEV)
+        got = kvattn.attention_weights(plan, c.q, c.k, lse, c.pages[0],
+                                       c.table, add_to=before)
+        assert torch.equal(got[0], before[0])
+        zero = kvattn.attention_weights(plan, c.q, c.k, lse, c.pages[0],
+                                        c.table)
+        assert (zero[0] == 0).all()
+
+
+def test_choices_and_evictions_of_nothing():
+    keep = kvattn.select_kept(torch.zeros(3, 2, 0, device=DEV), 4, 1, 1)
+    assert keep.shape == (3, 2, 4) and (keep == -1).all()
+    assert kvattn.select_kept(torch.zeros(0, 9, device=DEV), 4).shape == (0,
+                                                                          4)
+    kv = torch.zeros(1, 2, 0, 64, dtype=torch.float16, device=DEV)
+    got, keep = kvattn.evict_kv_caches([[(kv, kv)]], torch.zeros(
+        1, 2, 0, device=DEV), 5, 2, 1)
+    assert got.shape == (1, 1, 2, 2, 0, 64) and keep.shape == (1, 2, 0)
+    # no pages: every token of the choice is a row of zeros
+    pages = torch.zeros(0, 2, 16, 64, dtype=torch.float16, device=DEV)
+    w = torch.rand(3, 2, 40, device=DEV)
+    table = torch.zeros(3, 3, dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([40, 3, 0], dtype=torch.int32, device=DEV)
+    k, v, keep = kvattn.evict_pages(pages, pages, table, lengths, w, 5)
+    assert (k == 0).all() and (v == 0).all()
+    assert torch.equal((keep >= 0).sum(-1), torch.tensor(
+        [[5, 5], [3, 3], [0, 0]], device=DEV))
+    k, v, keep = kvattn.evict_pages(pages, pages, table[:0], lengths[:0],
+                                    w[:0], 5)
+    assert k.shape == (0, 2, 5, 64) and keep.shape == (0, 2, 5)
