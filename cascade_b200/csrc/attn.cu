@@ -161,9 +161,10 @@ __device__ __forceinline__ void give_back(float (&o)[kN], const KvSource &kv,
 // What bounds it (B200, D = 128).  Prompts: the chain of a row tile, softmax
 // (about 2100 cycles a tile, of which 1024 on the special-function unit) then
 // PV and QK (1040 cycles of MMA and 300 of hand-over), two chains at a time:
-// 16384 tokens of 64 heads take 3.7 to 4.0 ms, 1100 to 1190 TFLOP/s (4.4 ms in
-// a long run, under the power cap).  Decode: HBM; 64 sequences of 4200 tokens
-// read 1.12 GB in 183 to 193 us, 5.8 to 6.1 TB/s.
+// 16384 tokens of 64 heads take 3.8 ms in a run of ten calls, 1160 TFLOP/s, and
+// 4.3 to 4.4 ms, 1010 TFLOP/s, in a long run under the power cap.  Decode: HBM;
+// 64 sequences of 4200 tokens read 1.12 GB in 179 us a call on one cache over
+// and over, 6.2 TB/s, and in 198 to 214 us on caches that change.
 template <int D, bool kBf16, int kForm>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ FwdArgs a,
@@ -989,7 +990,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the partial results of items that several CTAs worked on: one warp
 // per row, weights exp(lse_p - max lse), in the order of the parts.  It reads a
 // few megabytes, mostly from L2; launched early, it is there when the parts
-// are, so that what it costs is one round trip.
+// are, so that what it costs is one round trip.  A part's weight is __expf's:
+// off by 2 + 1.2 |x| units in the last place (x = lse_p - max lse), so by less
+// than 2^-18 of a weight of e^-16 or more, and smaller ones count for less; an
+// output is rounded by 2^-11 or 2^-8.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256)
     attn_merge_kernel(const __grid_constant__ FwdArgs a, const Merge *merges,
@@ -1059,7 +1063,8 @@ int run_fwd(const FwdArgs &a, const TileMaps &maps,
     once.set();
   }
   // early: the blocks are there, barriers set, when the kernel before ends
-  // (8 prompts up to 1500 tokens: 135 us a pass against 139)
+  // (8 prompts up to 1500 tokens: 146.9 us a pass against 148.7; 8 trees of 64
+  // drafts 73.3 against 75.6)
   CB_CUDA(launch_early(kernel, dim3(p.ctas), dim3(kThreads), Sh::kSmem, s, a,
                        maps));
   count_launches(1);

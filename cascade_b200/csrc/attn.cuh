@@ -116,9 +116,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity,
 }
 
 // For a loop that polls: gives up when it has had nothing to do for 2^25 rounds
-// (over a second; `rounds` starts at 0 and is set back to 0 by progress).  Counted,
-// as the waits are, and not timed: a process that does not get the GPU for a
-// while has waited for nothing.
+// (over a second; `rounds` starts at 0 and is set back to 0 by progress).
+// Counted, as the waits are, and not timed: a process that does not get the
+// GPU for a while has waited for nothing.
 __device__ __forceinline__ void give_up_after(uint32_t *rounds,
                                               volatile int *give_up) {
   if (++*rounds > (1u << 25) && *give_up == 0) {
@@ -382,6 +382,11 @@ __device__ __forceinline__ void store32(void *dst, const uint32_t (&v)[8],
   }
 }
 
+// 2^x by the special-function unit: within 2 units in the last place (2^-22 of
+// the value), and results below 2^-126 are 0.  The rounding of a score of 16 to
+// FP32 alone moves its weight by as much.  One instruction a score: the
+// exponentials bound these kernels, and a polynomial of degree 5 on the FMA
+// pipe took as many cycles.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -476,8 +481,8 @@ int diag_give_up();
 // Tensor maps for tiles that TMA can fetch: 64 columns of up to 32 rows of
 // one head, in the 128-byte swizzle.  A warp fetches its 32 rows of a tile
 // with a few instructions, where cp.async takes 16 of each lane (a decode step
-// of 64 sequences: 201 us against 205; a prompt on stored pages: 199 against
-// 211).
+// of 64 sequences: 214 us against 253; prompts on stored pages: 205 against
+// 213).
 struct TileMaps {
   CUtensorMap kp, vp;              // [page][head][token of the page][d]
   CUtensorMap k, v;                // [token][head][d]

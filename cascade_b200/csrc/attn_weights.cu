@@ -68,9 +68,9 @@ static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
 //
 // What bounds it (B200, D = 128).  Whole prompts: one exponential per score,
 // the special-function unit is 70 % active; 8192 tokens of 32 heads over 8
-// take 343 to 375 us, of which the exponentials alone are 239.  Decode: HBM;
-// 32 sequences of 4200 tokens read 278 MB in 63 us, the launch, the first
-// loads and the last sums included.
+// take 344 us (369 to 380 in a long run under the power cap), of which the
+// exponentials alone are 239.  Decode: HBM; 32 sequences of 4200 tokens read
+// 278 MB in 64 us, the launch, the first loads and the last sums included.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kWThreads, 1)
     attn_weights_kernel(const __grid_constant__ WeightArgs a,

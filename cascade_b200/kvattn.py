@@ -20,14 +20,17 @@ count as unseen.  Query head h uses key/value head h // (q_heads //
 kv_heads).  Tensors are float16 or bfloat16, head_dim 64 or 128 and
 contiguous; other strides may be anything whose rows start on 16-byte
 boundaries (a slice of a fused projection, a [1, heads, seq, dim] cache
-permuted to [seq, heads, dim]).  Outputs share no memory with inputs, except
-where a call says so.  Rows of `out` that belong to no sequence are left as
-they were.  A value of V that is not finite leaves the rows that see it not
-finite, and the rows that do not see it alone.  There are no backward passes:
-tensors that require a gradient are refused while gradients are enabled.
+permuted to [seq, heads, dim]).  Pages have q's type; load_kv_pages returns
+float16, so a bfloat16 model converts what it loads.  Outputs share no memory
+with inputs, except where a call says so.  Rows of `out` that belong to no
+sequence are left as they were.  A value of V that is not finite leaves the
+rows that see it not finite, and the rows that do not see it alone.  There are
+no backward passes: tensors that require a gradient are refused while
+gradients are enabled.
 
 Work is enqueued on the current stream of the tensors' device.  A plan may be
-used on any stream, and in captured graphs for as long as it is kept alive;
+used on any stream, and in captured graphs for as long as it is kept alive
+(a replay has the lengths of the plan: the next decode step needs another);
 workspaces are allocated per call, so calls on several streams and graphs
 that overlap share nothing.  Waits inside the attention kernels are bounded:
 results of a block whose wait ran out (which takes a broken device or library)
@@ -468,7 +471,7 @@ def select_kept(weights, budget, recent=0, sink=0, lengths=None):
     """The tokens to keep: weights is float32 [sequences, ..., tokens] (up to
     three leading dimensions, contiguous rows).  Each row keeps its first
     `sink` and last `recent` tokens and those of the largest weights, ties to
-    the lowest position, `budget` in all; NaN ranks below every number.
+    the lowest position, `budget` in all; NaN ranks with minus infinity.
     lengths (int32 CUDA [sequences], clamped to the row) ends the rows of a
     sequence early.  Returns int32 [sequences, ..., budget], ascending; a row
     of fewer tokens than budget keeps all and ends in -1."""
