@@ -67,7 +67,7 @@ static_assert(weights_smem<128>() <= 232448, "shared memory of one SM");
 // number.  A chunk's sum is taken by itself before it joins the total.
 //
 // What bounds it (B200, D = 128).  Whole prompts: one exponential per score,
-// the special-function unit is 70 % active; 8192 tokens of 32 heads over 8
+// the special-function unit is 72 % active; 8192 tokens of 32 heads over 8
 // take 344 us (369 to 380 in a long run under the power cap), of which the
 // exponentials alone are 239.  Decode: HBM; 32 sequences of 4200 tokens read
 // 278 MB in 64 us, the launch, the first loads and the last sums included.
